@@ -483,6 +483,83 @@ int pkv_decode_layers(const pkv_layer_weights* layers, int32_t num_layers, const
                       int64_t rope_rows, float eps, void* workspace, size_t workspace_bytes,
                       int32_t* err_flag, void* stream);
 
+/*
+ * Attention of each sequence's newest tokens over its paged cache, the tokens
+ * of all sequences packed: row b owns q/out rows [q_starts[b], q_starts[b+1])
+ * (its T_b new tokens, any number from 0 up, in order; q_starts is device
+ * int32 [batch+1], ascending, within [0, num_tokens]) and sees its own
+ * kv_lens[b] cached positions.  With causal != 0 its token i sits at position
+ * kv_lens[b] - T_b + i (bottom-right, as pkv_paged_prefill) and sees the
+ * positions up to that one; else every token sees all kv_lens[b] positions.
+ * One call therefore covers decode rows (T_b = 1), checks of a few drafted
+ * tokens, suffixes after a shared prefix and chunks of long prompts, mixed.
+ *
+ * q, out: [num_tokens][Hq][128] bf16 (strides st, sh: multiples of 8, 16-byte
+ * aligned bases).  Query heads per KV head: 1 .. PKV_CHUNK_MAX_GROUP.
+ * max_kv_len >= max(kv_lens) sizes the launch (a captured launch passes its
+ * capacity; shorter rows cost nothing).  A token that sees no position is a
+ * NaN row, as 0/0 is everywhere in this library; a row with T_b = 0 writes
+ * nothing, and out rows that belong to no sequence are left as they were.
+ * workspace: >= pkv_chunk_workspace_size() bytes, 16-byte aligned, contents
+ * irrelevant before and after; calls that may overlap on the GPU need one
+ * each.
+ */
+#define PKV_CHUNK_MAX_GROUP 64
+
+size_t pkv_chunk_workspace_size(int32_t batch, int32_t num_tokens, int32_t num_q_heads,
+                                int32_t num_kv_heads, int32_t max_kv_len);
+
+int pkv_paged_chunk(const void* q, int64_t q_st, int64_t q_sh,
+                    const void* k_pool, const void* v_pool, int64_t num_slots,
+                    const int32_t* block_tables, int64_t table_pitch,
+                    const int32_t* seq_rows, const int32_t* q_starts, const int32_t* kv_lens,
+                    int32_t max_kv_len, int32_t batch, int32_t num_tokens,
+                    int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+                    int32_t causal, float sm_scale, void* out, int64_t o_st, int64_t o_sh,
+                    void* workspace, size_t workspace_bytes,
+                    int32_t* err_flag, void* stream);
+
+/*
+ * pkv_paged_chunk over the FP8 pool: blocks are read in place (no dense bf16
+ * copy), K and V as e4m3 * scale.
+ */
+int pkv_paged_chunk_fp8(const void* q, int64_t q_st, int64_t q_sh,
+                        const void* kv8_pool, int64_t num_blocks,
+                        const int32_t* block_tables, int64_t table_pitch,
+                        const int32_t* seq_rows, const int32_t* q_starts, const int32_t* kv_lens,
+                        int32_t max_kv_len, int32_t batch, int32_t num_tokens,
+                        int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+                        int32_t causal, float sm_scale, void* out, int64_t o_st, int64_t o_sh,
+                        void* workspace, size_t workspace_bytes,
+                        int32_t* err_flag, void* stream);
+
+/*
+ * Copy blocks of a pool to other blocks, in every plane: plane p's block
+ * dst[i] receives its block src[i], i < n (src, dst: device int32).  A plane
+ * is num_blocks blocks of block_bytes contiguous bytes, planes plane_stride
+ * bytes apart: the bf16 cache has 2 * layers planes (K and V) with
+ * block_bytes = 16 * Hkv * 256, the FP8 cache one per layer with
+ * block_bytes = Hkv * pkv_fp8_block_bytes().
+ * The pairs are copied in no order: dst entries must be distinct, and no dst
+ * may be the src of another pair (a src may repeat).  src[i] == dst[i] and
+ * src[i], dst[i] both negative (padding of a captured launch) copy nothing;
+ * any other id outside [0, num_blocks) sets PKV_DEVERR_BLOCK_ID and the pair
+ * is skipped.
+ */
+int pkv_copy_blocks(void* pool, int32_t num_planes, int64_t plane_stride, int64_t block_bytes,
+                    int32_t num_blocks, const int32_t* src, const int32_t* dst, int32_t n,
+                    int32_t* err_flag, void* stream);
+
+/*
+ * pkv_copy_blocks, and every entry of tables[table_rows][table_cols] (rows
+ * table_pitch apart) that names a src[i] is set to dst[i], in the same
+ * launch.  src must ascend strictly (entries are found by bisection).
+ */
+int pkv_move_blocks(void* pool, int32_t num_planes, int64_t plane_stride, int64_t block_bytes,
+                    int32_t num_blocks, const int32_t* src, const int32_t* dst, int32_t n,
+                    int32_t* tables, int32_t table_rows, int32_t table_cols, int64_t table_pitch,
+                    int32_t* err_flag, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

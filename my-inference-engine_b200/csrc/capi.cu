@@ -959,4 +959,128 @@ int pkv_decode_layers(const pkv_layer_weights* layers, int32_t num_layers, const
       pkv::launch_decode_layers(p, maps, pl, static_cast<cudaStream_t>(stream)), "decode_layers");
 }
 
+// ---------------------------------------------------------------- packed chunks
+size_t pkv_chunk_workspace_size(int32_t batch, int32_t num_tokens, int32_t num_q_heads,
+                                int32_t num_kv_heads, int32_t max_kv_len) {
+  if (batch <= 0 || num_tokens <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 ||
+      num_q_heads % num_kv_heads != 0 || num_q_heads / num_kv_heads > PKV_CHUNK_MAX_GROUP)
+    return 0;
+  return pkv::chunk_workspace_bytes(batch, num_tokens, num_q_heads, num_kv_heads, max_kv_len);
+}
+
+// What both pool formats check of a packed-chunk call; fills `a` but its pool.
+static int chunk_common(pkv::ChunkLaunch& a, const void* q, int64_t q_st, int64_t q_sh,
+                        const int32_t* block_tables, int64_t table_pitch, const int32_t* seq_rows,
+                        const int32_t* q_starts, const int32_t* kv_lens, int32_t max_kv_len,
+                        int32_t batch, int32_t num_tokens, int32_t num_q_heads,
+                        int32_t num_kv_heads, int32_t causal, float sm_scale, void* out,
+                        int64_t o_st, int64_t o_sh, void* workspace, size_t workspace_bytes,
+                        int32_t* err_flag, void* stream) {
+  if (num_q_heads / num_kv_heads > PKV_CHUNK_MAX_GROUP)
+    return fail(PKV_ERR_UNSUPPORTED, "at most %d query heads per KV head (got %d)",
+                PKV_CHUNK_MAX_GROUP, num_q_heads / num_kv_heads);
+  if (batch < 0 || num_tokens < 0 || max_kv_len < 0)
+    return fail(PKV_ERR_INVALID, "negative batch / num_tokens / max_kv_len");
+  if (batch == 0 || num_tokens == 0) return ok();
+  int st = check_qo(q, out, q_st, q_sh, 0, o_st, o_sh, 0);
+  if (st) return st;
+  if (!q_starts || !kv_lens) return fail(PKV_ERR_INVALID, "null q_starts or kv_lens");
+  if (!(sm_scale > 0.f) || !(sm_scale < INFINITY))
+    return fail(PKV_ERR_INVALID, "sm_scale must be positive and finite");
+  if (static_cast<int64_t>(num_tokens) * num_q_heads > (int64_t(1) << 30) ||
+      static_cast<int64_t>(batch) * num_kv_heads > (int64_t(1) << 24))
+    return fail(PKV_ERR_UNSUPPORTED, "too many rows or tokens for one launch");
+  const size_t need = pkv::chunk_workspace_bytes(batch, num_tokens, num_q_heads, num_kv_heads, max_kv_len);
+  if (need > 0) {
+    if (!workspace || workspace_bytes < need)
+      return fail(PKV_ERR_WORKSPACE, "paged_chunk needs %zu workspace bytes, got %zu", need,
+                  workspace ? workspace_bytes : (size_t)0);
+    if (!aligned16(workspace)) return fail(PKV_ERR_ALIGN, "workspace not 16-byte aligned");
+  }
+  a.q = q; a.q_st = q_st; a.q_sh = q_sh;
+  a.out = out; a.o_st = o_st; a.o_sh = o_sh;
+  a.tables = block_tables; a.pitch = table_pitch; a.rows = seq_rows;
+  a.q_starts = q_starts; a.kv_lens = kv_lens; a.max_kv_len = max_kv_len;
+  a.batch = batch; a.num_tokens = num_tokens;
+  a.num_q_heads = num_q_heads; a.num_kv_heads = num_kv_heads;
+  a.causal = causal; a.sm_scale = sm_scale;
+  a.workspace = workspace; a.workspace_bytes = workspace_bytes; a.err = err_flag;
+  return launch_status(pkv::launch_chunk(a, static_cast<cudaStream_t>(stream)), "paged_chunk");
+}
+
+int pkv_paged_chunk(const void* q, int64_t q_st, int64_t q_sh, const void* k_pool,
+                    const void* v_pool, int64_t num_slots, const int32_t* block_tables,
+                    int64_t table_pitch, const int32_t* seq_rows, const int32_t* q_starts,
+                    const int32_t* kv_lens, int32_t max_kv_len, int32_t batch, int32_t num_tokens,
+                    int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, int32_t causal,
+                    float sm_scale, void* out, int64_t o_st, int64_t o_sh, void* workspace,
+                    size_t workspace_bytes, int32_t* err_flag, void* stream) {
+  int st = check_heads(num_q_heads, num_kv_heads, head_dim);
+  if (st) return st;
+  if ((st = check_pool(k_pool, v_pool, num_slots, block_tables, table_pitch))) return st;
+  pkv::ChunkLaunch a{};
+  a.k_pool = k_pool; a.v_pool = v_pool;
+  a.num_blocks = static_cast<int32_t>(num_slots / 16);
+  return chunk_common(a, q, q_st, q_sh, block_tables, table_pitch, seq_rows, q_starts, kv_lens,
+                      max_kv_len, batch, num_tokens, num_q_heads, num_kv_heads, causal, sm_scale,
+                      out, o_st, o_sh, workspace, workspace_bytes, err_flag, stream);
+}
+
+int pkv_paged_chunk_fp8(const void* q, int64_t q_st, int64_t q_sh, const void* kv8_pool,
+                        int64_t num_blocks, const int32_t* block_tables, int64_t table_pitch,
+                        const int32_t* seq_rows, const int32_t* q_starts, const int32_t* kv_lens,
+                        int32_t max_kv_len, int32_t batch, int32_t num_tokens, int32_t num_q_heads,
+                        int32_t num_kv_heads, int32_t head_dim, int32_t causal, float sm_scale,
+                        void* out, int64_t o_st, int64_t o_sh, void* workspace,
+                        size_t workspace_bytes, int32_t* err_flag, void* stream) {
+  int st = check_heads(num_q_heads, num_kv_heads, head_dim);
+  if (st) return st;
+  if ((st = check_pool8(kv8_pool, num_blocks, block_tables, table_pitch))) return st;
+  pkv::ChunkLaunch a{};
+  a.kv8 = kv8_pool;
+  a.num_blocks = static_cast<int32_t>(num_blocks);
+  return chunk_common(a, q, q_st, q_sh, block_tables, table_pitch, seq_rows, q_starts, kv_lens,
+                      max_kv_len, batch, num_tokens, num_q_heads, num_kv_heads, causal, sm_scale,
+                      out, o_st, o_sh, workspace, workspace_bytes, err_flag, stream);
+}
+
+// ---------------------------------------------------------------- blocks
+static int check_pages(const void* pool, int32_t num_planes, int64_t plane_stride,
+                       int64_t block_bytes, int32_t num_blocks, const int32_t* src,
+                       const int32_t* dst, int32_t n) {
+  if (n < 0 || num_planes < 0) return fail(PKV_ERR_INVALID, "negative pair or plane count");
+  if (!pool || (n > 0 && (!src || !dst))) return fail(PKV_ERR_INVALID, "null pool, src or dst");
+  if (num_blocks <= 0 || block_bytes <= 0) return fail(PKV_ERR_INVALID, "empty pool");
+  if (block_bytes % 16 != 0 || plane_stride % 16 != 0 || !aligned16(pool))
+    return fail(PKV_ERR_ALIGN, "pool, block size and plane stride must be 16-byte aligned");
+  if (num_planes > 1 && plane_stride / num_blocks < block_bytes)
+    return fail(PKV_ERR_INVALID, "plane_stride smaller than a plane's blocks");
+  return PKV_OK;
+}
+
+int pkv_copy_blocks(void* pool, int32_t num_planes, int64_t plane_stride, int64_t block_bytes,
+                    int32_t num_blocks, const int32_t* src, const int32_t* dst, int32_t n,
+                    int32_t* err_flag, void* stream) {
+  int st = check_pages(pool, num_planes, plane_stride, block_bytes, num_blocks, src, dst, n);
+  if (st) return st;
+  if (n == 0 || num_planes == 0) return ok();
+  pkv::PageLaunch a{pool, num_planes, plane_stride, block_bytes, num_blocks, src, dst, n,
+                    nullptr, 0, 0, 0, err_flag};
+  return launch_status(pkv::launch_copy_blocks(a, static_cast<cudaStream_t>(stream)), "copy_blocks");
+}
+
+int pkv_move_blocks(void* pool, int32_t num_planes, int64_t plane_stride, int64_t block_bytes,
+                    int32_t num_blocks, const int32_t* src, const int32_t* dst, int32_t n,
+                    int32_t* tables, int32_t table_rows, int32_t table_cols, int64_t table_pitch,
+                    int32_t* err_flag, void* stream) {
+  int st = check_pages(pool, num_planes, plane_stride, block_bytes, num_blocks, src, dst, n);
+  if (st) return st;
+  if (!tables || table_rows < 0 || table_cols < 0 || table_pitch < table_cols)
+    return fail(PKV_ERR_INVALID, "null tables or bad table shape");
+  if (n == 0 || num_planes == 0) return ok();
+  pkv::PageLaunch a{pool, num_planes, plane_stride, block_bytes, num_blocks, src, dst, n,
+                    tables, table_pitch, table_rows, table_cols, err_flag};
+  return launch_status(pkv::launch_copy_blocks(a, static_cast<cudaStream_t>(stream)), "move_blocks");
+}
+
 }  // extern "C"

@@ -271,4 +271,47 @@ void carve_decode_layers(LayersParams& p, void* ws, int32_t rows, int32_t sms, i
 cudaError_t launch_decode_layers(const LayersParams& p, const LayersMaps& maps,
                                  const LayersPlan& pl, cudaStream_t stream);
 
+// Attention of packed new tokens over the paged cache (chunk.cu).
+struct ChunkLaunch {
+  const void* q;
+  int64_t q_st, q_sh;
+  void* out;
+  int64_t o_st, o_sh;
+  const void* k_pool;  // bf16 planes of the layer ...
+  const void* v_pool;
+  const void* kv8;     // ... or its FP8 chunks
+  int32_t num_blocks;
+  const int32_t* tables;
+  int64_t pitch;
+  const int32_t* rows;
+  const int32_t* q_starts;
+  const int32_t* kv_lens;
+  int32_t max_kv_len, batch, num_tokens, num_q_heads, num_kv_heads;
+  int32_t causal;
+  float sm_scale;
+  void* workspace;
+  size_t workspace_bytes;
+  int32_t* err;
+};
+size_t chunk_workspace_bytes(int32_t batch, int32_t num_tokens, int32_t num_q_heads,
+                             int32_t num_kv_heads, int32_t max_kv_len);
+cudaError_t launch_chunk(const ChunkLaunch& a, cudaStream_t stream);
+
+// Blocks copied to other blocks in every plane of a pool (pages.cu); with
+// tables, the entries naming a source are redirected too.
+struct PageLaunch {
+  void* pool;
+  int32_t num_planes;
+  int64_t plane_stride, block_bytes;  // bytes
+  int32_t num_blocks;
+  const int32_t* src;
+  const int32_t* dst;
+  int32_t n;
+  int32_t* tables;  // nullable
+  int64_t table_pitch;
+  int32_t table_rows, table_cols;
+  int32_t* err;
+};
+cudaError_t launch_copy_blocks(const PageLaunch& a, cudaStream_t stream);
+
 }  // namespace pkv

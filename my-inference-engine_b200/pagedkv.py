@@ -97,6 +97,20 @@ _SIGNATURES = {
         [_vp, _i64, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _i32, _i32,
          _i32, _i32, _i32, _i32, _i32, ctypes.c_float, _vp, _i64, _i64, _i64, _vp,
          ctypes.c_size_t, _vp, _vp], ctypes.c_int),
+    "pkv_chunk_workspace_size": ([_i32, _i32, _i32, _i32, _i32], ctypes.c_size_t),
+    "pkv_paged_chunk": (
+        [_vp, _i64, _i64, _vp, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32,
+         _i32, _i32, ctypes.c_float, _vp, _i64, _i64, _vp, ctypes.c_size_t, _vp, _vp],
+        ctypes.c_int),
+    "pkv_paged_chunk_fp8": (
+        [_vp, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32,
+         _i32, _i32, ctypes.c_float, _vp, _i64, _i64, _vp, ctypes.c_size_t, _vp, _vp],
+        ctypes.c_int),
+    "pkv_copy_blocks": (
+        [_vp, _i32, _i64, _i64, _i32, _vp, _vp, _i32, _vp, _vp], ctypes.c_int),
+    "pkv_move_blocks": (
+        [_vp, _i32, _i64, _i64, _i32, _vp, _vp, _i32, _vp, _i32, _i32, _i64, _vp, _vp],
+        ctypes.c_int),
 }
 
 _lib = None
@@ -491,6 +505,161 @@ def linear_rope_append(x: torch.Tensor, w_qkv: torch.Tensor, bias: torch.Tensor 
         _ptr(starts), _ptr(q_lens), B, Hq, num_kv_heads, T, D, _ptr(ws), ws.numel(), _ptr(err),
         _stream(x.device))
     _check(st, "pkv_linear_rope_append")
+
+
+# ---------------------------------------------------------------- packed chunks
+def _int32_vector(t: torch.Tensor, what: str, device: torch.device, n: int | None = None) -> None:
+    if t.dtype != torch.int32 or t.dim() != 1 or (n is not None and t.shape[0] != n):
+        raise ValueError(f"{what} must be an int32 vector{'' if n is None else f' of {n}'}, "
+                         f"got {t.dtype} {tuple(t.shape)}")
+    if t.device != device:
+        raise ValueError(f"{what} is on {t.device}, expected {device}")
+    if t.shape[0] > 1 and t.stride(0) != 1:
+        raise ValueError(f"{what} must be contiguous")
+
+
+def _check_err(err: torch.Tensor | None, device: torch.device) -> None:
+    if err is not None and (err.dtype != torch.int32 or err.device != device or err.numel() < 1):
+        raise ValueError(f"err must be an int32 tensor on {device}")
+
+
+def _check_tables(tables: torch.Tensor, device: torch.device) -> None:
+    if tables.dtype != torch.int32 or tables.dim() != 2 or tables.device != device:
+        raise ValueError(f"tables must be an int32 matrix on {device}, got {tables.dtype} "
+                         f"{tuple(tables.shape)} on {tables.device}")
+    if tables.shape[1] > 1 and tables.stride(1) != 1:
+        raise ValueError("table rows must be contiguous")
+
+
+def _chunk_args(q, tables, rows, q_starts, kv_lens, max_kv_len, out, num_kv_heads, err):
+    """Checks both packed-chunk calls share; returns (tokens, Hq, batch)."""
+    dev = q.device
+    if dev.type != "cuda":
+        raise ValueError("Expected CUDA tensors")
+    if q.dtype != torch.bfloat16 or q.dim() != 3 or q.shape[2] != HEAD_DIM:
+        raise ValueError(f"q must be bf16 [tokens, heads, {HEAD_DIM}], got {q.dtype} {tuple(q.shape)}")
+    if out.dtype != torch.bfloat16 or out.shape != q.shape or out.device != dev:
+        raise ValueError("out must match q in type, shape and device")
+    if q.numel() and (q.stride(2) != 1 or out.stride(2) != 1):
+        raise ValueError("q and out need a contiguous last dimension")
+    _int32_vector(kv_lens, "kv_lens", dev)
+    batch = kv_lens.shape[0]
+    _int32_vector(q_starts, "q_starts", dev, batch + 1)
+    if rows is not None:
+        _int32_vector(rows, "rows", dev, batch)
+    _check_tables(tables, dev)
+    if rows is None and tables.shape[0] < batch:
+        raise ValueError(f"{tables.shape[0]} table rows for {batch} sequences")
+    _check_err(err, dev)
+    if max_kv_len < 0:
+        raise ValueError("max_kv_len must not be negative")
+    return q.shape[0], q.shape[1], batch
+
+
+def _chunk_workspace(batch, tokens, hq, hkv, max_kv_len, device):
+    """Scratch of one packed-chunk call.  Taken from torch's allocator for
+    each call, not kept: calls on two streams, or two captured graphs, then
+    never share it."""
+    need = lib().pkv_chunk_workspace_size(batch, tokens, hq, hkv, max_kv_len)
+    return torch.empty(need, dtype=torch.uint8, device=device) if need else None
+
+
+def paged_chunk(q: torch.Tensor, k_plane: torch.Tensor, v_plane: torch.Tensor,
+                tables: torch.Tensor, rows: torch.Tensor | None, q_starts: torch.Tensor,
+                kv_lens: torch.Tensor, max_kv_len: int, out: torch.Tensor, causal: bool,
+                sm_scale: float, num_kv_heads: int, err: torch.Tensor | None = None) -> None:
+    """pkv_paged_chunk.  q, out: [tokens, Hq, 128] packed; q_starts int32
+    [B + 1]; the pool planes are [num_slots, Hkv, 128] bf16."""
+    N, Hq, B = _chunk_args(q, tables, rows, q_starts, kv_lens, max_kv_len, out, num_kv_heads, err)
+    for name, t in (("k_plane", k_plane), ("v_plane", v_plane)):
+        if (t.dtype != torch.bfloat16 or t.dim() != 3 or t.shape[1:] != (num_kv_heads, HEAD_DIM)
+                or not t.is_contiguous() or t.device != q.device):
+            raise ValueError(f"{name} must be contiguous bf16 [slots, {num_kv_heads}, {HEAD_DIM}] on "
+                             f"{q.device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    if k_plane.shape != v_plane.shape:
+        raise ValueError("k_plane and v_plane must have the same shape")
+    with torch.cuda.device(q.device):
+        ws = _chunk_workspace(B, N, Hq, num_kv_heads, max_kv_len, q.device)
+        st = lib().pkv_paged_chunk(
+            _ptr(q), q.stride(0), q.stride(1), _ptr(k_plane), _ptr(v_plane), k_plane.shape[0],
+            _ptr(tables), tables.stride(0), _ptr(rows), _ptr(q_starts), _ptr(kv_lens), max_kv_len,
+            B, N, Hq, num_kv_heads, HEAD_DIM, int(causal), sm_scale, _ptr(out), out.stride(0),
+            out.stride(1), _ptr(ws), ws.numel() if ws is not None else 0, _ptr(err),
+            _stream(q.device))
+    _check(st, "pkv_paged_chunk")
+
+
+def paged_chunk_fp8(q: torch.Tensor, pool8: torch.Tensor, tables: torch.Tensor,
+                    rows: torch.Tensor | None, q_starts: torch.Tensor, kv_lens: torch.Tensor,
+                    max_kv_len: int, out: torch.Tensor, causal: bool, sm_scale: float,
+                    err: torch.Tensor | None = None) -> None:
+    """pkv_paged_chunk_fp8.  q, out: [tokens, Hq, 128] packed; pool8 uint8
+    [blocks, Hkv, chunk]."""
+    Hkv = _check_pool8(pool8, q.device)
+    N, Hq, B = _chunk_args(q, tables, rows, q_starts, kv_lens, max_kv_len, out, Hkv, err)
+    with torch.cuda.device(q.device):
+        ws = _chunk_workspace(B, N, Hq, Hkv, max_kv_len, q.device)
+        st = lib().pkv_paged_chunk_fp8(
+            _ptr(q), q.stride(0), q.stride(1), _ptr(pool8), pool8.shape[0], _ptr(tables),
+            tables.stride(0), _ptr(rows), _ptr(q_starts), _ptr(kv_lens), max_kv_len, B, N, Hq,
+            Hkv, HEAD_DIM, int(causal), sm_scale, _ptr(out), out.stride(0), out.stride(1),
+            _ptr(ws), ws.numel() if ws is not None else 0, _ptr(err), _stream(q.device))
+    _check(st, "pkv_paged_chunk_fp8")
+
+
+def _check_pool8(pool8: torch.Tensor, device: torch.device) -> int:
+    if (pool8.dtype != torch.uint8 or pool8.dim() != 3 or pool8.shape[2] != fp8_block_bytes()
+            or not pool8.is_contiguous() or pool8.device != device):
+        raise ValueError(f"pool8 must be contiguous uint8 [blocks, Hkv, {fp8_block_bytes()}] on "
+                         f"{device}, got {pool8.dtype} {tuple(pool8.shape)} on {pool8.device}")
+    return pool8.shape[1]
+
+
+# ---------------------------------------------------------------- blocks
+def _page_args(pool: torch.Tensor, src: torch.Tensor, dst: torch.Tensor, err):
+    """(planes, plane bytes, block bytes, blocks, pairs) of a cache's bf16 `buf`
+    [.., slots, Hkv, 128] or FP8 `pool8` [.., blocks, Hkv, chunk]."""
+    if pool.device.type != "cuda":
+        raise ValueError("Expected CUDA tensors")
+    if pool.dim() < 3 or not pool.is_contiguous():
+        raise ValueError("the pool must be contiguous, with slots (or blocks), heads and one more dimension")
+    if pool.dtype == torch.bfloat16 and pool.shape[-1] == HEAD_DIM:
+        if pool.shape[-3] % BLOCK_TOKENS:
+            raise ValueError(f"{pool.shape[-3]} slots are not a multiple of {BLOCK_TOKENS}")
+        blocks, block_bytes = pool.shape[-3] // BLOCK_TOKENS, BLOCK_TOKENS * pool.shape[-2] * HEAD_DIM * 2
+    elif pool.dtype == torch.uint8 and pool.shape[-1] == fp8_block_bytes():
+        blocks, block_bytes = pool.shape[-3], pool.shape[-2] * pool.shape[-1]
+    else:
+        raise ValueError(f"not a bf16 or FP8 pool: {pool.dtype} {tuple(pool.shape)}")
+    _int32_vector(src, "src", pool.device)
+    _int32_vector(dst, "dst", pool.device, src.shape[0])
+    _check_err(err, pool.device)
+    return math.prod(pool.shape[:-3]), blocks * block_bytes, block_bytes, blocks, src.shape[0]
+
+
+def copy_blocks(pool: torch.Tensor, src: torch.Tensor, dst: torch.Tensor,
+                err: torch.Tensor | None = None) -> None:
+    """pkv_copy_blocks: block dst[i] of every plane of `pool` (a cache's whole
+    buf or pool8, or one layer of it) receives block src[i].  dst entries are
+    distinct and none is the src of another pair."""
+    planes, plane, block, blocks, n = _page_args(pool, src, dst, err)
+    with torch.cuda.device(pool.device):
+        st = lib().pkv_copy_blocks(_ptr(pool), planes, plane, block, blocks, _ptr(src), _ptr(dst), n,
+                                   _ptr(err), _stream(pool.device))
+    _check(st, "pkv_copy_blocks")
+
+
+def move_blocks(pool: torch.Tensor, src: torch.Tensor, dst: torch.Tensor, tables: torch.Tensor,
+                err: torch.Tensor | None = None) -> None:
+    """pkv_move_blocks: copy_blocks, and the entries of `tables` (int32
+    [rows, columns]) that name a src[i] become dst[i].  src ascends strictly."""
+    planes, plane, block, blocks, n = _page_args(pool, src, dst, err)
+    _check_tables(tables, pool.device)
+    with torch.cuda.device(pool.device):
+        st = lib().pkv_move_blocks(_ptr(pool), planes, plane, block, blocks, _ptr(src), _ptr(dst), n,
+                                   _ptr(tables), tables.shape[0], tables.shape[1], tables.stride(0),
+                                   _ptr(err), _stream(pool.device))
+    _check(st, "pkv_move_blocks")
 
 
 def default_scale(d: int = HEAD_DIM) -> float:

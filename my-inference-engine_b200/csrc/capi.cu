@@ -72,6 +72,26 @@ int encode_pool(CUtensorMap* m, const void* base, int64_t num_slots, int32_t hkv
   return PKV_OK;
 }
 
+// Pool plane as {64 dims, 8 tokens, 2 halves, slots / 8, heads}: one box
+// {64, 8, 2, 2, 1} is a 16-token block of a head, 4 KiB, and lands as 1 KiB
+// groups of 8 tokens x 64 dims (128B swizzle), halves 1 KiB and token groups
+// 2 KiB apart, so consecutive blocks continue one another.
+int encode_blocks(CUtensorMap* m, const void* base, int64_t num_slots, int32_t hkv) {
+  EncodeFn fn = encode_fn();
+  if (!fn) return fail(PKV_ERR_DRIVER, "cuTensorMapEncodeTiled entry point unavailable");
+  const cuuint64_t token = static_cast<cuuint64_t>(hkv) * 256;
+  cuuint64_t dims[5] = {64, 8, 2, static_cast<cuuint64_t>(num_slots / 8),
+                        static_cast<cuuint64_t>(hkv)};
+  cuuint64_t strides[4] = {token, 128, 8 * token, 256};
+  cuuint32_t box[5] = {64, 8, 2, 2, 1};
+  cuuint32_t es[5] = {1, 1, 1, 1, 1};
+  CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5, const_cast<void*>(base), dims, strides,
+                  box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(PKV_ERR_DRIVER, "block tensor map encode failed (%d)", (int)r);
+  return PKV_OK;
+}
+
 // Dense [B][Hkv][S][128] bf16 with element strides -> 4-D map, box {64,16,1,1}.
 int encode_dense(CUtensorMap* m, const void* base, int32_t B, int32_t hkv, int32_t S, int64_t sb,
                  int64_t sh, int64_t ss) {
@@ -1019,7 +1039,8 @@ int pkv_paged_chunk(const void* q, int64_t q_st, int64_t q_sh, const void* k_poo
   if (st) return st;
   if ((st = check_pool(k_pool, v_pool, num_slots, block_tables, table_pitch))) return st;
   pkv::ChunkLaunch a{};
-  a.k_pool = k_pool; a.v_pool = v_pool;
+  if ((st = encode_blocks(&a.kmap, k_pool, num_slots, num_kv_heads))) return st;
+  if ((st = encode_blocks(&a.vmap, v_pool, num_slots, num_kv_heads))) return st;
   a.num_blocks = static_cast<int32_t>(num_slots / 16);
   return chunk_common(a, q, q_st, q_sh, block_tables, table_pitch, seq_rows, q_starts, kv_lens,
                       max_kv_len, batch, num_tokens, num_q_heads, num_kv_heads, causal, sm_scale,

@@ -277,9 +277,8 @@ struct ChunkLaunch {
   int64_t q_st, q_sh;
   void* out;
   int64_t o_st, o_sh;
-  const void* k_pool;  // bf16 planes of the layer ...
-  const void* v_pool;
-  const void* kv8;     // ... or its FP8 chunks
+  CUtensorMap kmap, vmap;  // bf16 planes of the layer (5-D, box = one block of a head) ...
+  const void* kv8;         // ... or its FP8 chunks
   int32_t num_blocks;
   const int32_t* tables;
   int64_t pitch;

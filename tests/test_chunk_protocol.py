@@ -1,0 +1,459 @@
+"""The packed-chunk kernel's synchronisation protocol and work split
+(csrc/chunk.cu), modelled on the CPU.
+
+Protocol: the roles (copies, tensor issue, two Q writers of which one hands
+out the items, two slots of four softmax warps, FP8: four widening warps) run
+as generators under random scheduling; copies land in any order, tensor
+instructions and commits run in issue order, mbarriers have the hardware's
+phase parity.  Every read is checked for the tile it was meant for.
+
+Work split: the cut of the summed item costs into one range per CTA, restated
+in Python: every key tile of every item is worked exactly once, the parts of a
+cut item are the consecutive CTAs that the first one names, and no partial
+slot is used twice."""
+import random
+
+import pytest
+
+from test_prefill_protocol import Barrier, Race
+
+RING = 3
+
+
+def run_kernel(items, seed, fp8, stages=None, scales=4, merge_wait=True, always_commit=False):
+    """items: [(two, nt)].  Raises Race on a wrong read, a lost update or a hang."""
+    rng = random.Random(seed)
+    stages = stages or (4 if fp8 else 5)
+    raws = 13
+    B = {"q_full": Barrier(2), "q_free": Barrier(1), "ml": Barrier(8), "ep": Barrier(8)}
+    for i in range(RING):
+        B[f"item_full{i}"], B[f"item_empty{i}"] = Barrier(1), Barrier(15 if fp8 else 11)
+    for i in range(stages):
+        B[f"kv_full{i}"], B[f"kv_empty{i}"] = Barrier(4 if fp8 else 1), Barrier(1)
+    for s in range(2):
+        B[f"s_full{s}"], B[f"p_full{s}"], B[f"o_full{s}"] = Barrier(1), Barrier(4), Barrier(1)
+    for i in range(raws):
+        B[f"raw_full{i}"], B[f"raw_empty{i}"] = Barrier(1), Barrier(4)
+    for i in range(4):
+        B[f"sc_full{i}"] = Barrier(4)
+    item_ring = [None] * RING
+    Q = [None, None]
+    kv = [[None] * 4 for _ in range(stages)]  # per widening warp; the copy engine writes all four
+    raw = [None] * raws
+    sc = [[None] * 4 for _ in range(scales)]
+    S = [[None] * 4 for _ in range(2)]
+    O = [set(), set()]
+    ml = [[None] * 4 for _ in range(2)]
+    tma, pipe, finished = [], [], []
+    STOP = (None, -1)
+
+    def wait(name, phase):
+        return lambda: B[name].test(phase & 1)
+
+    def need(ok, what):
+        if not ok:
+            raise Race(what)
+
+    def nxt(n):
+        yield wait(f"item_full{n % RING}", n // RING)
+        it = item_ring[n % RING]
+        need(it[0] == n, "item overwritten")
+        B[f"item_empty{n % RING}"].arrive()
+        return it[1]
+
+    def q_write(n, which, n_load):
+        if n_load:
+            yield wait("q_free", n_load - 1)
+        Q[which] = n
+        yield None
+        B["q_full"].arrive()
+
+    def items_role():
+        n_load = 0
+        for n, it in enumerate(list(items) + [STOP]):
+            if n >= RING:
+                yield wait(f"item_empty{n % RING}", n // RING - 1)
+            item_ring[n % RING] = (n, it)
+            B[f"item_full{n % RING}"].arrive()
+            yield None
+            if it[1] > 0:
+                yield from q_write(n, 1, n_load)
+                n_load += 1
+
+    def q_role():
+        n_load = 0
+        n = 0
+        while True:
+            it = yield from nxt(n)
+            if it[1] < 0:
+                return
+            if it[1]:
+                yield from q_write(n, 0, n_load)
+                n_load += 1
+            n += 1
+
+    def copy_role():
+        n = seq = 0
+        while True:
+            it = yield from nxt(n)
+            if it[1] < 0:
+                return
+            for j in range(it[1]):
+                if fp8:
+                    for b in range(8):
+                        st = seq % raws
+                        if seq >= raws:
+                            yield wait(f"raw_empty{st}", seq // raws - 1)
+                        B[f"raw_full{st}"].expect_tx(1)
+                        tma.append((raw, st, (n, j, b), f"raw_full{st}"))
+                        seq += 1
+                        yield None
+                else:
+                    for w in "KV":
+                        st = seq % stages
+                        if seq >= stages:
+                            yield wait(f"kv_empty{st}", seq // stages - 1)
+                        B[f"kv_full{st}"].expect_tx(1)
+                        tma.append((kv, st, [(w, n, j)] * 4, f"kv_full{st}"))
+                        seq += 1
+                        yield None
+            n += 1
+
+    def widen_role(w):
+        n = seq = r = key = 0
+        while True:
+            it = yield from nxt(n)
+            if it[1] < 0:
+                return
+            for j in range(it[1]):
+                for what in "KV":
+                    st = seq % stages
+                    if seq >= stages:
+                        yield wait(f"kv_empty{st}", seq // stages - 1)
+                    for b in range(8):
+                        rs = (r + b) % raws
+                        if what == "K":
+                            yield wait(f"raw_full{rs}", (r + b) // raws)
+                        need(raw[rs] == (n, j, b), "raw chunk")
+                        if what == "V":
+                            B[f"raw_empty{rs}"].arrive()
+                        if rng.random() < 0.2:
+                            yield None
+                    kv[st][w] = (what, n, j)
+                    if what == "K":
+                        sc[key % scales][w] = key
+                        yield None
+                        B[f"sc_full{key & 3}"].arrive()
+                        key += 1
+                    B[f"kv_full{st}"].arrive()
+                    seq += 1
+                    yield None
+                r += 8
+            n += 1
+
+    def mma():
+        n = seq = n_q = 0
+        n_p = [0, 0]
+        while True:
+            it = yield from nxt(n)
+            if it[1] < 0:
+                return
+            two, nt = it
+            if not nt:
+                n += 1
+                continue
+            yield wait("q_full", n_q)
+            n_q += 1
+
+            def qk(j, slot, last):
+                i = seq + 2 * j
+                yield wait(f"kv_full{i % stages}", i // stages)
+                pipe.append(("QK", n, j, slot, i % stages))
+                pipe.append(("commit", f"s_full{slot}"))
+                if last:
+                    pipe.append(("commit", f"kv_empty{i % stages}"))
+
+            def pv(j, slot, fresh, last):
+                i = seq + 2 * j + 1
+                yield wait(f"kv_full{i % stages}", i // stages)
+                yield wait(f"p_full{slot}", n_p[slot])
+                n_p[slot] += 1
+                pipe.append(("PV", n, j, slot, i % stages, fresh))
+                if last:
+                    pipe.append(("commit", f"kv_empty{i % stages}"))
+
+            if two:
+                yield from qk(0, 0, False)
+                yield from qk(0, 1, True)
+                if nt == 1:
+                    pipe.append(("commit", "q_free"))
+                for j in range(nt):
+                    for slot in range(2):
+                        yield from pv(j, slot, j == 0, slot == 1)
+                        if j + 1 < nt:
+                            yield from qk(j + 1, slot, slot == 1)
+                            if slot == 1 and j + 2 == nt:
+                                pipe.append(("commit", "q_free"))
+                        else:
+                            pipe.append(("commit", f"o_full{slot}"))
+            else:
+                yield from qk(0, 0, True)
+                if nt > 1:
+                    yield from qk(1, 1, True)
+                if nt <= 2:
+                    pipe.append(("commit", "q_free"))
+                for j in range(nt):
+                    yield from pv(j, j & 1, j < 2, True)
+                    if j + 2 < nt:
+                        yield from qk(j + 2, j & 1, True)
+                        if j + 3 == nt:
+                            pipe.append(("commit", "q_free"))
+                pipe.append(("commit", "o_full0"))
+                if nt > 1 or always_commit:
+                    pipe.append(("commit", "o_full1"))
+            seq += 2 * nt
+            n += 1
+
+    def softmax(slot, q):
+        n = n_tile = n_done = n_ml = n_key = 0
+        while True:
+            it = yield from nxt(n)
+            if it[1] < 0:
+                return
+            two, nt = it
+            if not nt:
+                n += 1
+                continue
+            mine = list(range(nt)) if two else list(range(slot, nt, 2))
+            for a, j in enumerate(mine):
+                yield wait(f"s_full{slot}", n_tile)
+                n_tile += 1
+                need(S[slot][q] == ("S", n, j), f"S {S[slot][q]} for {(n, j)}")
+                if fp8:
+                    yield wait(f"sc_full{(n_key + j) & 3}", (n_key + j) >> 2)
+                    need(all(v == n_key + j for v in sc[(n_key + j) % scales]), "scales")
+                if rng.random() < 0.5:
+                    yield None
+                if a and rng.random() < 0.5:  # rescales O
+                    need(O[slot] == {(n, i) for i in mine[:a]}, "O during a rescale")
+                if fp8:
+                    need(all(v == n_key + j for v in sc[(n_key + j) % scales]), "scales, second read")
+                S[slot][q] = ("P", n, j)
+                B[f"p_full{slot}"].arrive()
+            n_key += nt
+            if mine or always_commit:
+                yield wait(f"o_full{slot}", n_done)
+                n_done += 1
+            if two:
+                need(O[slot] == {(n, j) for j in mine}, "O at the end")
+            else:
+                ml[slot][q] = n
+                yield None
+                B["ml"].arrive()
+                yield wait("ml", n_ml)
+                need(ml[0][q] == n and ml[1][q] == n, "exchanged sums")
+                yield None
+                for s in range(2):
+                    if len(range(s, nt, 2)):
+                        need(O[s] == {(n, j) for j in range(s, nt, 2)}, "O of both slots at the end")
+                need(ml[0][q] == n and ml[1][q] == n, "exchanged sums, second read")
+                B["ep"].arrive()
+                if merge_wait:
+                    yield wait("ep", n_ml)
+                n_ml += 1
+            finished.append((n, slot, q))
+            n += 1
+
+    def pipe_step():
+        op = pipe.pop(0)
+        if op[0] == "commit":
+            B[op[1]].arrive()
+        elif op[0] == "QK":
+            _, n, j, slot, st = op
+            need(Q == [n, n], "Q tile")
+            need(all(v == ("K", n, j) for v in kv[st]), "K tile")
+            S[slot][:] = [("S", n, j)] * 4
+        else:
+            _, n, j, slot, st, fresh = op
+            need(S[slot] == [("P", n, j)] * 4, f"P {S[slot]}")
+            need(all(v == ("V", n, j) for v in kv[st]), "V tile")
+            if fresh:
+                O[slot].clear()
+            O[slot].add((n, j))
+
+    actors = [items_role(), q_role(), copy_role(), mma()]
+    actors += [softmax(s, q) for s in range(2) for q in range(4)]
+    if fp8:
+        actors += [widen_role(w) for w in range(4)]
+    live = {i: (a, None) for i, a in enumerate(actors)}
+    weight = [rng.choice([1, 1, 3, 10]) for _ in range(len(actors) + 2)]
+    while live or tma or pipe:
+        ready = [i for i, (_, p) in live.items() if p is None or p()]
+        ops = [(i, weight[i]) for i in ready]
+        if tma:
+            ops.append(("tma", weight[-1]))
+        if pipe:
+            ops.append(("pipe", weight[-2]))
+        if not ops:
+            raise Race("hang")
+        pick = rng.choices([o for o, _ in ops], [w for _, w in ops])[0]
+        if pick == "tma":
+            mem, at, val, bar = tma.pop(rng.randrange(len(tma)))
+            mem[at] = val
+            B[bar].complete_tx(1)
+        elif pick == "pipe":
+            pipe_step()
+        else:
+            a = live[pick][0]
+            try:
+                live[pick] = (a, next(a))
+            except StopIteration:
+                del live[pick]
+    assert len(finished) == 8 * sum(nt > 0 for _, nt in items)
+
+
+def some_items(rng, fp8):
+    return [(not fp8 and rng.random() < 0.5, rng.choice([0, 1, 1, 2, 3, 4, 5, 9])) for _ in range(rng.randint(1, 6))]
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+def test_protocol_under_random_timing(fp8):
+    for seed in range(250 if fp8 else 500):
+        run_kernel(some_items(random.Random(seed), fp8), seed, fp8)
+
+
+def test_the_model_sees_a_missing_wait():
+    """Without the wait after the slots' join, a slot's next P.V overwrites an O tile still being read."""
+    with pytest.raises(Race):
+        for seed in range(400):
+            run_kernel([(False, 2)] * 4, seed, False, merge_wait=False)
+
+
+def test_the_model_sees_an_unwatched_phase():
+    """A commit to the barrier of a slot that has no tile of the item can complete two phases unseen."""
+    with pytest.raises(Race):
+        for seed in range(800):
+            run_kernel([(True, 2), (False, 1), (True, 2), (False, 1)], seed, False, always_commit=True)
+
+
+def test_the_model_sees_too_few_scale_buffers():
+    with pytest.raises(Race):
+        for seed in range(300):
+            run_kernel([(False, 9)] * 2, seed, True, scales=2)
+
+
+# ---------------------------------------------------------------- work split
+ITEM, STEP, KEYS = 384, 384 + 4 * 128, 128
+
+
+class Split:
+    """struct Work and item_role of csrc/chunk.cu."""
+
+    def __init__(self, new, kv, group, hkv, fp8, causal):
+        self.new, self.kv, self.hkv, self.causal = new, kv, hkv, causal
+        self.tpt = 128 // group
+        self.wfull = 1 if fp8 else 2
+        self.block = self.tpt * self.wfull
+
+    def n(self, b):
+        return -(-self.new[b] // self.block)
+
+    def key_end(self, b, i):
+        if not self.causal:
+            return self.kv[b]
+        return max(0, self.kv[b] - self.new[b] + min(self.new[b], (i + 1) * self.block))
+
+    def weight(self, b, i):
+        return self.wfull if min(self.new[b] - i * self.block, self.block) > self.tpt else 1
+
+    def before(self, b, i):
+        if not self.causal:
+            keys = i * self.kv[b]
+        else:
+            a = self.kv[b] - self.new[b]
+            z = -a // self.block if a < 0 else 0
+            m = max(0, i - z)
+            keys = m * a + self.block * (m * (m + 1) // 2 + m * z)
+        return i * ITEM + keys * self.wfull
+
+    def cost(self, b, i):
+        return ITEM + self.weight(b, i) * self.key_end(b, i)
+
+    def head(self, b):
+        return self.before(b, self.n(b) - 1) + self.cost(b, self.n(b) - 1) if self.n(b) else 0
+
+    def ranges(self, ctas):
+        total = sum(self.head(b) * self.hkv for b in range(len(self.new)))
+        step = max(-(-total // ctas), STEP)
+        return step, [(c * step, min(total, (c + 1) * step)) for c in range(ctas)]
+
+    def cta(self, c, step, lo, hi):
+        base, out, desc = 0, [], None
+        for b in range(len(self.new)):
+            if base >= hi:
+                break
+            row_end = base + self.head(b) * self.hkv
+            for h in range(self.hkv):
+                for i in range(self.n(b)):
+                    s = base + h * self.head(b) + self.before(b, i)
+                    w, ke = self.weight(b, i), self.key_end(b, i)
+                    end, kt = s + ITEM + w * ke, -(-ke // KEYS)
+                    if s >= hi or end <= lo:
+                        continue
+
+                    def cut(at):
+                        d = at - s - ITEM
+                        return 0 if d <= 0 else min(kt, d // (w * KEYS))
+
+                    t0 = 0 if lo <= s else cut(lo)
+                    t1 = kt if hi >= end else cut(hi)
+                    if (lo > s) if kt == 0 else t0 >= t1:
+                        continue
+                    slot = -1 if t0 == 0 and t1 == kt else (1 if t0 == 0 else 0)
+                    if slot == 1:
+                        assert desc is None
+                        desc = ((b, h, i), (end - 1) // step - c + 1)
+                    out.append(((b, h, i), t0, t1, kt, slot))
+            base = row_end
+        return out, desc
+
+
+@pytest.mark.parametrize("seed", range(60))
+def test_every_key_tile_is_worked_once(seed):
+    rng = random.Random(seed)
+    group, fp8, causal = rng.choice([1, 4, 6, 7, 8, 64]), rng.random() < 0.5, rng.random() < 0.7
+    rows = rng.choice([1, 2, 5, 17])
+    new = [rng.choice([0, 1, 3, 21, 22, 43, 200, rng.randint(1, 600)]) for _ in range(rows)]
+    kv = [rng.choice([0, t, t + rng.randint(0, 3000), rng.randint(0, 400), t + 20000]) for t in new]
+    sp = Split(new, kv, group, rng.choice([1, 2, 8]), fp8, causal)
+    # the closed form of the summed costs is the sum
+    for b in range(rows):
+        at = 0
+        for i in range(sp.n(b)):
+            assert sp.before(b, i) == at
+            at += sp.cost(b, i)
+        assert sp.head(b) == at
+    ctas = rng.choice([2, 11, 148])
+    step, ranges = sp.ranges(ctas)
+    work, slots, descs = {}, {}, {}
+    for c, (lo, hi) in enumerate(ranges):
+        items, desc = sp.cta(c, step, lo, hi)
+        for key, t0, t1, kt, slot in items:
+            work.setdefault(key, []).append((t0, t1, kt, c, slot))
+            if slot >= 0:
+                assert (c, slot) not in slots
+                slots[c, slot] = key
+        if desc:
+            descs[desc[0]] = (c, desc[1])
+    for b in range(rows):
+        for h in range(sp.hkv):
+            for i in range(sp.n(b)):
+                parts = sorted(work[b, h, i])
+                assert parts[0][0] == 0 and parts[-1][1] == parts[0][2]
+                assert all(x[1] == y[0] for x, y in zip(parts, parts[1:]))
+                if len(parts) == 1:
+                    assert parts[0][4] == -1 and (b, h, i) not in descs
+                else:
+                    first, count = descs[b, h, i]
+                    assert [p[3] for p in parts] == list(range(first, first + count))
+                    assert [p[4] for p in parts] == [1] + [0] * (count - 1)

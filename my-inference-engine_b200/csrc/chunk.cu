@@ -21,23 +21,22 @@
 // replays for other lengths.
 //
 // CTA (one per SM), warps:
-//   0      K/V copies: one 5-D TMA box of 4 KiB per block for K and for V
-//          (FP8: one bulk copy of a block's chunk), through the block table
-//   1      owns TMEM, issues tcgen05.mma
-//   2, 3   write the next item's Q tile(s) to shared memory (FP8: as f16 of
-//          q / 16); warp 3 also walks the range and hands the items out
+//   0, 12  copies of K and of V, a 5-D TMA box of 4 KiB per block, through the
+//          block table (FP8: warp 0, one bulk copy of a block's chunk)
+//   1      owns TMEM, issues the Q.K's
+//   2      issues the P.V's
+//   3      walks the range and hands the items out
 //   4-7    softmax of slot A, 8-11 of slot B: a thread owns a tile row
-//   12-15  (FP8) widen e4m3 to f16 tiles (exact)
-// Two slots, each one S / P and one O tile in tensor memory, keep the tensor
-// cores busy while the other slot's softmax runs.  An item of more than 128
+//   13-15  write the items' Q tiles to shared memory
+//   12-15  (FP8) do so as f16 of q / 16, and widen e4m3 to f16 tiles (exact)
+// Two slots, each with a P and an O tile in tensor memory, share one S tile:
+// softmax warps take S into registers and free it at once, so the next Q.K
+// (the other slot's) runs under their exponentials.  An item of more than 128
 // rows gives each slot one of its two tiles (the K/V tiles are shared); a
 // smaller one gives the slots alternate key tiles and joins them at its end.
-// Order of the tensor instructions: P.V(j) of a slot, then Q.K(j + 1) of it;
-// one commit after Q.K therefore says that P.V(j) is done too, and O may be
-// rescaled without another wait.
 //
-// P takes S's columns as 16-bit pairs and is the A operand from tensor
-// memory.  bf16 pool: P in bf16.  FP8 pool: scores are scaled per key, and
+// P, as 16-bit pairs, is the A operand from tensor memory.
+//  bf16 pool: P in bf16.  FP8 pool: scores are scaled per key, and
 // the value scale goes into the exponent, p' = 2^(s + log2 vs - base), so
 // that P'V needs no scale; l sums p' / vs.  P' in f16 against base = max - 7
 // (at most 2^15 with the lazy maximum): 11 bits, and 2^-29 of the largest
@@ -63,30 +62,35 @@ constexpr float kP8Shift = 7.f;   // FP8: P' up to 2^(8 + 7)
 constexpr int kItemCost = 384;
 constexpr int kMinStep = kItemCost + 4 * kKeys;
 constexpr int kItemRing = 3;
+constexpr int kGroup = 4;  // FP8: blocks to a copy barrier
+// tensor memory columns: S, then each slot's P, then each slot's O
+constexpr uint32_t kColP = 128, kColO = 256;
 
 template <bool kFp8>
 struct Cfg {
-  static constexpr int kThreads = kFp8 ? 512 : 384;
+  static constexpr int kThreads = 512;
   static constexpr int kTiles = kFp8 ? 1 : 2;   // tiles of a full item
-  static constexpr int kStages = kFp8 ? 4 : 5;  // 32 KiB K or V tiles
-  static constexpr int kRaw = kFp8 ? 13 : 0;    // chunks in flight
+  // 32 KiB tiles; a ring each, so that no barrier is polled by two copiers of
+  // whom each sees every second phase only
+  static constexpr int kKStages = kFp8 ? 2 : 3, kVStages = 2;
+  static constexpr int kRaw = kFp8 ? 3 : 0;     // groups of kGroup chunks in flight
   static constexpr int kOffQ = 0;
-  static constexpr int kOffKV = kOffQ + kTiles * kOperand;
-  static constexpr int kOffRaw = kOffKV + kStages * kOperand;
-  static constexpr int kOffScale = kOffRaw + kRaw * kFp8HeadBlockBytes;  // [4][3][128]
+  static constexpr int kOffK = kOffQ + kTiles * kOperand;
+  static constexpr int kOffV = kOffK + kKStages * kOperand;
+  static constexpr int kOffRaw = kOffV + kVStages * kOperand;
+  static constexpr int kOffScale = kOffRaw + kRaw * kGroup * kFp8HeadBlockBytes;  // [4][3][128]
   static constexpr int kOffMl = kOffScale + (kFp8 ? 4 * 3 * kKeys * 4 : 0);  // [2][128] float2
   static constexpr int kOffItem = kOffMl + 2 * kRows * 8;
   static constexpr int kOffBar = kOffItem + kItemRing * 64;
-  static constexpr int kBars = 2 * kItemRing + 2 + 2 * kStages + 6 + 3 + 2 * kRaw + 4;
+  static constexpr int kBars = 2 * kItemRing + 2 + 2 * (kKStages + kVStages) + 7 + 3 + 2 * kRaw + 4;
   static constexpr int kOffScan = kOffBar + kBars * 8 + 16;  // 16 warp sums, base, row
   static constexpr int kSmem = kOffScan + 18 * 8;
-  // setmaxnreg: launch registers x threads covers the warpgroups' shares
-  static constexpr int kRegsLaunch = kFp8 ? 128 : 168;
-  static constexpr int kRegsLow = kFp8 ? 72 : 80;    // warps 0-3
-  static constexpr int kRegsConv = 72;               // warps 12-15
-  static constexpr int kRegsSoftmax = kFp8 ? 184 : 208;
-  static_assert(128 * kRegsLow + 256 * kRegsSoftmax + (kFp8 ? 128 * kRegsConv : 0) <=
-                    kRegsLaunch * kThreads,
+  // setmaxnreg: the warpgroups' shares of the launch's 128 per thread
+  static constexpr int kRegsLaunch = 128;
+  static constexpr int kRegsLow = 72;                // warps 0-3
+  static constexpr int kRegsSoftmax = kFp8 ? 184 : 200;
+  static constexpr int kRegsAux = kFp8 ? 72 : 40;    // warps 12-15
+  static_assert(kRegsLow + 2 * kRegsSoftmax + kRegsAux <= 4 * kRegsLaunch,
                 "register split exceeds the launch allocation");
   static_assert(kSmem <= 227 * 1024, "shared memory exceeds the per-CTA limit");
 };
@@ -176,16 +180,78 @@ struct __align__(16) Item {
 };
 static_assert(sizeof(Item) <= 64, "item ring");
 
-__device__ __forceinline__ uint64_t kmajor(uint32_t base, int kk) {
-  return sdesc(base + (kk >> 2) * kRegion + (kk & 3) * 32, 16, 1024);
-}
+// Shared-memory descriptors as (low word, high word): the high word is a
+// constant of the layout, the low word the start address and the leading
+// byte offset, both in 16-byte units, so a step along K is one addition.
+// K-major tiles (Q, FP8's K and V): 64-element regions of 128 rows, 8-row
+// groups 1 KiB apart; a step of 16 elements is 32 bytes, four per region.
 // bf16 tiles as the 5-D boxes land: block b's 8-token groups of 64 dims at
 // b * 4096 + group * 2048 + half * 1024 (128-byte rows, 128B swizzle).
-__device__ __forceinline__ uint64_t box_k(uint32_t base, int kk) {
-  return sdesc(base + (kk >> 2) * 1024 + (kk & 3) * 32, 16, 2048);
+constexpr uint32_t kDescHi = (1u << 14) | (2u << 29);  // version, 128B swizzle
+constexpr uint32_t kHiKMajor = kDescHi | (1024 >> 4);
+constexpr uint32_t kHiBoxK = kDescHi | (2048 >> 4);
+constexpr uint32_t kHiBoxV = kDescHi | (2048 >> 4);
+constexpr uint32_t kLoKMajor = 1u << 16;              // leading offset unused (16 bytes)
+constexpr uint32_t kLoBoxV = (1024u >> 4) << 16;      // 64-dim groups 1 KiB apart
+
+// Eight tensor instructions (K = 8 x 16) by a converged warp: elect.sync
+// inside the statement picks one lane, so control and operands stay uniform
+// for the compiler; a warp that shares its scheduler with two softmax warps
+// gets few issue slots, and every instruction between two tensor
+// instructions costs tens of cycles.  STEP4: from step 3 to step 4 of an
+// operand, in 16-byte units (steps within a half: STEP).
+#define PKV_MMA_STEP(a, da, b, db) "add.u32 " a ", " a ", " da ";\n\tadd.u32 " b ", " b ", " db ";\n\t"
+template <uint32_t kHiA, uint32_t kHiB, uint32_t kJumpA, uint32_t kJumpB, uint32_t kStepB>
+__device__ __forceinline__ void mma_ss8(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc) {
+#define PKV_SS(acc) \
+  "mov.b64 da, {la, %4};\n\tmov.b64 db, {lb, %5};\n\t" \
+  "@e tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, " acc ";\n\t"
+  asm volatile(
+      "{\n\t.reg .pred t, f, e;\n\t.reg .b32 la, lb;\n\t.reg .b64 da, db;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\tsetp.eq.u32 t, 0, 0;\n\tsetp.ne.u32 f, 0, 0;\n\t"
+      "mov.b32 la, %1;\n\tmov.b32 lb, %2;\n\t" PKV_SS("f") PKV_MMA_STEP("la", "2", "lb", "%8")
+          PKV_SS("t") PKV_MMA_STEP("la", "2", "lb", "%8") PKV_SS("t") PKV_MMA_STEP("la", "2", "lb", "%8")
+              PKV_SS("t") PKV_MMA_STEP("la", "%6", "lb", "%7") PKV_SS("t")
+                  PKV_MMA_STEP("la", "2", "lb", "%8") PKV_SS("t") PKV_MMA_STEP("la", "2", "lb", "%8")
+                      PKV_SS("t") PKV_MMA_STEP("la", "2", "lb", "%8") PKV_SS("t") "}" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "n"(kHiA), "n"(kHiB), "n"(kJumpA), "n"(kJumpB), "n"(kStepB)
+      : "memory");
+#undef PKV_SS
 }
-__device__ __forceinline__ uint64_t box_v(uint32_t base, int kb) {
-  return sdesc(base + kb * 4096, 1024, 2048);
+// A from tensor memory, 8 columns per step.
+template <uint32_t kHiB, uint32_t kJumpB, uint32_t kStepB>
+__device__ __forceinline__ void mma_ts8(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc,
+                                        uint32_t accumulate) {
+#define PKV_TS(acc) \
+  "mov.b64 db, {lb, %5};\n\t@e tcgen05.mma.cta_group::1.kind::f16 [%0], [la], db, %3, " acc ";\n\t"
+  asm volatile(
+      "{\n\t.reg .pred t, f, e;\n\t.reg .b32 la, lb;\n\t.reg .b64 db;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\tsetp.eq.u32 t, 0, 0;\n\tsetp.ne.u32 f, %4, 0;\n\t"
+      "mov.b32 la, %1;\n\tmov.b32 lb, %2;\n\t" PKV_TS("f") PKV_MMA_STEP("la", "8", "lb", "%7")
+          PKV_TS("t") PKV_MMA_STEP("la", "8", "lb", "%7") PKV_TS("t") PKV_MMA_STEP("la", "8", "lb", "%7")
+              PKV_TS("t") PKV_MMA_STEP("la", "8", "lb", "%6") PKV_TS("t")
+                  PKV_MMA_STEP("la", "8", "lb", "%7") PKV_TS("t") PKV_MMA_STEP("la", "8", "lb", "%7")
+                      PKV_TS("t") PKV_MMA_STEP("la", "8", "lb", "%7") PKV_TS("t") "}" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "n"(kHiB), "n"(kJumpB), "n"(kStepB)
+      : "memory");
+#undef PKV_TS
+}
+#undef PKV_MMA_STEP
+__device__ __forceinline__ void mma_ts1(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t b_hi,
+                                        uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, e;\n\t.reg .b64 db;\n\telect.sync _|e, 0xffffffff;\n\t"
+      "setp.ne.b32 p, %5, 0;\n\tmov.b64 db, {%2, %3};\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %4, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void mma_commit(uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+      "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(
+          smem_u32(bar))
+      : "memory");
 }
 
 __device__ __forceinline__ void tma_load_5d(void* dst, const CUtensorMap* map, uint64_t* bar,
@@ -205,12 +271,24 @@ __device__ __forceinline__ uint64_t now_ns() {
   return t;
 }
 
+// A place in a ring of N, and the phase of its barriers' use.
+template <int N>
+struct RingPos {
+  uint32_t st = 0, ph = 0;
+  __device__ void next() {
+    if (++st == N) {
+      st = 0;
+      ph ^= 1;
+    }
+  }
+};
+
 template <bool kFp8>
 struct Ctx {
   using C = Cfg<kFp8>;
   uint8_t* smem;
-  uint64_t *item_full, *item_empty, *q_full, *q_free, *kv_full, *kv_empty, *s_full, *p_full,
-      *o_full, *ml_bar, *ep_bar, *mma_done, *raw_full, *raw_empty, *sc_full;
+  uint64_t *item_full, *item_empty, *q_full, *q_free, *k_full, *k_empty, *v_full, *v_empty, *s_full, *s_free, *p_full,
+      *pv_done, *ml_bar, *ep_bar, *mma_done, *raw_full, *raw_empty, *sc_full;
   DevErr err;
 
   __device__ Ctx(uint8_t* s, int32_t* e) : smem(s), err{e} {
@@ -224,11 +302,14 @@ struct Ctx {
     item_empty = take(kItemRing);
     q_full = take(1);
     q_free = take(1);
-    kv_full = take(C::kStages);
-    kv_empty = take(C::kStages);
+    k_full = take(C::kKStages);
+    k_empty = take(C::kKStages);
+    v_full = take(C::kVStages);
+    v_empty = take(C::kVStages);
     s_full = take(2);
+    s_free = take(1);
     p_full = take(2);
-    o_full = take(2);
+    pv_done = take(2);
     ml_bar = take(1);
     ep_bar = take(1);
     mma_done = take(1);
@@ -253,58 +334,76 @@ struct Ctx {
     err.raise(PKV_DEVERR_TIMEOUT);
     return false;
   }
-  __device__ bool wait_warp(uint64_t* bar, uint32_t phase) const {
+  // A whole warp.
+  __device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t phase) const {
+    if (__all_sync(0xffffffffu, mbar_test(bar, phase & 1))) return true;
     return __all_sync(0xffffffffu, wait(bar, phase));
   }
   // Item n, read by a whole warp; false after a wait that ran out.
   __device__ bool next(int n, Item& it) const {
     if (!wait_warp(&item_full[n % kItemRing], n / kItemRing)) return false;
     it = *item(n);
-    __syncwarp();
+    // An arrive does not wait for loads in flight, so what they bring has to
+    // be used before it: here one word of each 16 bytes.
+    it.kvh = __shfl_sync(0xffffffffu, it.kvh, 0);
+    it.t1 = __shfl_sync(0xffffffffu, it.t1, 0);
+    it.slot = __shfl_sync(0xffffffffu, it.slot, 0);
     if ((threadIdx.x & 31) == 0) mbar_arrive(&item_empty[n % kItemRing]);
     return true;
   }
 };
 
 // ---------------------------------------------------------------- Q tiles
-// Warps 2 and 3: rows of the item, 16-byte chunk c of row r at chunk
-// c ^ (r & 7) of its 128-byte line (K-major, 128B swizzle).  Rows past the
-// item's are not written: they only reach their own rows of S and O.
-template <bool kFp8>
-__device__ void load_q(const ChunkParams& p, uint8_t* smem, const Item& it, int tpt, int thread) {
-  const int rows = it.ntok * p.group;
-  constexpr int kBatch = 8;
-  for (int base = 0; base < rows * 16; base += 64 * kBatch) {
+// The item's rows, 16-byte chunk c of row r at chunk c ^ (r & 7) of its
+// 128-byte line (K-major, 128B swizzle).  Rows past the item's are not
+// written: they only reach their own rows of S and O.
+struct QRows {
+  int rows, per_tile;  // rows of the item and of a full tile
+  __device__ const __nv_bfloat16* src(const ChunkParams& p, const Item& it, int i) const {
+    const int r = i >> 4, tok = r / p.group, head = it.kvh * p.group + r - tok * p.group;
+    return p.q + (it.first + tok) * p.q_st + head * p.q_sh + (i & 15) * 8;
+  }
+  __device__ uint32_t dst(int i) const {
+    int r = i >> 4;
+    const int c = i & 15;
+    const uint32_t tile = r >= per_tile ? kOperand : 0;
+    if (tile) r -= per_tile;
+    return tile + (c >> 3) * kRegion + swz128(r, c & 7);
+  }
+};
+
+// bf16 pool: three warps, asynchronous copies, all in flight at once.
+__device__ void load_q(const ChunkParams& p, uint8_t* tiles, const Item& it, int tpt, int thread) {
+  const QRows q{it.ntok * p.group, tpt * p.group};
+  for (int i = thread; i < q.rows * 16; i += 96)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(tiles) + q.dst(i)),
+                 "l"(q.src(p, it, i))
+                 : "memory");
+  asm volatile("cp.async.wait_all;" ::: "memory");
+}
+
+// FP8 pool: q / 16 as f16, 128 threads.  (1/16 keeps any |q| below 2^20 in
+// f16's range; it is exact from 2^-10 up, below that off by at most 2^-21.)
+__device__ void load_q_f16(const ChunkParams& p, uint8_t* tiles, const Item& it, int tpt,
+                           int thread) {
+  const QRows q{it.ntok * p.group, tpt * p.group};
+  constexpr int kBatch = 4;
+  for (int base = thread; base < q.rows * 16; base += 128 * kBatch) {
     uint4 v[kBatch];
 #pragma unroll
-    for (int k = 0; k < kBatch; ++k) {
-      const int i = base + k * 64 + thread;
-      if (i < rows * 16) {
-        const int r = i >> 4, tok = r / p.group, head = it.kvh * p.group + r - tok * p.group;
-        v[k] = *reinterpret_cast<const uint4*>(p.q + (it.first + tok) * p.q_st + head * p.q_sh +
-                                               (i & 15) * 8);
-      }
-    }
+    for (int k = 0; k < kBatch; ++k)
+      if (base + k * 128 < q.rows * 16)
+        v[k] = *reinterpret_cast<const uint4*>(q.src(p, it, base + k * 128));
 #pragma unroll
     for (int k = 0; k < kBatch; ++k) {
-      const int i = base + k * 64 + thread;
-      if (i < rows * 16) {
-        int r = i >> 4;
-        const int c = i & 15;
-        uint8_t* dst = smem + Cfg<kFp8>::kOffQ;
-        if (Cfg<kFp8>::kTiles == 2 && r >= tpt * p.group) {
-          r -= tpt * p.group;
-          dst += kOperand;
-        }
-        if constexpr (kFp8) {
-          uint32_t* w = reinterpret_cast<uint32_t*>(&v[k]);
+      if (base + k * 128 < q.rows * 16) {
+        uint32_t* w = reinterpret_cast<uint32_t*>(&v[k]);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float2 f = __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&w[e]));
-            w[e] = pack_f16(f.x * 0.0625f, f.y * 0.0625f);
-          }
+        for (int e = 0; e < 4; ++e) {
+          const float2 f = __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&w[e]));
+          w[e] = pack_f16(f.x * 0.0625f, f.y * 0.0625f);
         }
-        *reinterpret_cast<uint4*>(dst + (c >> 3) * kRegion + swz128(r, c & 7)) = v[k];
+        *reinterpret_cast<uint4*>(tiles + q.dst(base + k * 128)) = v[k];
       }
     }
   }
@@ -332,6 +431,33 @@ __device__ __forceinline__ void store_cols(const float (&v)[32], __nv_bfloat16* 
 }
 
 // ---------------------------------------------------------------- softmax
+// Two fp32 operations in one instruction (sm_100).
+__device__ __forceinline__ void fma2(float& x0, float& x1, float a0, float a1, float b0, float b1) {
+  asm("{\n\t.reg .b64 x, a, b;\n\tmov.b64 x, {%0, %1};\n\tmov.b64 a, {%2, %3};\n\t"
+      "mov.b64 b, {%4, %5};\n\tfma.rn.f32x2 x, x, a, b;\n\tmov.b64 {%0, %1}, x;\n\t}"
+      : "+f"(x0), "+f"(x1)
+      : "f"(a0), "f"(a1), "f"(b0), "f"(b1));
+}
+__device__ __forceinline__ void fma2_to(float& y0, float& y1, float a0, float a1, float b0,
+                                        float b1) {
+  asm("{\n\t.reg .b64 y, a, b;\n\tmov.b64 y, {%0, %1};\n\tmov.b64 a, {%2, %3};\n\t"
+      "mov.b64 b, {%4, %5};\n\tfma.rn.f32x2 y, a, b, y;\n\tmov.b64 {%0, %1}, y;\n\t}"
+      : "+f"(y0), "+f"(y1)
+      : "f"(a0), "f"(a1), "f"(b0), "f"(b1));
+}
+__device__ __forceinline__ void add2(float& x0, float& x1, float a0, float a1) {
+  asm("{\n\t.reg .b64 x, a;\n\tmov.b64 x, {%0, %1};\n\tmov.b64 a, {%2, %3};\n\t"
+      "add.rn.f32x2 x, x, a;\n\tmov.b64 {%0, %1}, x;\n\t}"
+      : "+f"(x0), "+f"(x1)
+      : "f"(a0), "f"(a1));
+}
+__device__ __forceinline__ void mul2(float& x0, float& x1, float a) {
+  asm("{\n\t.reg .b64 x, a;\n\tmov.b64 x, {%0, %1};\n\tmov.b64 a, {%2, %2};\n\t"
+      "mul.rn.f32x2 x, x, a;\n\tmov.b64 {%0, %1}, x;\n\t}"
+      : "+f"(x0), "+f"(x1)
+      : "f"(a));
+}
+
 template <bool kFp8>
 __device__ void softmax_role(const ChunkParams& p, const Ctx<kFp8>& x, uint32_t tmem, int slot,
                              int tpt) {
@@ -340,10 +466,10 @@ __device__ void softmax_role(const ChunkParams& p, const Ctx<kFp8>& x, uint32_t 
   const int quarter = warp & 3;
   const int r = quarter * 32 + lane;
   const uint32_t lane_addr = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
-  const uint32_t col_s = lane_addr + slot * 128, col_o = lane_addr + 256 + slot * 128;
+  const uint32_t col_p = lane_addr + kColP + slot * 64, col_o = lane_addr + kColO + slot * 128;
   const int rtok = r / p.group, rhead = r - rtok * p.group;
   float2* ml = reinterpret_cast<float2*>(x.smem + C::kOffMl);
-  uint32_t n_tile = 0, n_done = 0, n_ml = 0;  // phases waited for on this slot's barriers
+  uint32_t n_tile = 0, n_ml = 0;  // tiles of this slot, joins of the two slots so far
   uint32_t n_key = 0;                         // key tiles of all items so far (FP8 scale ring)
   for (int n = 0;; ++n) {
     Item it;
@@ -371,7 +497,10 @@ __device__ void softmax_role(const ChunkParams& p, const Ctx<kFp8>& x, uint32_t 
       if (busy) {
         tc_fence_after();
         float s[128];
-        tmem_ld32x4_sync(col_s, s);
+        tmem_ld32x4_sync(lane_addr, s);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(x.s_free);
         const int left = lim - j * kKeys;  // visible keys of this tile
         const float* sc = nullptr;
         if constexpr (kFp8) {
@@ -382,10 +511,8 @@ __device__ void softmax_role(const ChunkParams& p, const Ctx<kFp8>& x, uint32_t 
           for (int i = 0; i < 128; i += 4) {
             const float4 a = *reinterpret_cast<const float4*>(sc + i);
             const float4 b = *reinterpret_cast<const float4*>(sc + kKeys + i);
-            s[i + 0] = fmaf(s[i + 0], a.x, b.x);
-            s[i + 1] = fmaf(s[i + 1], a.y, b.y);
-            s[i + 2] = fmaf(s[i + 2], a.z, b.z);
-            s[i + 3] = fmaf(s[i + 3], a.w, b.w);
+            fma2(s[i + 0], s[i + 1], a.x, a.y, b.x, b.y);
+            fma2(s[i + 2], s[i + 3], a.z, a.w, b.z, b.w);
           }
         }
         if (left < kKeys) {
@@ -393,13 +520,14 @@ __device__ void softmax_role(const ChunkParams& p, const Ctx<kFp8>& x, uint32_t 
           for (int i = 0; i < 128; ++i)
             if (i >= left) s[i] = -INFINITY;
         }
-        float pm[8];
+        float pm[4];
 #pragma unroll
-        for (int u = 0; u < 8; ++u) pm[u] = fmaxf(s[u], s[u + 8]);
+        for (int u = 0; u < 4; ++u) pm[u] = fmaxf(s[u], s[u + 4]);
 #pragma unroll
-        for (int i = 16; i < 128; ++i) pm[i & 7] = fmaxf(pm[i & 7], s[i]);
-        float mx = fmaxf(fmaxf(fmaxf(pm[0], pm[1]), fmaxf(pm[2], pm[3])),
-                         fmaxf(fmaxf(pm[4], pm[5]), fmaxf(pm[6], pm[7])));
+        for (int i = 8; i < 128; i += 8)
+#pragma unroll
+          for (int u = 0; u < 4; ++u) pm[u] = fmaxf(fmaxf(pm[u], s[i + u]), s[i + u + 4]);
+        float mx = fmaxf(fmaxf(pm[0], pm[1]), fmaxf(pm[2], pm[3]));
         if constexpr (!kFp8) mx *= p.scale_log2;
         // the running maximum moves only by more than 2^8
         const float mn = (mx > m + kLazyLog2 || m == -INFINITY) ? mx : m;
@@ -407,58 +535,68 @@ __device__ void softmax_role(const ChunkParams& p, const Ctx<kFp8>& x, uint32_t 
         const float base = mn == -INFINITY ? 0.f : (kFp8 ? mn - kP8Shift : mn);
         m = mn;
         float ps[4] = {0.f, 0.f, 0.f, 0.f};
-        // P(j) as 16-bit pairs over columns [0, 64) of S, already read
+        // P(j) as 16-bit pairs
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           uint32_t pk[16];
 #pragma unroll
           for (int i = 0; i < 32; i += 4) {
-            float e[4];
+            float* e = s + c * 32 + i;
+            if constexpr (kFp8) {
+              add2(e[0], e[1], -base, -base);
+              add2(e[2], e[3], -base, -base);
+            } else {
+              fma2(e[0], e[1], p.scale_log2, p.scale_log2, -base, -base);
+              fma2(e[2], e[3], p.scale_log2, p.scale_log2, -base, -base);
+            }
 #pragma unroll
-            for (int u = 0; u < 4; ++u)
-              e[u] = ex2(kFp8 ? s[c * 32 + i + u] - base
-                              : fmaf(s[c * 32 + i + u], p.scale_log2, -base));
+            for (int u = 0; u < 4; ++u) e[u] = ex2(e[u]);
             if constexpr (kFp8) {
               const float4 iv = *reinterpret_cast<const float4*>(sc + 2 * kKeys + c * 32 + i);
-              ps[0] = fmaf(e[0], iv.x, ps[0]);
-              ps[1] = fmaf(e[1], iv.y, ps[1]);
-              ps[2] = fmaf(e[2], iv.z, ps[2]);
-              ps[3] = fmaf(e[3], iv.w, ps[3]);
+              fma2_to(ps[0], ps[1], e[0], e[1], iv.x, iv.y);
+              fma2_to(ps[2], ps[3], e[2], e[3], iv.z, iv.w);
               pk[i / 2] = pack_f16(e[0], e[1]);
               pk[i / 2 + 1] = pack_f16(e[2], e[3]);
             } else {
-#pragma unroll
-              for (int u = 0; u < 4; ++u) ps[u] += e[u];
+              add2(ps[0], ps[1], e[0], e[1]);
+              add2(ps[2], ps[3], e[2], e[3]);
               pk[i / 2] = pack_bf16(e[0], e[1]);
               pk[i / 2 + 1] = pack_bf16(e[2], e[3]);
             }
           }
-          tmem_st16u(col_s + c * 16, pk);
+          if (c == 0) {  // P and O are the slot's again once its last P.V is done
+            if (!first && !x.wait_warp(&x.pv_done[slot], n_tile - 2)) return;
+            tc_fence_after();
+          }
+          tmem_st16u(col_p + c * 16, pk);
         }
         l = l * alpha + ((ps[0] + ps[1]) + (ps[2] + ps[3]));
-        if (!first && __any_sync(0xffffffffu, alpha != 1.f)) {
+        // (l is never negative: with it the vote uses every scale read, which
+        // the arrive below must not overtake)
+        if (__any_sync(0xffffffffu, alpha != 1.f || l < 0.f) && !first) {
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
             float v[32];
             tmem_ld32_sync(col_o + c * 32, v);
 #pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] *= alpha;
+            for (int i = 0; i < 32; i += 2) mul2(v[i], v[i + 1], alpha);
             tmem_st32(col_o + c * 32, v);
           }
         }
-        first = false;
         tmem_wait_st();
         tc_fence_before();
+      } else {
+        if (lane == 0) mbar_arrive(x.s_free);
+        // without rows too: an arrival a tile ahead would end the wrong phase
+        if (!first && !x.wait_warp(&x.pv_done[slot], n_tile - 2)) return;
       }
+      first = false;
       __syncwarp();
       if (lane == 0) mbar_arrive(&x.p_full[slot]);
     }
     n_key += it.t1 - it.t0;
     // ---- end of the item
-    if (whole || slot == 0 || it.t1 - it.t0 > 1) {
-      if (!x.wait_warp(&x.o_full[slot], n_done)) return;
-      ++n_done;
-    }
+    if (!first && !x.wait_warp(&x.pv_done[slot], n_tile - 1)) return;
     tc_fence_after();
     const float base = m == -INFINITY ? 0.f : (kFp8 ? m - kP8Shift : m);
     const bool direct = it.slot < 0;
@@ -503,7 +641,7 @@ __device__ void softmax_role(const ChunkParams& p, const Ctx<kFp8>& x, uint32_t 
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           float v[32], w[32];
-          const uint32_t at = lane_addr + 256 + slot * 64 + c * 32;
+          const uint32_t at = lane_addr + kColO + slot * 64 + c * 32;
           tmem_ld32_sync(at, v);
           if (has_b) {
             tmem_ld32_sync(at + 128, w);
@@ -535,16 +673,27 @@ __device__ void softmax_role(const ChunkParams& p, const Ctx<kFp8>& x, uint32_t 
 }
 
 // ---------------------------------------------------------------- tensor core
+// Two warps issue, one the Q.K's and one the P.V's: the tensor cores' queue
+// holds a few instructions only, and a single warp that waits for P leaves
+// them idle although the next Q.K could start (and the other way round).
 template <bool kFp8>
-__device__ void mma_role(const ChunkParams& p, const Ctx<kFp8>& x, uint32_t tmem) {
+struct Tensor {
   using C = Cfg<kFp8>;
-  constexpr uint32_t kFmt = kFp8 ? 0u : ((1u << 7) | (1u << 10));  // f16 / bf16 operands
-  constexpr uint32_t kIdesc = (1u << 4) | kFmt | ((kKeys >> 3) << 17) | ((kRows >> 4) << 24);
-  constexpr uint32_t kIdescPV = kFp8 ? kIdesc : kIdesc | (1u << 16);  // bf16 V: MN-major
-  const int lane = threadIdx.x & 31;
-  const uint32_t sq = smem_u32(x.smem + C::kOffQ), skv = smem_u32(x.smem + C::kOffKV);
-  uint32_t seq = 0;               // K/V tiles taken so far: K(j) at seq + 2j, V(j) after it
-  uint32_t n_q = 0, n_p0 = 0, n_p1 = 0;  // phases of q_full and of p_full[0], [1]
+  static constexpr uint32_t kFmt = kFp8 ? 0u : ((1u << 7) | (1u << 10));  // f16 / bf16 operands
+  static constexpr uint32_t kIdesc =
+      (1u << 4) | kFmt | ((kKeys >> 3) << 17) | ((kRows >> 4) << 24);
+  static constexpr uint32_t kIdescPV = kFp8 ? kIdesc : kIdesc | (1u << 16);  // bf16 V: MN-major
+};
+
+// S = Q (tile of the slot) . K, tile by tile, each when the slot before has
+// taken S.
+template <bool kFp8>
+__device__ void qk_role(const ChunkParams& p, const Ctx<kFp8>& x, uint32_t tmem) {
+  using C = Cfg<kFp8>;
+  const uint32_t sq = kLoKMajor | (smem_u32(x.smem + C::kOffQ) >> 4);
+  const uint32_t sk = kLoKMajor | (smem_u32(x.smem + C::kOffK) >> 4);
+  RingPos<C::kKStages> k;
+  uint32_t n_q = 0, n_s = 0;  // Q tiles, Q.K's so far
   for (int n = 0;; ++n) {
     Item it;
     if (!x.next(n, it) || it.t1 < 0) return;
@@ -552,35 +701,51 @@ __device__ void mma_role(const ChunkParams& p, const Ctx<kFp8>& x, uint32_t tmem
     if (nt == 0) continue;
     if (!x.wait_warp(x.q_full, n_q)) return;
     ++n_q;
-    // S of `slot` = Q (tile of the slot) . K(j)
-    auto qk = [&](int j, int slot, bool last_use) -> bool {
-      const uint32_t i = seq + 2 * j, st = i % C::kStages;
-      if (!x.wait_warp(&x.kv_full[st], i / C::kStages)) return false;
-      if (lane == 0) {
+    for (int j = 0; j < nt; ++j) {
+      if (!x.wait_warp(&x.k_full[k.st], k.ph)) return;
+      const uint32_t b = sk + k.st * (kOperand >> 4);
+      for (int t = 0; t <= (it.two ? 1 : 0); ++t) {
+        if (n_s && !x.wait_warp(x.s_free, n_s - 1)) return;
+        ++n_s;
         tc_fence_after();
-        const uint32_t a = sq + (it.two ? slot * kOperand : 0), b = skv + st * kOperand;
-#pragma unroll
-        for (int kk = 0; kk < 8; ++kk)
-          umma(tmem + slot * 128, kmajor(a, kk), kFp8 ? kmajor(b, kk) : box_k(b, kk), kIdesc,
-               kk > 0 ? 1u : 0u);
-        umma_commit(&x.s_full[slot]);
-        if (last_use) umma_commit(&x.kv_empty[st]);
+        if constexpr (kFp8)
+          mma_ss8<kHiKMajor, kHiKMajor, (kRegion >> 4) - 6, (kRegion >> 4) - 6, 2>(
+              tmem, sq, b, Tensor<kFp8>::kIdesc);
+        else
+          mma_ss8<kHiKMajor, kHiBoxK, (kRegion >> 4) - 6, (1024 >> 4) - 6, 2>(
+              tmem, sq + t * (kOperand >> 4), b, Tensor<kFp8>::kIdesc);
+        mma_commit(&x.s_full[it.two ? t : j & 1]);
       }
-      __syncwarp();
-      return true;
-    };
-    // O of `slot` (+)= P . V(j)
-    auto pv = [&](int j, int slot, bool fresh, bool first_use, bool last_use) -> bool {
-      const uint32_t i = seq + 2 * j + 1, st = i % C::kStages;
-      if (!x.wait_warp(&x.kv_full[st], i / C::kStages)) return false;
-      const int key0 = (it.t0 + j) * kKeys;
-      const int nb = min(kTileBlocks, (it.key_end - key0 + kBlockTokens - 1) / kBlockTokens);
-      if (!kFp8 && first_use) {
+      mma_commit(&x.k_empty[k.st]);
+      k.next();
+    }
+    mma_commit(x.q_free);
+  }
+}
+
+// O of the slot (+)= P . V
+template <bool kFp8>
+__device__ void pv_role(const ChunkParams& p, const Ctx<kFp8>& x, uint32_t tmem) {
+  using C = Cfg<kFp8>;
+  constexpr uint32_t kIdesc = Tensor<kFp8>::kIdescPV;
+  const int lane = threadIdx.x & 31;
+  const uint32_t sv = (kFp8 ? kLoKMajor : kLoBoxV) | (smem_u32(x.smem + C::kOffV) >> 4);
+  RingPos<C::kVStages> v;
+  uint32_t n_p0 = 0, n_p1 = 0;  // P.V's of each slot so far
+  for (int n = 0;; ++n) {
+    Item it;
+    if (!x.next(n, it) || it.t1 < 0) return;
+    const int nt = it.t1 - it.t0;
+    for (int j = 0; j < nt; ++j) {
+      if (!x.wait_warp(&x.v_full[v.st], v.ph)) return;
+      const int left = it.key_end - (it.t0 + j) * kKeys;  // keys of this tile, and beyond
+      if (!kFp8 && left < kKeys) {
         // the rest of the cache's last block holds no position: zero rows, so
         // that P's zeros do not meet whatever is stored there
-        const int end = it.kv - key0, t = end & (kBlockTokens - 1);
+        const int nb = (left + kBlockTokens - 1) / kBlockTokens;
+        const int end = it.kv - (it.t0 + j) * kKeys, t = end & (kBlockTokens - 1);
         if (t && end < nb * kBlockTokens) {
-          uint8_t* blk = x.smem + C::kOffKV + st * kOperand + (end / kBlockTokens) * 4096;
+          uint8_t* blk = x.smem + C::kOffV + v.st * kOperand + (end / kBlockTokens) * 4096;
           for (int c = t * 16 + lane; c < kBlockTokens * 16; c += 32) {
             const int tok = c >> 4, half = (c >> 3) & 1;
             *reinterpret_cast<uint4*>(blk + (tok >> 3) * 2048 + half * 1024 + (tok & 7) * 128 +
@@ -590,58 +755,32 @@ __device__ void mma_role(const ChunkParams& p, const Ctx<kFp8>& x, uint32_t tmem
           __syncwarp();
         }
       }
-      uint32_t& np = slot ? n_p1 : n_p0;
-      if (!x.wait_warp(&x.p_full[slot], np)) return false;
-      ++np;
-      if (lane == 0) {
+      const uint32_t b = sv + v.st * (kOperand >> 4);
+      for (int t = 0; t <= (it.two ? 1 : 0); ++t) {
+        const int slot = it.two ? t : j & 1;
+        uint32_t& np = slot ? n_p1 : n_p0;
+        if (!x.wait_warp(&x.p_full[slot], np)) return;
+        ++np;
         tc_fence_after();
-        const uint32_t b = skv + st * kOperand;
-        for (int kb = 0; kb < nb; ++kb)
-          umma_ts(tmem + 256 + slot * 128, tmem + slot * 128 + kb * 8,
-                  kFp8 ? kmajor(b, kb) : box_v(b, kb), kIdescPV, (!fresh || kb > 0) ? 1u : 0u);
-        if (last_use) umma_commit(&x.kv_empty[st]);
-      }
-      __syncwarp();
-      return true;
-    };
-    auto commit = [&](uint64_t* bar) {
-      if (lane == 0) umma_commit(bar);
-      __syncwarp();
-    };
-    if (it.two) {
-      if (!qk(0, 0, false) || !qk(0, 1, true)) return;
-      if (nt == 1) commit(x.q_free);
-      for (int j = 0; j < nt; ++j) {
-        if (!pv(j, 0, j == 0, true, false)) return;
-        if (j + 1 < nt) {
-          if (!qk(j + 1, 0, false)) return;
+        const uint32_t d = tmem + kColO + slot * 128, a = tmem + kColP + slot * 64;
+        const bool more = it.two ? j > 0 : j > 1;  // onto what the item has so far
+        if (left > kKeys - kBlockTokens) {
+          if constexpr (kFp8)
+            mma_ts8<kHiKMajor, (kRegion >> 4) - 6, 2>(d, a, b, kIdesc, more);
+          else
+            mma_ts8<kHiBoxV, 256, 256>(d, a, b, kIdesc, more);
         } else {
-          commit(&x.o_full[0]);
+          const int nb = (left + kBlockTokens - 1) / kBlockTokens;
+          for (int kb = 0; kb < nb; ++kb)
+            mma_ts1(d, a + kb * 8,
+                    b + (kFp8 ? (kb >> 2) * (kRegion >> 4) + (kb & 3) * 2 : kb * 256),
+                    kFp8 ? kHiKMajor : kHiBoxV, kIdesc, (more || kb > 0) ? 1u : 0u);
         }
-        if (!pv(j, 1, j == 0, false, true)) return;
-        if (j + 1 < nt) {
-          if (!qk(j + 1, 1, true)) return;
-          if (j + 2 == nt) commit(x.q_free);
-        } else {
-          commit(&x.o_full[1]);
-        }
+        mma_commit(&x.pv_done[slot]);
       }
-    } else {
-      if (!qk(0, 0, true) || (nt > 1 && !qk(1, 1, true))) return;
-      if (nt <= 2) commit(x.q_free);
-      for (int j = 0; j < nt; ++j) {
-        if (!pv(j, j & 1, j < 2, true, true)) return;
-        if (j + 2 < nt) {
-          if (!qk(j + 2, j & 1, true)) return;
-          if (j + 3 == nt) commit(x.q_free);
-        }
-      }
-      commit(&x.o_full[0]);
-      // a slot without a tile waits for nothing of this item, so its barrier
-      // must not move on: two phases unseen look like none
-      if (nt > 1) commit(&x.o_full[1]);
+      mma_commit(&x.v_empty[v.st]);
+      v.next();
     }
-    seq += 2 * nt;
   }
 }
 
@@ -662,7 +801,11 @@ struct BlockIds {
     }
     return id;
   }
-  __device__ void start(const DevErr& err) {
+  __device__ BlockIds(const ChunkParams& p, const Item& it, const DevErr& err)
+      : trow(p.tables + static_cast<int64_t>(it.table_row) * p.pitch),
+        first(it.t0 * kTileBlocks),
+        count(min(it.t1 * kTileBlocks, (it.key_end + kBlockTokens - 1) / kBlockTokens) - first),
+        num_blocks(p.num_blocks) {
     cur = load(0, err);
     nxt = load(1, err);
   }
@@ -674,13 +817,15 @@ struct BlockIds {
   }
 };
 
-template <bool kFp8>
-__device__ void copy_role(const ChunkParams& p, const Ctx<kFp8>& x, const CUtensorMap* kmap,
-                          const CUtensorMap* vmap) {
-  using C = Cfg<kFp8>;
+// bf16 pool: one warp copies the K tiles, another the V tiles: a
+// thread takes over 100 cycles per box, 16 of them a tile of both.
+template <int kStages>
+__device__ void copy_role(const ChunkParams& p, const Ctx<false>& x, const CUtensorMap* map,
+                          uint64_t* full, uint64_t* empty, uint8_t* ring) {
   const int lane = threadIdx.x & 31;
   const uint64_t keep = policy_evict_last();
-  uint32_t seq = 0;  // K/V tiles (FP8: chunks) issued so far
+  RingPos<kStages> r;
+  uint32_t n_tile = 0;
   bool ok = true;
   for (int n = 0; ok; ++n) {
     Item it;
@@ -688,55 +833,72 @@ __device__ void copy_role(const ChunkParams& p, const Ctx<kFp8>& x, const CUtens
     if (!ok || it.t1 < 0) break;
     const int nt = it.t1 - it.t0;
     if (nt == 0) continue;
-    BlockIds ids;
-    ids.trow = p.tables + static_cast<int64_t>(it.table_row) * p.pitch;
-    ids.first = it.t0 * kTileBlocks;
-    ids.count = min(it.t1 * kTileBlocks, (it.key_end + kBlockTokens - 1) / kBlockTokens) - ids.first;
-    ids.num_blocks = p.num_blocks;
-    ids.start(x.err);
-    for (int j = 0; j < nt && ok; ++j) {
+    BlockIds ids(p, it, x.err);
+    for (int j = 0; j < nt; ++j) {
       const int b0 = j * kTileBlocks;
       if (j && (b0 & 31) == 0) ids.advance(b0, x.err);
       const int nb = min(kTileBlocks, ids.count - b0);
-      if constexpr (kFp8) {
-        for (int b = 0; b < nb && ok; ++b, ++seq) {
-          const uint32_t st = seq % C::kRaw, ph = seq / C::kRaw;
-          const int id = ids.at(b0 + b);
-          if (ph) ok = x.wait_warp(&x.raw_empty[st], ph - 1);
-          if (ok && lane == 0) {
-            mbar_arrive_expect_tx(&x.raw_full[st], kFp8HeadBlockBytes);
-            bulk_load(x.smem + C::kOffRaw + st * kFp8HeadBlockBytes,
-                      p.kv8 + (static_cast<int64_t>(id) * p.hkv + it.kvh) * kFp8HeadBlockBytes,
-                      kFp8HeadBlockBytes, &x.raw_full[st], keep);
-          }
-          __syncwarp();
-        }
-      } else {
-#pragma unroll
-        for (int which = 0; which < 2; ++which, ++seq) {
-          const uint32_t st = seq % C::kStages, ph = seq / C::kStages;
-          if (ph && !x.wait_warp(&x.kv_empty[st], ph - 1)) {
-            ok = false;
-            break;
-          }
-          if (lane == 0) mbar_arrive_expect_tx(&x.kv_full[st], nb * 4096);
-          for (int b = 0; b < nb; ++b) {
-            const int id = ids.at(b0 + b);
-            if (lane == 0)
-              tma_load_5d(x.smem + C::kOffKV + st * kOperand + b * 4096, which ? vmap : kmap,
-                          &x.kv_full[st], 0, 0, 0, id * 2, it.kvh, keep);
-          }
-          __syncwarp();
-        }
+      if (n_tile >= kStages && !x.wait_warp(&empty[r.st], r.ph ^ 1)) {
+        ok = false;
+        break;
       }
+      uint8_t* dst = ring + r.st * kOperand;
+      uint64_t* bar = &full[r.st];
+      if (lane == 0) mbar_arrive_expect_tx(bar, nb * 4096);
+      for (int b = 0; b < nb; ++b) {
+        const int id = ids.at(b0 + b);
+        if (lane == 0) tma_load_5d(dst + b * 4096, map, bar, 0, 0, 0, id * 2, it.kvh, keep);
+      }
+      __syncwarp();
+      r.next();
+      ++n_tile;
     }
   }
-  if (!ok) {
-    // copies still in flight get a bounded time to land before the CTA ends
-    const uint32_t ring = kFp8 ? C::kRaw : C::kStages;
-    for (uint32_t s = seq > ring ? seq - ring : 0; s < seq; ++s)
-      x.wait(kFp8 ? &x.raw_full[s % ring] : &x.kv_full[s % ring], s / ring);
+  if (!ok) {  // copies still in flight get a bounded time to land before the CTA ends
+    for (uint32_t t = n_tile > kStages ? n_tile - kStages : 0; t < n_tile; ++t)
+      x.wait(&full[t % kStages], t / kStages);
   }
+}
+
+// FP8 pool: one bulk copy per block, four blocks to a barrier.
+__device__ void copy_role(const ChunkParams& p, const Ctx<true>& x) {
+  using C = Cfg<true>;
+  const int lane = threadIdx.x & 31;
+  const uint64_t keep = policy_evict_last();
+  RingPos<C::kRaw> r;
+  uint32_t n_group = 0;
+  bool ok = true;
+  for (int n = 0; ok; ++n) {
+    Item it;
+    ok = x.next(n, it);
+    if (!ok || it.t1 < 0) break;
+    if (it.t1 == it.t0) continue;
+    BlockIds ids(p, it, x.err);
+    for (int b0 = 0; b0 < ids.count; b0 += kGroup) {
+      if (b0 && (b0 & 31) == 0) ids.advance(b0, x.err);
+      if (n_group >= C::kRaw && !x.wait_warp(&x.raw_empty[r.st], r.ph ^ 1)) {
+        ok = false;
+        break;
+      }
+      const int nb = min(kGroup, ids.count - b0);
+      uint8_t* dst = x.smem + C::kOffRaw + r.st * kGroup * kFp8HeadBlockBytes;
+      if (lane == 0) mbar_arrive_expect_tx(&x.raw_full[r.st], nb * kFp8HeadBlockBytes);
+#pragma unroll
+      for (int b = 0; b < kGroup; ++b) {
+        const int id = ids.at(b0 + b);
+        if (lane == 0 && b < nb)
+          bulk_load(dst + b * kFp8HeadBlockBytes,
+                    p.kv8 + (static_cast<int64_t>(id) * p.hkv + it.kvh) * kFp8HeadBlockBytes,
+                    kFp8HeadBlockBytes, &x.raw_full[r.st], keep);
+      }
+      __syncwarp();
+      ++n_group;
+      r.next();
+    }
+  }
+  if (!ok)
+    for (uint32_t g = n_group > C::kRaw ? n_group - C::kRaw : 0; g < n_group; ++g)
+      x.wait(&x.raw_full[g % C::kRaw], g / C::kRaw);
 }
 
 // ---------------------------------------------------------------- FP8 widening
@@ -757,7 +919,7 @@ __device__ __forceinline__ uint32_t keep_pair(uint32_t w, int t, int valid) {
   return t + 1 < valid ? w : (t < valid ? w & 0xffffu : 0u);
 }
 
-__device__ void widen_role(const ChunkParams& p, const Ctx<true>& x) {
+__device__ void widen_role(const ChunkParams& p, const Ctx<true>& x, int tpt) {
   using C = Cfg<true>;
   const int c = threadIdx.x - 384, lane = c & 31;
   const int pair = ((lane >> 4) & 1) + 2 * (c >> 5);
@@ -767,22 +929,39 @@ __device__ void widen_role(const ChunkParams& p, const Ctx<true>& x) {
   const uint32_t k_dst = (grp >> 2) * kRegion + tok * 128;
   const uint32_t k_lo = ((((grp & 3) * 2) ^ (tok & 7)) << 4);
   const uint32_t k_hi = ((((grp & 3) * 2 + 1) ^ (tok & 7)) << 4);
-  uint32_t seq = 0, raw = 0, key = 0;
+  uint32_t key = 0, n_load = 0;  // key tiles, Q tiles so far
+  RingPos<C::kRaw> g;            // the copy group of the tile's first block
+  RingPos<C::kKStages> k;
+  RingPos<C::kVStages> v;
   for (int n = 0;; ++n) {
     Item it;
     if (!x.next(n, it) || it.t1 < 0) return;
     const int nt = it.t1 - it.t0;
+    if (nt) {
+      if (n_load && !x.wait_warp(x.q_free, n_load - 1)) return;
+      ++n_load;
+      load_q_f16(p, x.smem + C::kOffQ, it, tpt, c);
+      fence_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(x.q_full);
+    }
     const int nblk = (it.key_end + kBlockTokens - 1) / kBlockTokens;
     for (int j = 0; j < nt; ++j) {
       const int b0 = (it.t0 + j) * kTileBlocks, nb = min(kTileBlocks, nblk - b0);
       // ---- K tile and the keys' scales
-      uint32_t st = seq % C::kStages, ph = seq / C::kStages;
-      if (ph && !x.wait_warp(&x.kv_empty[st], ph - 1)) return;
-      uint8_t* dst = x.smem + C::kOffKV + st * kOperand;
+      if (key >= C::kKStages && !x.wait_warp(&x.k_empty[k.st], k.ph ^ 1)) return;
+      uint8_t* dst = x.smem + C::kOffK + k.st * kOperand;
+      const bool second = nb > kGroup;  // the tile has blocks in two groups
+      RingPos<C::kRaw> g2 = g;
+      g2.next();
+      if (!x.wait_warp(&x.raw_full[g.st], g.ph)) return;
+      if (second && !x.wait_warp(&x.raw_full[g2.st], g2.ph)) return;
+      const uint8_t* raw0 = x.smem + C::kOffRaw + g.st * kGroup * kFp8HeadBlockBytes;
+      const uint8_t* raw1 = x.smem + C::kOffRaw + g2.st * kGroup * kFp8HeadBlockBytes -
+                            kGroup * kFp8HeadBlockBytes;  // block b of the tile, b >= kGroup
+#pragma unroll 4
       for (int b = 0; b < nb; ++b) {
-        const uint32_t rs = (raw + b) % C::kRaw;
-        if (!x.wait_warp(&x.raw_full[rs], (raw + b) / C::kRaw)) return;
-        const uint8_t* src = x.smem + C::kOffRaw + rs * kFp8HeadBlockBytes;
+        const uint8_t* src = (b < kGroup ? raw0 : raw1) + b * kFp8HeadBlockBytes;
         uint4 lo, hi;
         widen16(*reinterpret_cast<const uint4*>(src + k_src), lo, hi);
         *reinterpret_cast<uint4*>(dst + k_dst + b * 2048 + k_lo) = lo;
@@ -792,9 +971,9 @@ __device__ void widen_role(const ChunkParams& p, const Ctx<true>& x) {
         float ks = 0.f, lv = 0.f, iv = 0.f;
         const int pos = b0 * kBlockTokens + c;
         if (c < nb * kBlockTokens && pos < it.kv) {
-          const uint32_t rs = (raw + c / kBlockTokens) % C::kRaw;
+          const int b = c / kBlockTokens;
           const float* sc = reinterpret_cast<const float*>(
-              x.smem + C::kOffRaw + rs * kFp8HeadBlockBytes + kFp8KScaleOff);
+              (b < kGroup ? raw0 : raw1) + b * kFp8HeadBlockBytes + kFp8KScaleOff);
           ks = sc[c % kBlockTokens] * (16.f * p.scale_log2);
           // a value row below 2^-91 in size counts as if at that scale
           const float vs = fmaxf(sc[16 + c % kBlockTokens], 0x1p-100f);
@@ -810,22 +989,17 @@ __device__ void widen_role(const ChunkParams& p, const Ctx<true>& x) {
       __syncwarp();
       if (lane == 0) {
         mbar_arrive(&x.sc_full[key & 3]);
-        mbar_arrive(&x.kv_full[st]);
+        mbar_arrive(&x.k_full[k.st]);
       }
-      ++key;
-      ++seq;
+      k.next();
       // ---- V tile
-      st = seq % C::kStages;
-      ph = seq / C::kStages;
-      if (ph && !x.wait_warp(&x.kv_empty[st], ph - 1)) return;
-      dst = x.smem + C::kOffKV + st * kOperand;
+      if (key >= C::kVStages && !x.wait_warp(&x.v_empty[v.st], v.ph ^ 1)) return;
+      dst = x.smem + C::kOffV + v.st * kOperand;
+#pragma unroll 4
       for (int b = 0; b < nb; ++b) {
-        const uint32_t rs = (raw + b) % C::kRaw;
-        const uint8_t* src = x.smem + C::kOffRaw + rs * kFp8HeadBlockBytes + kFp8VOff;
+        const uint8_t* src = (b < kGroup ? raw0 : raw1) + b * kFp8HeadBlockBytes + kFp8VOff;
         uint4 lo, hi;
         widen16(*reinterpret_cast<const uint4*>(src + c * 16), lo, hi);
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&x.raw_empty[rs]);
         const int valid = it.kv - (b0 + b) * kBlockTokens;
         if (valid < kBlockTokens) {  // no position there: zeros for P's zeros
           lo.x = keep_pair(lo.x, 0, valid);
@@ -843,23 +1017,30 @@ __device__ void widen_role(const ChunkParams& p, const Ctx<true>& x) {
       }
       fence_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&x.kv_full[st]);
-      ++seq;
-      raw += nb;
+      if (lane == 0) {
+        // behind the stores: every load of the chunks has returned by then,
+        // which an arrive right behind the loads would not wait for
+        mbar_arrive(&x.v_full[v.st]);
+        mbar_arrive(&x.raw_empty[g.st]);
+        if (second) mbar_arrive(&x.raw_empty[g2.st]);
+      }
+      v.next();
+      ++key;
+      g.next();
+      if (second) g.next();
     }
   }
 }
 
 // ---------------------------------------------------------------- items
 // Warp 3: the items of this CTA's range [lo, hi) of the summed costs, from row
-// b whose first item starts at `base`; then its half of each Q tile.
+// b whose first item starts at `base`.
 template <bool kFp8>
 __device__ void item_role(const ChunkParams& p, const Ctx<kFp8>& x, const Work& w, int b,
                           int64_t base, int64_t lo, int64_t hi, int64_t step) {
   const int lane = threadIdx.x & 31;
   const int cta = blockIdx.x;
   int n = 0;
-  uint32_t n_load = 0;
   int4 desc = make_int4(0, 0, 0, 0);
   bool ok = true;
   auto push = [&](const Item& it) -> bool {
@@ -924,16 +1105,6 @@ __device__ void item_role(const ChunkParams& p, const Ctx<kFp8>& x, const Work& 
         if (it.slot == 1)  // this CTA holds the item's first keys: it names the parts
           desc = make_int4(static_cast<int>((end - 1) / step) - cta + 1, it.first, it.ntok, h);
         ok = push(it);
-        if (ok && it.t1 > 0) {
-          if (n_load) ok = x.wait_warp(x.q_free, n_load - 1);
-          if (ok) {
-            load_q<kFp8>(p, x.smem, it, w.tpt, 32 + lane);
-            fence_async_smem();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(x.q_full);
-            ++n_load;
-          }
-        }
       }
     }
     base = row_end;
@@ -947,19 +1118,17 @@ __device__ void item_role(const ChunkParams& p, const Ctx<kFp8>& x, const Work& 
   }
 }
 
-template <bool kFp8>
-__device__ void q_role(const ChunkParams& p, const Ctx<kFp8>& x, int tpt) {
-  const int lane = threadIdx.x & 31;
+__device__ void q_role(const ChunkParams& p, const Ctx<false>& x, int tpt) {
   uint32_t n_load = 0;
   for (int n = 0;; ++n) {
     Item it;
     if (!x.next(n, it) || it.t1 < 0) return;
     if (it.t1 == 0) continue;
     if (n_load && !x.wait_warp(x.q_free, n_load - 1)) return;
-    load_q<kFp8>(p, x.smem, it, tpt, lane);
+    load_q(p, x.smem + Cfg<false>::kOffQ, it, tpt, threadIdx.x - 416);
     fence_async_smem();
     __syncwarp();
-    if (lane == 0) mbar_arrive(x.q_full);
+    if ((threadIdx.x & 31) == 0) mbar_arrive(x.q_full);
     ++n_load;
   }
 }
@@ -990,22 +1159,27 @@ __global__ void __launch_bounds__(Cfg<kFp8>::kThreads, 1)
     }
     for (int i = 0; i < kItemRing; ++i) {
       mbar_init(&x.item_full[i], 1);
-      mbar_init(&x.item_empty[i], kFp8 ? 15 : 11);  // every warp but warp 3
+      mbar_init(&x.item_empty[i], 15);  // every warp but warp 3
     }
-    mbar_init(x.q_full, 2);
+    mbar_init(x.q_full, kFp8 ? 4 : 3);
     mbar_init(x.q_free, 1);
-    for (int i = 0; i < C::kStages; ++i) {
-      mbar_init(&x.kv_full[i], kFp8 ? 4 : 1);
-      mbar_init(&x.kv_empty[i], 1);
+    for (int i = 0; i < C::kKStages; ++i) {
+      mbar_init(&x.k_full[i], kFp8 ? 4 : 1);
+      mbar_init(&x.k_empty[i], 1);
+    }
+    for (int i = 0; i < C::kVStages; ++i) {
+      mbar_init(&x.v_full[i], kFp8 ? 4 : 1);
+      mbar_init(&x.v_empty[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&x.s_full[i], 1);
       mbar_init(&x.p_full[i], 4);
-      mbar_init(&x.o_full[i], 1);
+      mbar_init(&x.pv_done[i], 1);
     }
+    mbar_init(x.s_free, 4);
     mbar_init(x.ml_bar, 8);
     mbar_init(x.ep_bar, 8);
-    mbar_init(x.mma_done, 1);
+    mbar_init(x.mma_done, 2);
     for (int i = 0; i < C::kRaw; ++i) {
       mbar_init(&x.raw_full[i], 1);
       mbar_init(&x.raw_empty[i], 4);
@@ -1066,25 +1240,35 @@ __global__ void __launch_bounds__(Cfg<kFp8>::kThreads, 1)
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kRegsLow));
     if (warp == 0) {
-      copy_role<kFp8>(p, x, &kmap, &vmap);
+      if constexpr (kFp8)
+        copy_role(p, x);
+      else
+        copy_role<C::kKStages>(p, x, &kmap, x.k_full, x.k_empty, smem + C::kOffK);
     } else if (warp == 1) {
-      mma_role<kFp8>(p, x, tmem);
+      qk_role<kFp8>(p, x, tmem);
       // every tensor instruction has retired before TMEM is freed (after a
       // wait that ran out, some may be in flight here)
-      if (lane == 0) umma_commit(x.mma_done);
-      __syncwarp();
+      mma_commit(x.mma_done);
       x.wait_warp(x.mma_done, 0);
     } else if (warp == 2) {
-      q_role<kFp8>(p, x, w.tpt);
+      pv_role<kFp8>(p, x, tmem);
+      mma_commit(x.mma_done);
+      x.wait_warp(x.mma_done, 0);
     } else {
       item_role<kFp8>(p, x, w, static_cast<int>(s_row), s_base, lo, hi, step);
     }
   } else if (warp < 12) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::kRegsSoftmax));
     softmax_role<kFp8>(p, x, tmem, (warp - 4) >> 2, w.tpt);
-  } else if constexpr (kFp8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kRegsConv));
-    widen_role(p, x);
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kRegsAux));
+    if constexpr (kFp8) {
+      widen_role(p, x, w.tpt);
+    } else if (warp == 12) {
+      copy_role<C::kVStages>(p, x, &vmap, x.v_full, x.v_empty, smem + C::kOffV);
+    } else {
+      q_role(p, x, w.tpt);
+    }
   }
   __syncwarp();
   tc_fence_before();

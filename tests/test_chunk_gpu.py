@@ -243,6 +243,19 @@ def test_same_bits_on_every_call_and_capacity(cuda, fmt):
 
 
 @FMT
+@pytest.mark.parametrize("new,kv", [([21] * 40, [2048] * 40), ([10] * 40, [2000 + i for i in range(40)]),
+                                    ([700], [5000]), ([1500, 3], [9000, 20000])])
+def test_repeated_calls_give_the_same_bits(cuda, fmt, new, kv):
+    """Items back to back in every CTA, the rings full: a copy or a tile
+    released before it was read shows as other bits on some call."""
+    c = make(cuda, new, kv, 12, 2, fmt)
+    first = check(c)
+    for _ in range(40):
+        out, err = call(c)
+        assert err == 0 and torch.equal(out, first)
+
+
+@FMT
 def test_captured_graph_replays_on_other_lengths(cuda, fmt):
     """A call captured for a capacity of tokens and positions replays for any
     lengths within it: rows are padded with T = 0."""

@@ -1,11 +1,11 @@
 """The packed-chunk kernel's synchronisation protocol and work split
 (csrc/chunk.cu), modelled on the CPU.
 
-Protocol: the roles (copies, tensor issue, two Q writers of which one hands
-out the items, two slots of four softmax warps, FP8: four widening warps) run
-as generators under random scheduling; copies land in any order, tensor
-instructions and commits run in issue order, mbarriers have the hardware's
-phase parity.  Every read is checked for the tile it was meant for.
+Protocol: the roles (copies, the warp that hands out the items, three that
+write Q tiles, one issuing Q.K's and one P.V's, two slots of four softmax
+warps, FP8: four widening warps that also write Q) run as generators under random scheduling; copies
+land in any order, the tensor instructions and commits of one issuer run in
+order but those of the two in any, mbarriers have the hardware's phase parity.  Every read is checked for the tile it was meant for.
 
 Work split: the cut of the summed item costs into one range per CTA, restated
 in Python: every key tile of every item is worked exactly once, the parts of a
@@ -20,31 +20,40 @@ from test_prefill_protocol import Barrier, Race
 RING = 3
 
 
-def run_kernel(items, seed, fp8, stages=None, scales=4, merge_wait=True, always_commit=False):
+def run_kernel(items, seed, fp8, shared_ring=False, scales=4, merge_wait=True, idle_wait=True):
     """items: [(two, nt)].  Raises Race on a wrong read, a lost update or a hang."""
     rng = random.Random(seed)
-    stages = stages or (4 if fp8 else 5)
-    raws = 13
-    B = {"q_full": Barrier(2), "q_free": Barrier(1), "ml": Barrier(8), "ep": Barrier(8)}
+    k_stages, v_stages = (2, 2) if fp8 else (3, 2)
+    raws = 3  # groups of four chunks
+    B = {"q_full": Barrier(4 if fp8 else 3), "q_free": Barrier(1), "ml": Barrier(8), "ep": Barrier(8)}
     for i in range(RING):
-        B[f"item_full{i}"], B[f"item_empty{i}"] = Barrier(1), Barrier(15 if fp8 else 11)
-    for i in range(stages):
+        B[f"item_full{i}"], B[f"item_empty{i}"] = Barrier(1), Barrier(15)
+    for i in range(k_stages + v_stages):
         B[f"kv_full{i}"], B[f"kv_empty{i}"] = Barrier(4 if fp8 else 1), Barrier(1)
+
+    def ring(which, t):
+        """(stage, use) of K (0) or V (1) tile t: a ring each; shared_ring: one ring that alternates."""
+        if shared_ring:
+            return (2 * t + which) % (k_stages + v_stages), (2 * t + which) // (k_stages + v_stages)
+        return (k_stages + t % v_stages, t // v_stages) if which else (t % k_stages, t // k_stages)
+
+    B["s_free"] = Barrier(4)
     for s in range(2):
-        B[f"s_full{s}"], B[f"p_full{s}"], B[f"o_full{s}"] = Barrier(1), Barrier(4), Barrier(1)
+        B[f"s_full{s}"], B[f"p_full{s}"], B[f"pv_done{s}"] = Barrier(1), Barrier(4), Barrier(1)
     for i in range(raws):
         B[f"raw_full{i}"], B[f"raw_empty{i}"] = Barrier(1), Barrier(4)
     for i in range(4):
         B[f"sc_full{i}"] = Barrier(4)
     item_ring = [None] * RING
-    Q = [None, None]
-    kv = [[None] * 4 for _ in range(stages)]  # per widening warp; the copy engine writes all four
+    Q = [None] * (4 if fp8 else 3)
+    kv = [[None] * 4 for _ in range(k_stages + v_stages)]  # per widening warp; the copy engine writes all four
     raw = [None] * raws
     sc = [[None] * 4 for _ in range(scales)]
-    S = [[None] * 4 for _ in range(2)]
+    S = [None] * 4
+    P = [[None] * 4 for _ in range(2)]
     O = [set(), set()]
     ml = [[None] * 4 for _ in range(2)]
-    tma, pipe, finished = [], [], []
+    tma, qk_pipe, pv_pipe, finished = [], [], [], []
     STOP = (None, -1)
 
     def wait(name, phase):
@@ -64,81 +73,78 @@ def run_kernel(items, seed, fp8, stages=None, scales=4, merge_wait=True, always_
     def q_write(n, which, n_load):
         if n_load:
             yield wait("q_free", n_load - 1)
-        Q[which] = n
+        for w in which:
+            Q[w] = n
         yield None
         B["q_full"].arrive()
 
     def items_role():
-        n_load = 0
         for n, it in enumerate(list(items) + [STOP]):
             if n >= RING:
                 yield wait(f"item_empty{n % RING}", n // RING - 1)
             item_ring[n % RING] = (n, it)
             B[f"item_full{n % RING}"].arrive()
             yield None
-            if it[1] > 0:
-                yield from q_write(n, 1, n_load)
-                n_load += 1
 
-    def q_role():
-        n_load = 0
-        n = 0
+    def q_role(w):
+        n = n_load = 0
         while True:
             it = yield from nxt(n)
             if it[1] < 0:
                 return
             if it[1]:
-                yield from q_write(n, 0, n_load)
+                yield from q_write(n, [w], n_load)
                 n_load += 1
             n += 1
 
-    def copy_role():
-        n = seq = 0
+    def copy_role(which):
+        n = t = 0
         while True:
             it = yield from nxt(n)
             if it[1] < 0:
                 return
             for j in range(it[1]):
                 if fp8:
-                    for b in range(8):
-                        st = seq % raws
-                        if seq >= raws:
-                            yield wait(f"raw_empty{st}", seq // raws - 1)
+                    for g in range(2):
+                        st = t % raws
+                        if t >= raws:
+                            yield wait(f"raw_empty{st}", t // raws - 1)
                         B[f"raw_full{st}"].expect_tx(1)
-                        tma.append((raw, st, (n, j, b), f"raw_full{st}"))
-                        seq += 1
+                        tma.append((raw, st, (n, j, g), f"raw_full{st}"))
+                        t += 1
                         yield None
                 else:
-                    for w in "KV":
-                        st = seq % stages
-                        if seq >= stages:
-                            yield wait(f"kv_empty{st}", seq // stages - 1)
-                        B[f"kv_full{st}"].expect_tx(1)
-                        tma.append((kv, st, [(w, n, j)] * 4, f"kv_full{st}"))
-                        seq += 1
-                        yield None
+                    st, use = ring(which, t)
+                    if use:
+                        yield wait(f"kv_empty{st}", use - 1)
+                    B[f"kv_full{st}"].expect_tx(1)
+                    tma.append((kv, st, [("KV"[which], n, j)] * 4, f"kv_full{st}"))
+                    t += 1
+                    yield None
             n += 1
 
     def widen_role(w):
-        n = seq = r = key = 0
+        n = r = key = n_load = 0
         while True:
             it = yield from nxt(n)
             if it[1] < 0:
                 return
+            if it[1]:
+                yield from q_write(n, [w], n_load)
+                n_load += 1
             for j in range(it[1]):
                 for what in "KV":
-                    st = seq % stages
-                    if seq >= stages:
-                        yield wait(f"kv_empty{st}", seq // stages - 1)
-                    for b in range(8):
-                        rs = (r + b) % raws
+                    st, use = ring("KV".index(what), r // 2)
+                    if use:
+                        yield wait(f"kv_empty{st}", use - 1)
+                    for g in range(2):
+                        rs = (r + g) % raws
                         if what == "K":
-                            yield wait(f"raw_full{rs}", (r + b) // raws)
-                        need(raw[rs] == (n, j, b), "raw chunk")
-                        if what == "V":
-                            B[f"raw_empty{rs}"].arrive()
+                            yield wait(f"raw_full{rs}", (r + g) // raws)
+                        need(raw[rs] == (n, j, g), "raw chunks")
                         if rng.random() < 0.2:
                             yield None
+                        need(raw[rs] == (n, j, g), "raw chunks while read")
                     kv[st][w] = (what, n, j)
                     if what == "K":
                         sc[key % scales][w] = key
@@ -146,76 +152,60 @@ def run_kernel(items, seed, fp8, stages=None, scales=4, merge_wait=True, always_
                         B[f"sc_full{key & 3}"].arrive()
                         key += 1
                     B[f"kv_full{st}"].arrive()
-                    seq += 1
+                    if what == "V":
+                        B[f"raw_empty{r % raws}"].arrive()
+                        B[f"raw_empty{(r + 1) % raws}"].arrive()
                     yield None
-                r += 8
+                r += 2
             n += 1
 
-    def mma():
-        n = seq = n_q = 0
+    def qk_role():
+        n = k = n_q = n_s = 0
+        while True:
+            it = yield from nxt(n)
+            if it[1] < 0:
+                return
+            two, nt = it
+            if nt:
+                yield wait("q_full", n_q)
+                n_q += 1
+            for j in range(nt):
+                st, use = ring(0, k)
+                k += 1
+                yield wait(f"kv_full{st}", use)
+                for slot in (0, 1) if two else (j & 1,):
+                    if n_s:
+                        yield wait("s_free", n_s - 1)
+                    n_s += 1
+                    qk_pipe.append(("QK", n, j, slot, st))
+                    qk_pipe.append(("commit", f"s_full{slot}"))
+                qk_pipe.append(("commit", f"kv_empty{st}"))
+            if nt:
+                qk_pipe.append(("commit", "q_free"))
+            n += 1
+
+    def pv_role():
+        n = v = 0
         n_p = [0, 0]
         while True:
             it = yield from nxt(n)
             if it[1] < 0:
                 return
             two, nt = it
-            if not nt:
-                n += 1
-                continue
-            yield wait("q_full", n_q)
-            n_q += 1
-
-            def qk(j, slot, last):
-                i = seq + 2 * j
-                yield wait(f"kv_full{i % stages}", i // stages)
-                pipe.append(("QK", n, j, slot, i % stages))
-                pipe.append(("commit", f"s_full{slot}"))
-                if last:
-                    pipe.append(("commit", f"kv_empty{i % stages}"))
-
-            def pv(j, slot, fresh, last):
-                i = seq + 2 * j + 1
-                yield wait(f"kv_full{i % stages}", i // stages)
-                yield wait(f"p_full{slot}", n_p[slot])
-                n_p[slot] += 1
-                pipe.append(("PV", n, j, slot, i % stages, fresh))
-                if last:
-                    pipe.append(("commit", f"kv_empty{i % stages}"))
-
-            if two:
-                yield from qk(0, 0, False)
-                yield from qk(0, 1, True)
-                if nt == 1:
-                    pipe.append(("commit", "q_free"))
-                for j in range(nt):
-                    for slot in range(2):
-                        yield from pv(j, slot, j == 0, slot == 1)
-                        if j + 1 < nt:
-                            yield from qk(j + 1, slot, slot == 1)
-                            if slot == 1 and j + 2 == nt:
-                                pipe.append(("commit", "q_free"))
-                        else:
-                            pipe.append(("commit", f"o_full{slot}"))
-            else:
-                yield from qk(0, 0, True)
-                if nt > 1:
-                    yield from qk(1, 1, True)
-                if nt <= 2:
-                    pipe.append(("commit", "q_free"))
-                for j in range(nt):
-                    yield from pv(j, j & 1, j < 2, True)
-                    if j + 2 < nt:
-                        yield from qk(j + 2, j & 1, True)
-                        if j + 3 == nt:
-                            pipe.append(("commit", "q_free"))
-                pipe.append(("commit", "o_full0"))
-                if nt > 1 or always_commit:
-                    pipe.append(("commit", "o_full1"))
-            seq += 2 * nt
+            for j in range(nt):
+                st, use = ring(1, v)
+                v += 1
+                yield wait(f"kv_full{st}", use)
+                for slot in (0, 1) if two else (j & 1,):
+                    yield wait(f"p_full{slot}", n_p[slot])
+                    n_p[slot] += 1
+                    pv_pipe.append(("PV", n, j, slot, st, j < (1 if two else 2)))
+                    pv_pipe.append(("commit", f"pv_done{slot}"))
+                pv_pipe.append(("commit", f"kv_empty{st}"))
             n += 1
 
     def softmax(slot, q):
-        n = n_tile = n_done = n_ml = n_key = 0
+        n = n_tile = n_ml = n_key = 0
         while True:
             it = yield from nxt(n)
             if it[1] < 0:
@@ -224,26 +214,32 @@ def run_kernel(items, seed, fp8, stages=None, scales=4, merge_wait=True, always_
             if not nt:
                 n += 1
                 continue
+            busy = rng.random() < 0.7  # a warp whose rows are past the item's does no work
             mine = list(range(nt)) if two else list(range(slot, nt, 2))
             for a, j in enumerate(mine):
                 yield wait(f"s_full{slot}", n_tile)
                 n_tile += 1
-                need(S[slot][q] == ("S", n, j), f"S {S[slot][q]} for {(n, j)}")
-                if fp8:
+                need(S[q] == (n, j, slot), f"S {S[q]} for {(n, j, slot)}")
+                yield None
+                need(S[q] == (n, j, slot), "S while it is taken")
+                B["s_free"].arrive()
+                if busy and fp8:
                     yield wait(f"sc_full{(n_key + j) & 3}", (n_key + j) >> 2)
                     need(all(v == n_key + j for v in sc[(n_key + j) % scales]), "scales")
                 if rng.random() < 0.5:
                     yield None
-                if a and rng.random() < 0.5:  # rescales O
-                    need(O[slot] == {(n, i) for i in mine[:a]}, "O during a rescale")
-                if fp8:
-                    need(all(v == n_key + j for v in sc[(n_key + j) % scales]), "scales, second read")
-                S[slot][q] = ("P", n, j)
+                if a and (busy or idle_wait):
+                    yield wait(f"pv_done{slot}", n_tile - 2)
+                if busy:
+                    if a:
+                        need(O[slot] == {(n, i) for i in mine[:a]}, "O during a rescale")
+                    if fp8:
+                        need(all(v == n_key + j for v in sc[(n_key + j) % scales]), "scales, second read")
+                P[slot][q] = (n, j)
                 B[f"p_full{slot}"].arrive()
             n_key += nt
-            if mine or always_commit:
-                yield wait(f"o_full{slot}", n_done)
-                n_done += 1
+            if mine:
+                yield wait(f"pv_done{slot}", n_tile - 1)
             if two:
                 need(O[slot] == {(n, j) for j in mine}, "O at the end")
             else:
@@ -264,36 +260,39 @@ def run_kernel(items, seed, fp8, stages=None, scales=4, merge_wait=True, always_
             finished.append((n, slot, q))
             n += 1
 
-    def pipe_step():
+    def pipe_step(pipe):
         op = pipe.pop(0)
         if op[0] == "commit":
             B[op[1]].arrive()
         elif op[0] == "QK":
             _, n, j, slot, st = op
-            need(Q == [n, n], "Q tile")
+            need(set(Q) == {n}, "Q tile")
             need(all(v == ("K", n, j) for v in kv[st]), "K tile")
-            S[slot][:] = [("S", n, j)] * 4
+            S[:] = [(n, j, slot)] * 4
         else:
             _, n, j, slot, st, fresh = op
-            need(S[slot] == [("P", n, j)] * 4, f"P {S[slot]}")
+            need(P[slot] == [(n, j)] * 4, f"P {P[slot]}")
             need(all(v == ("V", n, j) for v in kv[st]), "V tile")
             if fresh:
                 O[slot].clear()
             O[slot].add((n, j))
 
-    actors = [items_role(), q_role(), copy_role(), mma()]
+    actors = [items_role(), qk_role(), pv_role()]
+    actors += [copy_role(None)] if fp8 else [copy_role(0), copy_role(1)] + [q_role(w) for w in range(3)]
     actors += [softmax(s, q) for s in range(2) for q in range(4)]
     if fp8:
         actors += [widen_role(w) for w in range(4)]
     live = {i: (a, None) for i, a in enumerate(actors)}
-    weight = [rng.choice([1, 1, 3, 10]) for _ in range(len(actors) + 2)]
-    while live or tma or pipe:
+    weight = [rng.choice([1, 1, 3, 10]) for _ in range(len(actors) + 3)]
+    while live or tma or qk_pipe or pv_pipe:
         ready = [i for i, (_, p) in live.items() if p is None or p()]
         ops = [(i, weight[i]) for i in ready]
         if tma:
             ops.append(("tma", weight[-1]))
-        if pipe:
-            ops.append(("pipe", weight[-2]))
+        if qk_pipe:
+            ops.append(("qk", weight[-2]))
+        if pv_pipe:
+            ops.append(("pv", weight[-3]))
         if not ops:
             raise Race("hang")
         pick = rng.choices([o for o, _ in ops], [w for _, w in ops])[0]
@@ -301,8 +300,8 @@ def run_kernel(items, seed, fp8, stages=None, scales=4, merge_wait=True, always_
             mem, at, val, bar = tma.pop(rng.randrange(len(tma)))
             mem[at] = val
             B[bar].complete_tx(1)
-        elif pick == "pipe":
-            pipe_step()
+        elif pick in ("qk", "pv"):
+            pipe_step(qk_pipe if pick == "qk" else pv_pipe)
         else:
             a = live[pick][0]
             try:
@@ -329,11 +328,18 @@ def test_the_model_sees_a_missing_wait():
             run_kernel([(False, 2)] * 4, seed, False, merge_wait=False)
 
 
-def test_the_model_sees_an_unwatched_phase():
-    """A commit to the barrier of a slot that has no tile of the item can complete two phases unseen."""
+def test_the_model_sees_an_arrival_too_early():
+    """A warp without rows that does not wait for its slot's P.V can end the phase of the tile before."""
     with pytest.raises(Race):
-        for seed in range(800):
-            run_kernel([(True, 2), (False, 1), (True, 2), (False, 1)], seed, False, always_commit=True)
+        for seed in range(400):
+            run_kernel([(True, 6)] * 2, seed, False, idle_wait=False)
+
+
+def test_the_model_sees_a_ring_with_two_copiers():
+    """One ring for K and V of an odd number of stages: each copier sees every second phase of a barrier only."""
+    with pytest.raises(Race):
+        for seed in range(300):
+            run_kernel([(True, 9)] * 2, seed, False, shared_ring=True)
 
 
 def test_the_model_sees_too_few_scale_buffers():

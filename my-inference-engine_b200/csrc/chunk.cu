@@ -28,19 +28,19 @@
 //   3      walks the range and hands the items out
 //   4-7    softmax of slot A, 8-11 of slot B: a thread owns a tile row
 //   13-15  write the items' Q tiles to shared memory
-//   12-15  (FP8) do so as f16 of q / 16, and widen e4m3 to f16 tiles (exact)
+//   12-15  (FP8) do so as f16 of q / 16, and widen K and V to f16 tiles
 // Two slots, each with a P and an O tile in tensor memory, share one S tile:
 // softmax warps take S into registers and free it at once, so the next Q.K
 // (the other slot's) runs under their exponentials.  An item of more than 128
 // rows gives each slot one of its two tiles (the K/V tiles are shared); a
 // smaller one gives the slots alternate key tiles and joins them at its end.
 //
-// P, as 16-bit pairs, is the A operand from tensor memory.
-//  bf16 pool: P in bf16.  FP8 pool: scores are scaled per key, and
-// the value scale goes into the exponent, p' = 2^(s + log2 vs - base), so
-// that P'V needs no scale; l sums p' / vs.  P' in f16 against base = max - 7
-// (at most 2^15 with the lazy maximum): 11 bits, and 2^-29 of the largest
-// term before a term falls below f16's normal range.
+// P, as 16-bit pairs, is the A operand from tensor memory: bf16, and f16 over
+// the FP8 pool, whose e4m3 keys and values are widened to f16 with their scale
+// applied (a score or probability then needs no scale of its own; as columns
+// of S the scales cost every softmax thread 96 loads a tile).  f16's range is
+// used up to 2^(8 + 7): base = maximum - 7, so a term keeps 11 bits down to
+// 2^-21 of the largest and is off by at most 2^-32 of it below.
 #include <math.h>
 
 #include "pkv_device.cuh"
@@ -62,7 +62,7 @@ constexpr float kP8Shift = 7.f;   // FP8: P' up to 2^(8 + 7)
 constexpr int kItemCost = 384;
 constexpr int kMinStep = kItemCost + 4 * kKeys;
 constexpr int kItemRing = 3;
-constexpr int kGroup = 4;  // FP8: blocks to a copy barrier
+constexpr int kGroup = 2;  // FP8: blocks to a copy barrier
 // tensor memory columns: S, then each slot's P, then each slot's O
 constexpr uint32_t kColP = 128, kColO = 256;
 
@@ -73,16 +73,16 @@ struct Cfg {
   // 32 KiB tiles; a ring each, so that no barrier is polled by two copiers of
   // whom each sees every second phase only
   static constexpr int kKStages = kFp8 ? 2 : 3, kVStages = 2;
-  static constexpr int kRaw = kFp8 ? 3 : 0;     // groups of kGroup chunks in flight
+  static constexpr int kRaw = kFp8 ? 7 : 0;     // groups of kGroup chunks in flight
   static constexpr int kOffQ = 0;
   static constexpr int kOffK = kOffQ + kTiles * kOperand;
   static constexpr int kOffV = kOffK + kKStages * kOperand;
   static constexpr int kOffRaw = kOffV + kVStages * kOperand;
-  static constexpr int kOffScale = kOffRaw + kRaw * kGroup * kFp8HeadBlockBytes;  // [4][3][128]
-  static constexpr int kOffMl = kOffScale + (kFp8 ? 4 * 3 * kKeys * 4 : 0);  // [2][128] float2
+  static constexpr int kOffScale = kOffRaw + kRaw * kGroup * kFp8HeadBlockBytes;  // [4 warps][128] f16
+  static constexpr int kOffMl = kOffScale + (kFp8 ? 4 * kKeys * 2 : 0);  // [2][128] float2
   static constexpr int kOffItem = kOffMl + 2 * kRows * 8;
   static constexpr int kOffBar = kOffItem + kItemRing * 64;
-  static constexpr int kBars = 2 * kItemRing + 2 + 2 * (kKStages + kVStages) + 7 + 3 + 2 * kRaw + 4;
+  static constexpr int kBars = 2 * kItemRing + 2 + 2 * (kKStages + kVStages) + 7 + 3 + 2 * kRaw;
   static constexpr int kOffScan = kOffBar + kBars * 8 + 16;  // 16 warp sums, base, row
   static constexpr int kSmem = kOffScan + 18 * 8;
   // setmaxnreg: the warpgroups' shares of the launch's 128 per thread
@@ -288,7 +288,7 @@ struct Ctx {
   using C = Cfg<kFp8>;
   uint8_t* smem;
   uint64_t *item_full, *item_empty, *q_full, *q_free, *k_full, *k_empty, *v_full, *v_empty, *s_full, *s_free, *p_full,
-      *pv_done, *ml_bar, *ep_bar, *mma_done, *raw_full, *raw_empty, *sc_full;
+      *pv_done, *ml_bar, *ep_bar, *mma_done, *raw_full, *raw_empty;
   DevErr err;
 
   __device__ Ctx(uint8_t* s, int32_t* e) : smem(s), err{e} {
@@ -315,7 +315,6 @@ struct Ctx {
     mma_done = take(1);
     raw_full = take(C::kRaw);
     raw_empty = take(C::kRaw);
-    sc_full = take(4);
   }
   __device__ uint32_t* tmem_slot() const {
     return reinterpret_cast<uint32_t*>(smem + C::kOffBar + C::kBars * 8);
@@ -438,13 +437,6 @@ __device__ __forceinline__ void fma2(float& x0, float& x1, float a0, float a1, f
       : "+f"(x0), "+f"(x1)
       : "f"(a0), "f"(a1), "f"(b0), "f"(b1));
 }
-__device__ __forceinline__ void fma2_to(float& y0, float& y1, float a0, float a1, float b0,
-                                        float b1) {
-  asm("{\n\t.reg .b64 y, a, b;\n\tmov.b64 y, {%0, %1};\n\tmov.b64 a, {%2, %3};\n\t"
-      "mov.b64 b, {%4, %5};\n\tfma.rn.f32x2 y, a, b, y;\n\tmov.b64 {%0, %1}, y;\n\t}"
-      : "+f"(y0), "+f"(y1)
-      : "f"(a0), "f"(a1), "f"(b0), "f"(b1));
-}
 __device__ __forceinline__ void add2(float& x0, float& x1, float a0, float a1) {
   asm("{\n\t.reg .b64 x, a;\n\tmov.b64 x, {%0, %1};\n\tmov.b64 a, {%2, %3};\n\t"
       "add.rn.f32x2 x, x, a;\n\tmov.b64 {%0, %1}, x;\n\t}"
@@ -470,7 +462,6 @@ __device__ void softmax_role(const ChunkParams& p, const Ctx<kFp8>& x, uint32_t 
   const int rtok = r / p.group, rhead = r - rtok * p.group;
   float2* ml = reinterpret_cast<float2*>(x.smem + C::kOffMl);
   uint32_t n_tile = 0, n_ml = 0;  // tiles of this slot, joins of the two slots so far
-  uint32_t n_key = 0;                         // key tiles of all items so far (FP8 scale ring)
   for (int n = 0;; ++n) {
     Item it;
     if (!x.next(n, it) || it.t1 < 0) return;
@@ -502,19 +493,6 @@ __device__ void softmax_role(const ChunkParams& p, const Ctx<kFp8>& x, uint32_t 
         __syncwarp();
         if (lane == 0) mbar_arrive(x.s_free);
         const int left = lim - j * kKeys;  // visible keys of this tile
-        const float* sc = nullptr;
-        if constexpr (kFp8) {
-          const uint32_t kt = n_key + (j - it.t0);
-          if (!x.wait_warp(&x.sc_full[kt & 3], kt >> 2)) return;
-          sc = reinterpret_cast<const float*>(x.smem + C::kOffScale) + (kt & 3) * 3 * kKeys;
-#pragma unroll
-          for (int i = 0; i < 128; i += 4) {
-            const float4 a = *reinterpret_cast<const float4*>(sc + i);
-            const float4 b = *reinterpret_cast<const float4*>(sc + kKeys + i);
-            fma2(s[i + 0], s[i + 1], a.x, a.y, b.x, b.y);
-            fma2(s[i + 2], s[i + 3], a.z, a.w, b.z, b.w);
-          }
-        }
         if (left < kKeys) {
 #pragma unroll
           for (int i = 0; i < 128; ++i)
@@ -528,7 +506,7 @@ __device__ void softmax_role(const ChunkParams& p, const Ctx<kFp8>& x, uint32_t 
 #pragma unroll
           for (int u = 0; u < 4; ++u) pm[u] = fmaxf(fmaxf(pm[u], s[i + u]), s[i + u + 4]);
         float mx = fmaxf(fmaxf(pm[0], pm[1]), fmaxf(pm[2], pm[3]));
-        if constexpr (!kFp8) mx *= p.scale_log2;
+        mx *= p.scale_log2;
         // the running maximum moves only by more than 2^8
         const float mn = (mx > m + kLazyLog2 || m == -INFINITY) ? mx : m;
         const float alpha = mn == m ? 1.f : ex2(m - mn);  // 0 from m = -inf
@@ -542,27 +520,14 @@ __device__ void softmax_role(const ChunkParams& p, const Ctx<kFp8>& x, uint32_t 
 #pragma unroll
           for (int i = 0; i < 32; i += 4) {
             float* e = s + c * 32 + i;
-            if constexpr (kFp8) {
-              add2(e[0], e[1], -base, -base);
-              add2(e[2], e[3], -base, -base);
-            } else {
-              fma2(e[0], e[1], p.scale_log2, p.scale_log2, -base, -base);
-              fma2(e[2], e[3], p.scale_log2, p.scale_log2, -base, -base);
-            }
+            fma2(e[0], e[1], p.scale_log2, p.scale_log2, -base, -base);
+            fma2(e[2], e[3], p.scale_log2, p.scale_log2, -base, -base);
 #pragma unroll
             for (int u = 0; u < 4; ++u) e[u] = ex2(e[u]);
-            if constexpr (kFp8) {
-              const float4 iv = *reinterpret_cast<const float4*>(sc + 2 * kKeys + c * 32 + i);
-              fma2_to(ps[0], ps[1], e[0], e[1], iv.x, iv.y);
-              fma2_to(ps[2], ps[3], e[2], e[3], iv.z, iv.w);
-              pk[i / 2] = pack_f16(e[0], e[1]);
-              pk[i / 2 + 1] = pack_f16(e[2], e[3]);
-            } else {
-              add2(ps[0], ps[1], e[0], e[1]);
-              add2(ps[2], ps[3], e[2], e[3]);
-              pk[i / 2] = pack_bf16(e[0], e[1]);
-              pk[i / 2 + 1] = pack_bf16(e[2], e[3]);
-            }
+            add2(ps[0], ps[1], e[0], e[1]);
+            add2(ps[2], ps[3], e[2], e[3]);
+            pk[i / 2] = kFp8 ? pack_f16(e[0], e[1]) : pack_bf16(e[0], e[1]);
+            pk[i / 2 + 1] = kFp8 ? pack_f16(e[2], e[3]) : pack_bf16(e[2], e[3]);
           }
           if (c == 0) {  // P and O are the slot's again once its last P.V is done
             if (!first && !x.wait_warp(&x.pv_done[slot], n_tile - 2)) return;
@@ -571,9 +536,7 @@ __device__ void softmax_role(const ChunkParams& p, const Ctx<kFp8>& x, uint32_t 
           tmem_st16u(col_p + c * 16, pk);
         }
         l = l * alpha + ((ps[0] + ps[1]) + (ps[2] + ps[3]));
-        // (l is never negative: with it the vote uses every scale read, which
-        // the arrive below must not overtake)
-        if (__any_sync(0xffffffffu, alpha != 1.f || l < 0.f) && !first) {
+        if (!first && __any_sync(0xffffffffu, alpha != 1.f)) {
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
             float v[32];
@@ -594,7 +557,6 @@ __device__ void softmax_role(const ChunkParams& p, const Ctx<kFp8>& x, uint32_t 
       __syncwarp();
       if (lane == 0) mbar_arrive(&x.p_full[slot]);
     }
-    n_key += it.t1 - it.t0;
     // ---- end of the item
     if (!first && !x.wait_warp(&x.pv_done[slot], n_tile - 1)) return;
     tc_fence_after();
@@ -902,16 +864,44 @@ __device__ void copy_role(const ChunkParams& p, const Ctx<true>& x) {
 }
 
 // ---------------------------------------------------------------- FP8 widening
-// Warps 12-15: thread c of 128.  K: one 16-byte group (token t, dims 16g ..)
-// per block; the lanes of a quarter-warp take tokens t and t ^ 5 with four
-// groups each, which keeps both the load (group ^ t) and the two stores
-// (chunk 2g + h ^ t) free of bank conflicts.  V is stored by dim, so its tile
-// is K-major with the keys contiguous; thread = dim.
-__device__ __forceinline__ void widen16(const uint4 raw, uint4& lo, uint4& hi) {
-  e4m3x4_to_f16x2x2(raw.x, lo.x, hi.x);
-  e4m3x4_to_f16x2x2(raw.y, lo.y, hi.y);
-  e4m3x4_to_f16x2x2(raw.z, lo.z, hi.z);
-  e4m3x4_to_f16x2x2(raw.w, lo.w, hi.w);
+// Warps 12-15: e4m3 * scale as f16 (the chunks hold 4 bits, f16 holds 11).
+// The scale is taken times 2^8 and the e4m3 value times 2^-8 (exact), so that
+// rows down to 1e-4 in size still have a normal f16 scale.  A key's scale is
+// two f16 terms: rounded to one it would move all of the key's products, and
+// so its score, by up to 2^-12 together, where their own roundings average
+// out.  For a value that is one more rounding among many.
+// K: one 16-byte group (token t, dims 16g ..) per block and thread; the lanes
+// of a quarter-warp take tokens t and t ^ 5 with four groups each, which keeps
+// both the load (group ^ t) and the two stores (chunk 2g + h ^ t) free of bank
+// conflicts.  V is stored by dim, so its tile is K-major with the keys
+// contiguous; thread = dim.
+__device__ __forceinline__ __half2 as_half2(uint32_t x) {
+  return *reinterpret_cast<const __half2*>(&x);
+}
+__device__ __forceinline__ uint32_t as_u32(__half2 x) {
+  return *reinterpret_cast<const uint32_t*>(&x);
+}
+// Four e4m3 bytes -> elements (2i, 2i + 1) and (2i + 8, 2i + 9), times 2^-8.
+__device__ __forceinline__ void widen4(uint32_t four, __half2& lo, __half2& hi) {
+  constexpr uint32_t kDown = 0x1c001c00u;  // 2^-8, twice
+  uint32_t a, b;
+  e4m3x4_to_f16x2x2(four, a, b);
+  lo = __hmul2(as_half2(a), as_half2(kDown));
+  hi = __hmul2(as_half2(b), as_half2(kDown));
+}
+__device__ __forceinline__ void widen_k(uint32_t four, __half2 s, __half2 rest, uint32_t& lo,
+                                        uint32_t& hi) {
+  __half2 a, b;
+  widen4(four, a, b);
+  lo = as_u32(__hfma2(a, s, __hmul2(a, rest)));
+  hi = as_u32(__hfma2(b, s, __hmul2(b, rest)));
+}
+__device__ __forceinline__ void widen_v(uint32_t four, uint32_t s_lo, uint32_t s_hi, uint32_t& lo,
+                                        uint32_t& hi) {
+  __half2 a, b;
+  widen4(four, a, b);
+  lo = as_u32(__hmul2(a, as_half2(s_lo)));
+  hi = as_u32(__hmul2(b, as_half2(s_hi)));
 }
 
 // The 16-bit halves of a pair (tokens t, t + 1) that lie before `valid`.
@@ -929,8 +919,10 @@ __device__ void widen_role(const ChunkParams& p, const Ctx<true>& x, int tpt) {
   const uint32_t k_dst = (grp >> 2) * kRegion + tok * 128;
   const uint32_t k_lo = ((((grp & 3) * 2) ^ (tok & 7)) << 4);
   const uint32_t k_hi = ((((grp & 3) * 2 + 1) ^ (tok & 7)) << 4);
+  // this warp's copy of the tile's V scales, f16
+  uint8_t* v_scale = x.smem + C::kOffScale + (c >> 5) * kKeys * 2;
   uint32_t key = 0, n_load = 0;  // key tiles, Q tiles so far
-  RingPos<C::kRaw> g;            // the copy group of the tile's first block
+  RingPos<C::kRaw> g;            // the next copy group
   RingPos<C::kKStages> k;
   RingPos<C::kVStages> v;
   for (int n = 0;; ++n) {
@@ -948,86 +940,89 @@ __device__ void widen_role(const ChunkParams& p, const Ctx<true>& x, int tpt) {
     const int nblk = (it.key_end + kBlockTokens - 1) / kBlockTokens;
     for (int j = 0; j < nt; ++j) {
       const int b0 = (it.t0 + j) * kTileBlocks, nb = min(kTileBlocks, nblk - b0);
-      // ---- K tile and the keys' scales
+      // ---- K tile, group by group of blocks as they land, and the V scales
       if (key >= C::kKStages && !x.wait_warp(&x.k_empty[k.st], k.ph ^ 1)) return;
-      uint8_t* dst = x.smem + C::kOffK + k.st * kOperand;
-      const bool second = nb > kGroup;  // the tile has blocks in two groups
-      RingPos<C::kRaw> g2 = g;
-      g2.next();
-      if (!x.wait_warp(&x.raw_full[g.st], g.ph)) return;
-      if (second && !x.wait_warp(&x.raw_full[g2.st], g2.ph)) return;
-      const uint8_t* raw0 = x.smem + C::kOffRaw + g.st * kGroup * kFp8HeadBlockBytes;
-      const uint8_t* raw1 = x.smem + C::kOffRaw + g2.st * kGroup * kFp8HeadBlockBytes -
-                            kGroup * kFp8HeadBlockBytes;  // block b of the tile, b >= kGroup
-#pragma unroll 4
-      for (int b = 0; b < nb; ++b) {
-        const uint8_t* src = (b < kGroup ? raw0 : raw1) + b * kFp8HeadBlockBytes;
-        uint4 lo, hi;
-        widen16(*reinterpret_cast<const uint4*>(src + k_src), lo, hi);
-        *reinterpret_cast<uint4*>(dst + k_dst + b * 2048 + k_lo) = lo;
-        *reinterpret_cast<uint4*>(dst + k_dst + b * 2048 + k_hi) = hi;
-      }
-      {
-        float ks = 0.f, lv = 0.f, iv = 0.f;
-        const int pos = b0 * kBlockTokens + c;
-        if (c < nb * kBlockTokens && pos < it.kv) {
-          const int b = c / kBlockTokens;
-          const float* sc = reinterpret_cast<const float*>(
-              (b < kGroup ? raw0 : raw1) + b * kFp8HeadBlockBytes + kFp8KScaleOff);
-          ks = sc[c % kBlockTokens] * (16.f * p.scale_log2);
-          // a value row below 2^-91 in size counts as if at that scale
-          const float vs = fmaxf(sc[16 + c % kBlockTokens], 0x1p-100f);
-          lv = log2f(vs);
-          iv = 1.f / vs;
+      uint8_t* dst = x.smem + C::kOffK + k.st * kOperand + k_dst;
+      RingPos<C::kRaw> q = g;
+      for (int b = 0; b < nb; b += kGroup, q.next()) {
+        if (!x.wait_warp(&x.raw_full[q.st], q.ph)) return;
+        const uint8_t* src = x.smem + C::kOffRaw + q.st * kGroup * kFp8HeadBlockBytes;
+        uint4 raw[kGroup];
+        float ks[kGroup];
+#pragma unroll
+        for (int u = 0; u < kGroup; ++u) {  // (a last odd block: stale bytes, masked keys)
+          raw[u] = *reinterpret_cast<const uint4*>(src + u * kFp8HeadBlockBytes + k_src);
+          ks[u] = *reinterpret_cast<const float*>(src + u * kFp8HeadBlockBytes + kFp8KScaleOff +
+                                                  tok * 4);
         }
-        float* sc = reinterpret_cast<float*>(x.smem + C::kOffScale) + (key & 3) * 3 * kKeys;
-        sc[c] = ks;
-        sc[kKeys + c] = lv;
-        sc[2 * kKeys + c] = iv;
+        if (lane < kGroup * 4) {  // lane: four tokens of a block
+          const int u = lane >> 2, t = (lane & 3) * 4;
+          const float4 s = *reinterpret_cast<const float4*>(src + u * kFp8HeadBlockBytes +
+                                                            kFp8VScaleOff + t * 4);
+          *reinterpret_cast<uint2*>(v_scale + ((b + u) * kBlockTokens + t) * 2) =
+              make_uint2(pack_f16(s.x * 256.f, s.y * 256.f), pack_f16(s.z * 256.f, s.w * 256.f));
+        }
+#pragma unroll
+        for (int u = 0; u < kGroup; ++u) {
+          const float up = ks[u] * 256.f;
+          const __half2 sc = __float2half2_rn(up);
+          const __half2 rest = __float2half2_rn(up - __low2float(sc));
+          uint4 lo, hi;
+          widen_k(raw[u].x, sc, rest, lo.x, hi.x);
+          widen_k(raw[u].y, sc, rest, lo.y, hi.y);
+          widen_k(raw[u].z, sc, rest, lo.z, hi.z);
+          widen_k(raw[u].w, sc, rest, lo.w, hi.w);
+          *reinterpret_cast<uint4*>(dst + (b + u) * 2048 + k_lo) = lo;
+          *reinterpret_cast<uint4*>(dst + (b + u) * 2048 + k_hi) = hi;
+        }
       }
       fence_async_smem();
       __syncwarp();
-      if (lane == 0) {
-        mbar_arrive(&x.sc_full[key & 3]);
-        mbar_arrive(&x.k_full[k.st]);
-      }
+      if (lane == 0) mbar_arrive(&x.k_full[k.st]);
       k.next();
       // ---- V tile
       if (key >= C::kVStages && !x.wait_warp(&x.v_empty[v.st], v.ph ^ 1)) return;
-      dst = x.smem + C::kOffV + v.st * kOperand;
-#pragma unroll 4
-      for (int b = 0; b < nb; ++b) {
-        const uint8_t* src = (b < kGroup ? raw0 : raw1) + b * kFp8HeadBlockBytes + kFp8VOff;
-        uint4 lo, hi;
-        widen16(*reinterpret_cast<const uint4*>(src + c * 16), lo, hi);
-        const int valid = it.kv - (b0 + b) * kBlockTokens;
-        if (valid < kBlockTokens) {  // no position there: zeros for P's zeros
-          lo.x = keep_pair(lo.x, 0, valid);
-          lo.y = keep_pair(lo.y, 2, valid);
-          lo.z = keep_pair(lo.z, 4, valid);
-          lo.w = keep_pair(lo.w, 6, valid);
-          hi.x = keep_pair(hi.x, 8, valid);
-          hi.y = keep_pair(hi.y, 10, valid);
-          hi.z = keep_pair(hi.z, 12, valid);
-          hi.w = keep_pair(hi.w, 14, valid);
+      dst = x.smem + C::kOffV + v.st * kOperand + c * 128;
+      for (int b = 0; b < nb; b += kGroup, g.next()) {
+        const uint8_t* src = x.smem + C::kOffRaw + g.st * kGroup * kFp8HeadBlockBytes + kFp8VOff;
+        uint4 raw[kGroup];
+#pragma unroll
+        for (int u = 0; u < kGroup; ++u)
+          raw[u] = *reinterpret_cast<const uint4*>(src + u * kFp8HeadBlockBytes + c * 16);
+#pragma unroll
+        for (int u = 0; u < kGroup; ++u) {
+          const uint4 sl = *reinterpret_cast<const uint4*>(v_scale + (b + u) * 32);
+          const uint4 sh = *reinterpret_cast<const uint4*>(v_scale + (b + u) * 32 + 16);
+          uint4 lo, hi;
+          widen_v(raw[u].x, sl.x, sh.x, lo.x, hi.x);
+          widen_v(raw[u].y, sl.y, sh.y, lo.y, hi.y);
+          widen_v(raw[u].z, sl.z, sh.z, lo.z, hi.z);
+          widen_v(raw[u].w, sl.w, sh.w, lo.w, hi.w);
+          const int valid = it.kv - (b0 + b + u) * kBlockTokens;
+          if (valid < kBlockTokens) {  // no position there: zeros for P's zeros
+            lo.x = keep_pair(lo.x, 0, valid);
+            lo.y = keep_pair(lo.y, 2, valid);
+            lo.z = keep_pair(lo.z, 4, valid);
+            lo.w = keep_pair(lo.w, 6, valid);
+            hi.x = keep_pair(hi.x, 8, valid);
+            hi.y = keep_pair(hi.y, 10, valid);
+            hi.z = keep_pair(hi.z, 12, valid);
+            hi.w = keep_pair(hi.w, 14, valid);
+          }
+          uint8_t* row = dst + ((b + u) >> 2) * kRegion;
+          *reinterpret_cast<uint4*>(row + (((((b + u) & 3) * 2) ^ (c & 7)) << 4)) = lo;
+          *reinterpret_cast<uint4*>(row + (((((b + u) & 3) * 2 + 1) ^ (c & 7)) << 4)) = hi;
         }
-        uint8_t* row = dst + (b >> 2) * kRegion + c * 128;
-        *reinterpret_cast<uint4*>(row + ((((b & 3) * 2) ^ (c & 7)) << 4)) = lo;
-        *reinterpret_cast<uint4*>(row + ((((b & 3) * 2 + 1) ^ (c & 7)) << 4)) = hi;
+        // behind the stores: every load of the chunks has returned by then,
+        // which an arrive right behind the loads would not wait for
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&x.raw_empty[g.st]);
       }
       fence_async_smem();
       __syncwarp();
-      if (lane == 0) {
-        // behind the stores: every load of the chunks has returned by then,
-        // which an arrive right behind the loads would not wait for
-        mbar_arrive(&x.v_full[v.st]);
-        mbar_arrive(&x.raw_empty[g.st]);
-        if (second) mbar_arrive(&x.raw_empty[g2.st]);
-      }
+      if (lane == 0) mbar_arrive(&x.v_full[v.st]);
       v.next();
       ++key;
-      g.next();
-      if (second) g.next();
     }
   }
 }
@@ -1184,7 +1179,6 @@ __global__ void __launch_bounds__(Cfg<kFp8>::kThreads, 1)
       mbar_init(&x.raw_full[i], 1);
       mbar_init(&x.raw_empty[i], 4);
     }
-    for (int i = 0; i < 4; ++i) mbar_init(&x.sc_full[i], 4);
     fence_mbar_init();
     s_row = p.batch;
     s_base = 0;
@@ -1403,7 +1397,7 @@ cudaError_t launch_chunk(const ChunkLaunch& a, cudaStream_t stream) {
   p.group = a.num_q_heads / a.num_kv_heads;
   p.num_blocks = a.num_blocks;
   p.causal = a.causal;
-  p.scale_log2 = a.sm_scale * 1.4426950408889634f;
+  p.scale_log2 = a.sm_scale * 1.4426950408889634f * (fp8 ? 16.f : 1.f);  // FP8: q / 16
   p.err = a.err;
   p.part_rows = pl.part_rows;
   if (pl.grid > 1) {

@@ -8,6 +8,11 @@ step), 2^-8 A; scores are fp32 sums of 128 products, off by at most
 130 * 2^-24 * S with S = scale * sum |q_d k_d|, which moves p by twice that
 relatively, and ex2, the sums over keys and the running rescale add a few
 2^-22 each: 2^-16 A covers them up to 64 rescales.
+
+The FP8 kernel takes e4m3 * scale as f16.  A key element is off by at most
+2^-12 of itself (one rounding to 11 bits; the scale is held in two terms), so a
+score by 2^-12 S and p by twice that relatively; a value element by 2^-12 for
+its scale and 2^-12 for the product, 2^-11 A in all.
 """
 import math
 
@@ -123,7 +128,10 @@ def plain(c, causal=True):
             A = torch.einsum("hts,shd->thd", p, v.abs())
             S = big.amax(-1).transpose(0, 1)[..., None] if n else 0.0
             o[at + a:at + z] = oo
-            tol[at + a:at + z] = 2.0 ** -8 * oo.abs() + (2.0 ** -8 + 2.0 ** -16 + 2 * 130 * 2.0 ** -24 * S) * A
+            rel = 2.0 ** -8 + 2.0 ** -16 + 2 * 130 * 2.0 ** -24 * S
+            if c["fmt"] == "fp8":
+                rel = rel + 2 * 2.0 ** -12 * S + 2.0 ** -11
+            tol[at + a:at + z] = 2.0 ** -8 * oo.abs() + rel * A
         at += t
     return o, tol
 

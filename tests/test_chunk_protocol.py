@@ -20,11 +20,11 @@ from test_prefill_protocol import Barrier, Race
 RING = 3
 
 
-def run_kernel(items, seed, fp8, shared_ring=False, scales=4, merge_wait=True, idle_wait=True):
+def run_kernel(items, seed, fp8, shared_ring=False, merge_wait=True, idle_wait=True):
     """items: [(two, nt)].  Raises Race on a wrong read, a lost update or a hang."""
     rng = random.Random(seed)
     k_stages, v_stages = (2, 2) if fp8 else (3, 2)
-    raws = 3  # groups of four chunks
+    raws = 7  # groups of two chunks
     B = {"q_full": Barrier(4 if fp8 else 3), "q_free": Barrier(1), "ml": Barrier(8), "ep": Barrier(8)}
     for i in range(RING):
         B[f"item_full{i}"], B[f"item_empty{i}"] = Barrier(1), Barrier(15)
@@ -42,13 +42,10 @@ def run_kernel(items, seed, fp8, shared_ring=False, scales=4, merge_wait=True, i
         B[f"s_full{s}"], B[f"p_full{s}"], B[f"pv_done{s}"] = Barrier(1), Barrier(4), Barrier(1)
     for i in range(raws):
         B[f"raw_full{i}"], B[f"raw_empty{i}"] = Barrier(1), Barrier(4)
-    for i in range(4):
-        B[f"sc_full{i}"] = Barrier(4)
     item_ring = [None] * RING
     Q = [None] * (4 if fp8 else 3)
     kv = [[None] * 4 for _ in range(k_stages + v_stages)]  # per widening warp; the copy engine writes all four
     raw = [None] * raws
-    sc = [[None] * 4 for _ in range(scales)]
     S = [None] * 4
     P = [[None] * 4 for _ in range(2)]
     O = [set(), set()]
@@ -105,7 +102,7 @@ def run_kernel(items, seed, fp8, shared_ring=False, scales=4, merge_wait=True, i
                 return
             for j in range(it[1]):
                 if fp8:
-                    for g in range(2):
+                    for g in range(4):
                         st = t % raws
                         if t >= raws:
                             yield wait(f"raw_empty{st}", t // raws - 1)
@@ -124,7 +121,7 @@ def run_kernel(items, seed, fp8, shared_ring=False, scales=4, merge_wait=True, i
             n += 1
 
     def widen_role(w):
-        n = r = key = n_load = 0
+        n = r = n_load = 0
         while True:
             it = yield from nxt(n)
             if it[1] < 0:
@@ -134,10 +131,10 @@ def run_kernel(items, seed, fp8, shared_ring=False, scales=4, merge_wait=True, i
                 n_load += 1
             for j in range(it[1]):
                 for what in "KV":
-                    st, use = ring("KV".index(what), r // 2)
+                    st, use = ring("KV".index(what), r // 4)
                     if use:
                         yield wait(f"kv_empty{st}", use - 1)
-                    for g in range(2):
+                    for g in range(4):
                         rs = (r + g) % raws
                         if what == "K":
                             yield wait(f"raw_full{rs}", (r + g) // raws)
@@ -145,18 +142,12 @@ def run_kernel(items, seed, fp8, shared_ring=False, scales=4, merge_wait=True, i
                         if rng.random() < 0.2:
                             yield None
                         need(raw[rs] == (n, j, g), "raw chunks while read")
+                        if what == "V":
+                            B[f"raw_empty{rs}"].arrive()
                     kv[st][w] = (what, n, j)
-                    if what == "K":
-                        sc[key % scales][w] = key
-                        yield None
-                        B[f"sc_full{key & 3}"].arrive()
-                        key += 1
-                    B[f"kv_full{st}"].arrive()
-                    if what == "V":
-                        B[f"raw_empty{r % raws}"].arrive()
-                        B[f"raw_empty{(r + 1) % raws}"].arrive()
                     yield None
-                r += 2
+                    B[f"kv_full{st}"].arrive()
+                r += 4
             n += 1
 
     def qk_role():
@@ -205,7 +196,7 @@ def run_kernel(items, seed, fp8, shared_ring=False, scales=4, merge_wait=True, i
             n += 1
 
     def softmax(slot, q):
-        n = n_tile = n_ml = n_key = 0
+        n = n_tile = n_ml = 0
         while True:
             it = yield from nxt(n)
             if it[1] < 0:
@@ -223,9 +214,6 @@ def run_kernel(items, seed, fp8, shared_ring=False, scales=4, merge_wait=True, i
                 yield None
                 need(S[q] == (n, j, slot), "S while it is taken")
                 B["s_free"].arrive()
-                if busy and fp8:
-                    yield wait(f"sc_full{(n_key + j) & 3}", (n_key + j) >> 2)
-                    need(all(v == n_key + j for v in sc[(n_key + j) % scales]), "scales")
                 if rng.random() < 0.5:
                     yield None
                 if a and (busy or idle_wait):
@@ -233,11 +221,8 @@ def run_kernel(items, seed, fp8, shared_ring=False, scales=4, merge_wait=True, i
                 if busy:
                     if a:
                         need(O[slot] == {(n, i) for i in mine[:a]}, "O during a rescale")
-                    if fp8:
-                        need(all(v == n_key + j for v in sc[(n_key + j) % scales]), "scales, second read")
                 P[slot][q] = (n, j)
                 B[f"p_full{slot}"].arrive()
-            n_key += nt
             if mine:
                 yield wait(f"pv_done{slot}", n_tile - 1)
             if two:
@@ -340,12 +325,6 @@ def test_the_model_sees_a_ring_with_two_copiers():
     with pytest.raises(Race):
         for seed in range(300):
             run_kernel([(True, 9)] * 2, seed, False, shared_ring=True)
-
-
-def test_the_model_sees_too_few_scale_buffers():
-    with pytest.raises(Race):
-        for seed in range(300):
-            run_kernel([(False, 9)] * 2, seed, True, scales=2)
 
 
 # ---------------------------------------------------------------- work split

@@ -62,7 +62,8 @@ constexpr float kP8Shift = 7.f;   // FP8: P' up to 2^(8 + 7)
 constexpr int kItemCost = 384;
 constexpr int kMinStep = kItemCost + 4 * kKeys;
 constexpr int kItemRing = 3;
-constexpr int kGroup = 2;  // FP8: blocks to a copy barrier
+// FP8: e4m3 bytes of a K or V tile, and four copies of its fp32 scales
+constexpr int kRawBytes = kKeys * kHeadDim + 4 * kKeys * 4;
 // tensor memory columns: S, then each slot's P, then each slot's O
 constexpr uint32_t kColP = 128, kColO = 256;
 
@@ -73,16 +74,16 @@ struct Cfg {
   // 32 KiB tiles; a ring each, so that no barrier is polled by two copiers of
   // whom each sees every second phase only
   static constexpr int kKStages = kFp8 ? 2 : 3, kVStages = 2;
-  static constexpr int kRaw = kFp8 ? 7 : 0;     // groups of kGroup chunks in flight
+  static constexpr int kRaw = kFp8 ? 3 : 0;  // FP8 tiles (K or V) read or in flight
   static constexpr int kOffQ = 0;
   static constexpr int kOffK = kOffQ + kTiles * kOperand;
   static constexpr int kOffV = kOffK + kKStages * kOperand;
   static constexpr int kOffRaw = kOffV + kVStages * kOperand;
-  static constexpr int kOffScale = kOffRaw + kRaw * kGroup * kFp8HeadBlockBytes;  // [4 warps][128] f16
-  static constexpr int kOffMl = kOffScale + (kFp8 ? 4 * kKeys * 2 : 0);  // [2][128] float2
+  static constexpr int kOffScale = kOffRaw + kRaw * kRawBytes;  // [4 warps][128] f16 scales
+  static constexpr int kOffMl = kOffScale + (kFp8 ? 4 * kKeys * 8 : 0);  // [2][128] float2
   static constexpr int kOffItem = kOffMl + 2 * kRows * 8;
   static constexpr int kOffBar = kOffItem + kItemRing * 64;
-  static constexpr int kBars = 2 * kItemRing + 2 + 2 * (kKStages + kVStages) + 7 + 3 + 2 * kRaw;
+  static constexpr int kBars = 2 * kItemRing + 2 + 2 * (kKStages + kVStages) + 7 + 3;
   static constexpr int kOffScan = kOffBar + kBars * 8 + 16;  // 16 warp sums, base, row
   static constexpr int kSmem = kOffScan + 18 * 8;
   // setmaxnreg: the warpgroups' shares of the launch's 128 per thread
@@ -92,6 +93,7 @@ struct Cfg {
   static constexpr int kRegsAux = kFp8 ? 72 : 40;    // warps 12-15
   static_assert(kRegsLow + 2 * kRegsSoftmax + kRegsAux <= 4 * kRegsLaunch,
                 "register split exceeds the launch allocation");
+  static_assert(kRaw <= 3, "landed() waits for at most two groups behind the oldest");
   static_assert(kSmem <= 227 * 1024, "shared memory exceeds the per-CTA limit");
 };
 
@@ -264,6 +266,22 @@ __device__ __forceinline__ void tma_load_5d(void* dst, const CUtensorMap* map, u
       : "memory");
 }
 
+// try_wait with a time hint: the warp sleeps until the phase completes or 1 ms
+// has passed.  Without one it comes back at once, and a dozen roles that poll
+// take the issue slots of the ones that work (a call then takes up to twice
+// as long).
+__device__ __forceinline__ bool suspend_on(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity), "r"(1000000u)
+      : "memory");
+  return ok != 0;
+}
+
 constexpr uint64_t kWaitNs = 4000000000ull;
 __device__ __forceinline__ uint64_t now_ns() {
   uint64_t t;
@@ -288,7 +306,7 @@ struct Ctx {
   using C = Cfg<kFp8>;
   uint8_t* smem;
   uint64_t *item_full, *item_empty, *q_full, *q_free, *k_full, *k_empty, *v_full, *v_empty, *s_full, *s_free, *p_full,
-      *pv_done, *ml_bar, *ep_bar, *mma_done, *raw_full, *raw_empty;
+      *pv_done, *ml_bar, *ep_bar, *mma_done;
   DevErr err;
 
   __device__ Ctx(uint8_t* s, int32_t* e) : smem(s), err{e} {
@@ -313,8 +331,6 @@ struct Ctx {
     ml_bar = take(1);
     ep_bar = take(1);
     mma_done = take(1);
-    raw_full = take(C::kRaw);
-    raw_empty = take(C::kRaw);
   }
   __device__ uint32_t* tmem_slot() const {
     return reinterpret_cast<uint32_t*>(smem + C::kOffBar + C::kBars * 8);
@@ -322,21 +338,19 @@ struct Ctx {
   __device__ Item* item(int n) const {
     return reinterpret_cast<Item*>(smem + C::kOffItem + (n % kItemRing) * 64);
   }
-  // Bounded by time: a role may wait for a whole item, nothing waits seconds.
-  __device__ bool wait(uint64_t* bar, uint32_t phase) const {
-    if (mbar_test(bar, phase & 1)) return true;
+  // A whole warp waits for a phase: false after kWaitNs (a role may wait for
+  // a whole item, nothing waits seconds).
+  __device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t phase) const {
+    if (__all_sync(0xffffffffu, suspend_on(bar, phase & 1))) return true;
+    return __all_sync(0xffffffffu, keep_waiting(bar, phase & 1));
+  }
+  __device__ bool keep_waiting(uint64_t* bar, uint32_t parity) const {
     const uint64_t t0 = now_ns();
     do {
-      for (int i = 0; i < 64; ++i)
-        if (mbar_test(bar, phase & 1)) return true;
+      if (suspend_on(bar, parity)) return true;
     } while (now_ns() - t0 < kWaitNs);
     err.raise(PKV_DEVERR_TIMEOUT);
     return false;
-  }
-  // A whole warp.
-  __device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t phase) const {
-    if (__all_sync(0xffffffffu, mbar_test(bar, phase & 1))) return true;
-    return __all_sync(0xffffffffu, wait(bar, phase));
   }
   // Item n, read by a whole warp; false after a wait that ran out.
   __device__ bool next(int n, Item& it) const {
@@ -763,6 +777,7 @@ struct BlockIds {
     }
     return id;
   }
+  __device__ BlockIds() : trow(nullptr), first(0), count(0), num_blocks(0), cur(0), nxt(0) {}
   __device__ BlockIds(const ChunkParams& p, const Item& it, const DevErr& err)
       : trow(p.tables + static_cast<int64_t>(it.table_row) * p.pitch),
         first(it.t0 * kTileBlocks),
@@ -818,90 +833,41 @@ __device__ void copy_role(const ChunkParams& p, const Ctx<false>& x, const CUten
   }
   if (!ok) {  // copies still in flight get a bounded time to land before the CTA ends
     for (uint32_t t = n_tile > kStages ? n_tile - kStages : 0; t < n_tile; ++t)
-      x.wait(&full[t % kStages], t / kStages);
+      x.wait_warp(&full[t % kStages], t / kStages);
   }
-}
-
-// FP8 pool: one bulk copy per block, four blocks to a barrier.
-__device__ void copy_role(const ChunkParams& p, const Ctx<true>& x) {
-  using C = Cfg<true>;
-  const int lane = threadIdx.x & 31;
-  const uint64_t keep = policy_evict_last();
-  RingPos<C::kRaw> r;
-  uint32_t n_group = 0;
-  bool ok = true;
-  for (int n = 0; ok; ++n) {
-    Item it;
-    ok = x.next(n, it);
-    if (!ok || it.t1 < 0) break;
-    if (it.t1 == it.t0) continue;
-    BlockIds ids(p, it, x.err);
-    for (int b0 = 0; b0 < ids.count; b0 += kGroup) {
-      if (b0 && (b0 & 31) == 0) ids.advance(b0, x.err);
-      if (n_group >= C::kRaw && !x.wait_warp(&x.raw_empty[r.st], r.ph ^ 1)) {
-        ok = false;
-        break;
-      }
-      const int nb = min(kGroup, ids.count - b0);
-      uint8_t* dst = x.smem + C::kOffRaw + r.st * kGroup * kFp8HeadBlockBytes;
-      if (lane == 0) mbar_arrive_expect_tx(&x.raw_full[r.st], nb * kFp8HeadBlockBytes);
-#pragma unroll
-      for (int b = 0; b < kGroup; ++b) {
-        const int id = ids.at(b0 + b);
-        if (lane == 0 && b < nb)
-          bulk_load(dst + b * kFp8HeadBlockBytes,
-                    p.kv8 + (static_cast<int64_t>(id) * p.hkv + it.kvh) * kFp8HeadBlockBytes,
-                    kFp8HeadBlockBytes, &x.raw_full[r.st], keep);
-      }
-      __syncwarp();
-      ++n_group;
-      r.next();
-    }
-  }
-  if (!ok)
-    for (uint32_t g = n_group > C::kRaw ? n_group - C::kRaw : 0; g < n_group; ++g)
-      x.wait(&x.raw_full[g % C::kRaw], g / C::kRaw);
 }
 
 // ---------------------------------------------------------------- FP8 widening
 // Warps 12-15: e4m3 * scale as f16 (the chunks hold 4 bits, f16 holds 11).
-// The scale is taken times 2^8 and the e4m3 value times 2^-8 (exact), so that
-// rows down to 1e-4 in size still have a normal f16 scale.  A key's scale is
-// two f16 terms: rounded to one it would move all of the key's products, and
-// so its score, by up to 2^-12 together, where their own roundings average
-// out.  For a value that is one more rounding among many.
+// A key's scale is two f16 terms: rounded to one it would move all of the
+// key's products, and so its score, by up to 2^-12 together, where their own
+// roundings average out.  For a value it is one more rounding among many.
+// These warps share the schedulers with the softmax, so what counts is the
+// number of instructions: the scales are rounded once per tile and warp.
 // K: one 16-byte group (token t, dims 16g ..) per block and thread; the lanes
 // of a quarter-warp take tokens t and t ^ 5 with four groups each, which keeps
-// both the load (group ^ t) and the two stores (chunk 2g + h ^ t) free of bank
-// conflicts.  V is stored by dim, so its tile is K-major with the keys
-// contiguous; thread = dim.
+// the two stores (chunk 2g + h ^ t) free of bank conflicts.  V is stored by
+// dim, so its tile is K-major with the keys contiguous; thread = dim.
 __device__ __forceinline__ __half2 as_half2(uint32_t x) {
   return *reinterpret_cast<const __half2*>(&x);
 }
 __device__ __forceinline__ uint32_t as_u32(__half2 x) {
   return *reinterpret_cast<const uint32_t*>(&x);
 }
-// Four e4m3 bytes -> elements (2i, 2i + 1) and (2i + 8, 2i + 9), times 2^-8.
-__device__ __forceinline__ void widen4(uint32_t four, __half2& lo, __half2& hi) {
-  constexpr uint32_t kDown = 0x1c001c00u;  // 2^-8, twice
+// Four e4m3 bytes -> elements (2i, 2i + 1) and (2i + 8, 2i + 9).
+__device__ __forceinline__ void widen_k(uint32_t four, uint32_t s, uint32_t rest, uint32_t& lo,
+                                        uint32_t& hi) {
   uint32_t a, b;
   e4m3x4_to_f16x2x2(four, a, b);
-  lo = __hmul2(as_half2(a), as_half2(kDown));
-  hi = __hmul2(as_half2(b), as_half2(kDown));
-}
-__device__ __forceinline__ void widen_k(uint32_t four, __half2 s, __half2 rest, uint32_t& lo,
-                                        uint32_t& hi) {
-  __half2 a, b;
-  widen4(four, a, b);
-  lo = as_u32(__hfma2(a, s, __hmul2(a, rest)));
-  hi = as_u32(__hfma2(b, s, __hmul2(b, rest)));
+  lo = as_u32(__hfma2(as_half2(a), as_half2(s), __hmul2(as_half2(a), as_half2(rest))));
+  hi = as_u32(__hfma2(as_half2(b), as_half2(s), __hmul2(as_half2(b), as_half2(rest))));
 }
 __device__ __forceinline__ void widen_v(uint32_t four, uint32_t s_lo, uint32_t s_hi, uint32_t& lo,
                                         uint32_t& hi) {
-  __half2 a, b;
-  widen4(four, a, b);
-  lo = as_u32(__hmul2(a, as_half2(s_lo)));
-  hi = as_u32(__hmul2(b, as_half2(s_hi)));
+  uint32_t a, b;
+  e4m3x4_to_f16x2x2(four, a, b);
+  lo = as_u32(__hmul2(as_half2(a), as_half2(s_lo)));
+  hi = as_u32(__hmul2(as_half2(b), as_half2(s_hi)));
 }
 
 // The 16-bit halves of a pair (tokens t, t + 1) that lie before `valid`.
@@ -909,26 +875,122 @@ __device__ __forceinline__ uint32_t keep_pair(uint32_t w, int t, int valid) {
   return t + 1 < valid ? w : (t < valid ? w & 0xffffu : 0u);
 }
 
+// The tiles K(0), V(0), K(1), ... of a CTA's items in order, copied by the
+// widening threads themselves: each brings the very bytes that it widens (and
+// a share of its warp's own copy of the scales), so a copy needs no barrier
+// but the thread's own wait.  (One thread issuing bulk copies for the CTA took
+// 3,900 cycles a tile.)  The copies run ahead of the widening, into items that
+// it has not taken yet: they only look at those.
+struct RawCopies {
+  const ChunkParams& p;
+  const Ctx<true>& x;
+  const uint32_t k_bytes;      // this thread's 16 bytes of a block's K
+  const int c, lane;
+  BlockIds ids{};
+  int kvh = 0, b0 = 0;         // of the item, the next tile's first block in it
+  int n = 0;                   // items looked at
+  bool is_v = false;
+  int slot = 0;
+
+  __device__ RawCopies(const ChunkParams& prm, const Ctx<true>& ctx, uint32_t kb, int thread)
+      : p(prm), x(ctx), k_bytes(kb), c(thread), lane(thread & 31) {}
+
+  static __device__ void copy16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+  }
+  __device__ const uint8_t* chunk(int id) const {
+    return p.kv8 + (static_cast<int64_t>(id) * p.hkv + kvh) * kFp8HeadBlockBytes;
+  }
+  // The next tile's copies, as one group; false if no further item is there.
+  __device__ bool issue() {
+    while (b0 >= ids.count) {
+      if (!__all_sync(0xffffffffu, mbar_test(&x.item_full[n % kItemRing], (n / kItemRing) & 1)))
+        return false;
+      const Item& it = *x.item(n);
+      if (it.t1 < 0) return false;  // looked at again on every call
+      ++n;
+      b0 = 0;
+      if (it.t1 > it.t0) {
+        kvh = it.kvh;
+        ids = BlockIds(p, it, x.err);
+      } else {
+        ids.count = 0;
+      }
+    }
+    if (!is_v && b0 && (b0 & 31) == 0) ids.advance(b0, x.err);
+    const int nb = min(kTileBlocks, ids.count - b0);
+    const uint32_t raw = smem_u32(x.smem + Cfg<true>::kOffRaw + slot * kRawBytes);
+    const uint32_t dst = raw + c * 16;
+    const uint32_t at = is_v ? kFp8VOff + c * 16 : k_bytes;
+    const uint32_t stride = p.hkv * kFp8HeadBlockBytes;
+    const uint8_t* from = p.kv8 + kvh * kFp8HeadBlockBytes + at;
+    if (nb == kTileBlocks) {
+#pragma unroll
+      for (int b = 0; b < kTileBlocks; ++b)
+        copy16(dst + b * 2048, from + static_cast<uint64_t>(static_cast<uint32_t>(ids.at(b0 + b))) * stride);
+    } else {
+      for (int b = 0; b < nb; ++b)
+        copy16(dst + b * 2048, from + static_cast<uint64_t>(static_cast<uint32_t>(ids.at(b0 + b))) * stride);
+    }
+    // lane: four tokens' scales of block lane / 4
+    const int id = __shfl_sync(0xffffffffu, ids.cur, (b0 + (lane >> 2)) & 31);
+    if (lane < nb * 4)
+      copy16(raw + kKeys * kHeadDim + (c >> 5) * kKeys * 4 + lane * 16,
+             chunk(id) + (is_v ? kFp8VScaleOff : kFp8KScaleOff) + (lane & 3) * 16);
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    if (is_v) b0 += kTileBlocks;
+    is_v = !is_v;
+    if (++slot == Cfg<true>::kRaw) slot = 0;
+    return true;
+  }
+};
+
 __device__ void widen_role(const ChunkParams& p, const Ctx<true>& x, int tpt) {
   using C = Cfg<true>;
   const int c = threadIdx.x - 384, lane = c & 31;
   const int pair = ((lane >> 4) & 1) + 2 * (c >> 5);
   const int tok = ((pair & 3) + (pair >> 2) * 8) ^ ((lane >> 2) & 1 ? 5 : 0);
   const int grp = (lane & 3) + ((lane >> 3) & 1) * 4;
-  const uint32_t k_src = tok * 128 + ((grp ^ (tok & 7)) << 4);
   const uint32_t k_dst = (grp >> 2) * kRegion + tok * 128;
   const uint32_t k_lo = ((((grp & 3) * 2) ^ (tok & 7)) << 4);
   const uint32_t k_hi = ((((grp & 3) * 2 + 1) ^ (tok & 7)) << 4);
-  // this warp's copy of the tile's V scales, f16
-  uint8_t* v_scale = x.smem + C::kOffScale + (c >> 5) * kKeys * 2;
+  // this warp's copy of the tile's scales: of keys both terms, twice each,
+  // of values f16 in order
+  uint8_t* scales = x.smem + C::kOffScale + (c >> 5) * kKeys * 8;
   uint32_t key = 0, n_load = 0;  // key tiles, Q tiles so far
-  RingPos<C::kRaw> g;            // the next copy group
+  int slot = 0;                  // of the next raw tile
+  int ahead = 0;                 // raw tiles copied or on their way, not widened
   RingPos<C::kKStages> k;
   RingPos<C::kVStages> v;
+  RawCopies copies(p, x, tok * 128 + ((grp ^ (tok & 7)) << 4), c);
+  auto fill = [&]() {
+    while (ahead < C::kRaw && copies.issue()) ++ahead;
+  };
+  // The next raw tile, once this thread's bytes and its warp's have landed.
+  // (Its item has been taken, so its copies can always be issued.)
+  auto landed = [&]() -> const uint8_t* {
+    if (ahead == 0) fill();
+    if (ahead >= 3)
+      asm volatile("cp.async.wait_group 2;" ::: "memory");
+    else if (ahead == 2)
+      asm volatile("cp.async.wait_group 1;" ::: "memory");
+    else
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncwarp();
+    return x.smem + C::kOffRaw + slot * kRawBytes;
+  };
+  // It has been read (its values are stored): the slot's next copies.
+  auto done = [&]() {
+    __syncwarp();
+    if (++slot == C::kRaw) slot = 0;
+    --ahead;
+    fill();
+  };
+  Item it;
   for (int n = 0;; ++n) {
-    Item it;
     if (!x.next(n, it) || it.t1 < 0) return;
     const int nt = it.t1 - it.t0;
+    fill();
     if (nt) {
       if (n_load && !x.wait_warp(x.q_free, n_load - 1)) return;
       ++n_load;
@@ -940,89 +1002,90 @@ __device__ void widen_role(const ChunkParams& p, const Ctx<true>& x, int tpt) {
     const int nblk = (it.key_end + kBlockTokens - 1) / kBlockTokens;
     for (int j = 0; j < nt; ++j) {
       const int b0 = (it.t0 + j) * kTileBlocks, nb = min(kTileBlocks, nblk - b0);
-      // ---- K tile, group by group of blocks as they land, and the V scales
+      // ---- K tile
       if (key >= C::kKStages && !x.wait_warp(&x.k_empty[k.st], k.ph ^ 1)) return;
+      const uint8_t* src = landed();
+      {
+        const float4 f = *reinterpret_cast<const float4*>(src + kKeys * kHeadDim +
+                                                          (c >> 5) * kKeys * 4 + lane * 16);
+        const float v[4] = {f.x, f.y, f.z, f.w};
+        uint32_t w[8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const __half2 s = __float2half2_rn(v[i]);
+          w[2 * i] = as_u32(s);
+          w[2 * i + 1] = as_u32(__float2half2_rn(v[i] - __low2float(s)));
+        }
+        uint4* at = reinterpret_cast<uint4*>(scales + lane * 32);
+        at[0] = make_uint4(w[0], w[1], w[2], w[3]);
+        at[1] = make_uint4(w[4], w[5], w[6], w[7]);
+        __syncwarp();
+      }
       uint8_t* dst = x.smem + C::kOffK + k.st * kOperand + k_dst;
-      RingPos<C::kRaw> q = g;
-      for (int b = 0; b < nb; b += kGroup, q.next()) {
-        if (!x.wait_warp(&x.raw_full[q.st], q.ph)) return;
-        const uint8_t* src = x.smem + C::kOffRaw + q.st * kGroup * kFp8HeadBlockBytes;
-        uint4 raw[kGroup];
-        float ks[kGroup];
-#pragma unroll
-        for (int u = 0; u < kGroup; ++u) {  // (a last odd block: stale bytes, masked keys)
-          raw[u] = *reinterpret_cast<const uint4*>(src + u * kFp8HeadBlockBytes + k_src);
-          ks[u] = *reinterpret_cast<const float*>(src + u * kFp8HeadBlockBytes + kFp8KScaleOff +
-                                                  tok * 4);
-        }
-        if (lane < kGroup * 4) {  // lane: four tokens of a block
-          const int u = lane >> 2, t = (lane & 3) * 4;
-          const float4 s = *reinterpret_cast<const float4*>(src + u * kFp8HeadBlockBytes +
-                                                            kFp8VScaleOff + t * 4);
-          *reinterpret_cast<uint2*>(v_scale + ((b + u) * kBlockTokens + t) * 2) =
-              make_uint2(pack_f16(s.x * 256.f, s.y * 256.f), pack_f16(s.z * 256.f, s.w * 256.f));
-        }
-#pragma unroll
-        for (int u = 0; u < kGroup; ++u) {
-          const float up = ks[u] * 256.f;
-          const __half2 sc = __float2half2_rn(up);
-          const __half2 rest = __float2half2_rn(up - __low2float(sc));
-          uint4 lo, hi;
-          widen_k(raw[u].x, sc, rest, lo.x, hi.x);
-          widen_k(raw[u].y, sc, rest, lo.y, hi.y);
-          widen_k(raw[u].z, sc, rest, lo.z, hi.z);
-          widen_k(raw[u].w, sc, rest, lo.w, hi.w);
-          *reinterpret_cast<uint4*>(dst + (b + u) * 2048 + k_lo) = lo;
-          *reinterpret_cast<uint4*>(dst + (b + u) * 2048 + k_hi) = hi;
-        }
+#pragma unroll 4
+      for (int b = 0; b < nb; ++b) {
+        const uint4 raw = *reinterpret_cast<const uint4*>(src + b * 2048 + c * 16);
+        const uint2 sc = *reinterpret_cast<const uint2*>(scales + (b * kBlockTokens + tok) * 8);
+        uint4 lo, hi;
+        widen_k(raw.x, sc.x, sc.y, lo.x, hi.x);
+        widen_k(raw.y, sc.x, sc.y, lo.y, hi.y);
+        widen_k(raw.z, sc.x, sc.y, lo.z, hi.z);
+        widen_k(raw.w, sc.x, sc.y, lo.w, hi.w);
+        *reinterpret_cast<uint4*>(dst + b * 2048 + k_lo) = lo;
+        *reinterpret_cast<uint4*>(dst + b * 2048 + k_hi) = hi;
       }
       fence_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(&x.k_full[k.st]);
       k.next();
+      done();
       // ---- V tile
       if (key >= C::kVStages && !x.wait_warp(&x.v_empty[v.st], v.ph ^ 1)) return;
-      dst = x.smem + C::kOffV + v.st * kOperand + c * 128;
-      for (int b = 0; b < nb; b += kGroup, g.next()) {
-        const uint8_t* src = x.smem + C::kOffRaw + g.st * kGroup * kFp8HeadBlockBytes + kFp8VOff;
-        uint4 raw[kGroup];
-#pragma unroll
-        for (int u = 0; u < kGroup; ++u)
-          raw[u] = *reinterpret_cast<const uint4*>(src + u * kFp8HeadBlockBytes + c * 16);
-#pragma unroll
-        for (int u = 0; u < kGroup; ++u) {
-          const uint4 sl = *reinterpret_cast<const uint4*>(v_scale + (b + u) * 32);
-          const uint4 sh = *reinterpret_cast<const uint4*>(v_scale + (b + u) * 32 + 16);
-          uint4 lo, hi;
-          widen_v(raw[u].x, sl.x, sh.x, lo.x, hi.x);
-          widen_v(raw[u].y, sl.y, sh.y, lo.y, hi.y);
-          widen_v(raw[u].z, sl.z, sh.z, lo.z, hi.z);
-          widen_v(raw[u].w, sl.w, sh.w, lo.w, hi.w);
-          const int valid = it.kv - (b0 + b + u) * kBlockTokens;
-          if (valid < kBlockTokens) {  // no position there: zeros for P's zeros
-            lo.x = keep_pair(lo.x, 0, valid);
-            lo.y = keep_pair(lo.y, 2, valid);
-            lo.z = keep_pair(lo.z, 4, valid);
-            lo.w = keep_pair(lo.w, 6, valid);
-            hi.x = keep_pair(hi.x, 8, valid);
-            hi.y = keep_pair(hi.y, 10, valid);
-            hi.z = keep_pair(hi.z, 12, valid);
-            hi.w = keep_pair(hi.w, 14, valid);
-          }
-          uint8_t* row = dst + ((b + u) >> 2) * kRegion;
-          *reinterpret_cast<uint4*>(row + (((((b + u) & 3) * 2) ^ (c & 7)) << 4)) = lo;
-          *reinterpret_cast<uint4*>(row + (((((b + u) & 3) * 2 + 1) ^ (c & 7)) << 4)) = hi;
-        }
-        // behind the stores: every load of the chunks has returned by then,
-        // which an arrive right behind the loads would not wait for
+      src = landed();
+      {
+        const float4 s = *reinterpret_cast<const float4*>(src + kKeys * kHeadDim +
+                                                          (c >> 5) * kKeys * 4 + lane * 16);
+        *reinterpret_cast<uint2*>(scales + lane * 8) =
+            make_uint2(pack_f16(s.x, s.y), pack_f16(s.z, s.w));
         __syncwarp();
-        if (lane == 0) mbar_arrive(&x.raw_empty[g.st]);
+      }
+      dst = x.smem + C::kOffV + v.st * kOperand + c * 128;
+      const int valid = it.kv - b0 * kBlockTokens;  // positions from the tile's first on
+#pragma unroll 4
+      for (int b = 0; b < nb; ++b) {
+        const uint4 raw = *reinterpret_cast<const uint4*>(src + b * 2048 + c * 16);
+        const uint4 sl = *reinterpret_cast<const uint4*>(scales + b * 32);
+        const uint4 sh = *reinterpret_cast<const uint4*>(scales + b * 32 + 16);
+        uint4 lo, hi;
+        widen_v(raw.x, sl.x, sh.x, lo.x, hi.x);
+        widen_v(raw.y, sl.y, sh.y, lo.y, hi.y);
+        widen_v(raw.z, sl.z, sh.z, lo.z, hi.z);
+        widen_v(raw.w, sl.w, sh.w, lo.w, hi.w);
+        uint8_t* row = dst + (b >> 2) * kRegion;
+        *reinterpret_cast<uint4*>(row + ((((b & 3) * 2) ^ (c & 7)) << 4)) = lo;
+        *reinterpret_cast<uint4*>(row + ((((b & 3) * 2 + 1) ^ (c & 7)) << 4)) = hi;
+      }
+      if (valid < nb * kBlockTokens) {
+        // no positions at the end of the last block: zeros for P's zeros
+        const int b = nb - 1, t = valid - b * kBlockTokens;
+        uint8_t* row = dst + (b >> 2) * kRegion;
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          uint4* at = reinterpret_cast<uint4*>(row + ((((b & 3) * 2 + half) ^ (c & 7)) << 4));
+          uint4 w = *at;
+          w.x = keep_pair(w.x, half * 8, t);
+          w.y = keep_pair(w.y, half * 8 + 2, t);
+          w.z = keep_pair(w.z, half * 8 + 4, t);
+          w.w = keep_pair(w.w, half * 8 + 6, t);
+          *at = w;
+        }
       }
       fence_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(&x.v_full[v.st]);
       v.next();
       ++key;
+      done();
     }
   }
 }
@@ -1154,7 +1217,7 @@ __global__ void __launch_bounds__(Cfg<kFp8>::kThreads, 1)
     }
     for (int i = 0; i < kItemRing; ++i) {
       mbar_init(&x.item_full[i], 1);
-      mbar_init(&x.item_empty[i], 15);  // every warp but warp 3
+      mbar_init(&x.item_empty[i], kFp8 ? 14 : 15);  // the warps that read items
     }
     mbar_init(x.q_full, kFp8 ? 4 : 3);
     mbar_init(x.q_free, 1);
@@ -1175,10 +1238,6 @@ __global__ void __launch_bounds__(Cfg<kFp8>::kThreads, 1)
     mbar_init(x.ml_bar, 8);
     mbar_init(x.ep_bar, 8);
     mbar_init(x.mma_done, 2);
-    for (int i = 0; i < C::kRaw; ++i) {
-      mbar_init(&x.raw_full[i], 1);
-      mbar_init(&x.raw_empty[i], 4);
-    }
     fence_mbar_init();
     s_row = p.batch;
     s_base = 0;
@@ -1234,9 +1293,7 @@ __global__ void __launch_bounds__(Cfg<kFp8>::kThreads, 1)
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kRegsLow));
     if (warp == 0) {
-      if constexpr (kFp8)
-        copy_role(p, x);
-      else
+      if constexpr (!kFp8)
         copy_role<C::kKStages>(p, x, &kmap, x.k_full, x.k_empty, smem + C::kOffK);
     } else if (warp == 1) {
       qk_role<kFp8>(p, x, tmem);

@@ -1,5 +1,6 @@
 // Attention of the newest tokens of each sequence over its paged cache, the
-// tokens of all sequences packed (sm_100a: tcgen05 + TMEM).
+// tokens of all sequences packed (sm_100a: tcgen05 + TMEM).  Sequences of few
+// new tokens are chunk_short.cu's; both leave what they cut to merge_kernel.
 //
 //   o_i = sum_j softmax_j(scale q_i . k_j) v_j      j < kv_len, and, causal,
 //                                                   j <= kv_len - T + i
@@ -43,8 +44,9 @@
 // 2^-21 of the largest and is off by at most 2^-32 of it below.
 #include <math.h>
 
-#include "pkv_device.cuh"
-#include "pkv_kernels.h"
+#include <algorithm>
+
+#include "chunk.cuh"
 #include "tc_device.cuh"
 
 namespace pkv {
@@ -55,7 +57,6 @@ constexpr int kKeys = 128;                         // keys of a tile
 constexpr int kTileBlocks = kKeys / kBlockTokens;  // 8
 constexpr int kRegion = kRows * 128;               // 128 rows x 64 elements
 constexpr int kOperand = 2 * kRegion;              // 32 KiB
-constexpr float kLazyLog2 = 8.f;  // the running maximum moves by more than this
 constexpr float kP8Shift = 7.f;   // FP8: P' up to 2^(8 + 7)
 // cost model, in keys of one tile: what an item costs besides its keys, and
 // the least a CTA is given
@@ -160,7 +161,7 @@ struct Work {
     const int s0 = min(max(__ldg(p.q_starts + b), 0), p.tokens);
     const int s1 = min(max(__ldg(p.q_starts + b + 1), s0), p.tokens);
     r.first = s0;
-    r.T = s1 - s0;
+    r.T = s1 - s0 > kShortRows / p.group ? s1 - s0 : 0;  // else the short kernel's
     r.kv = static_cast<int>(min(static_cast<int64_t>(max(__ldg(p.kv_lens + b), 0)),
                                 min(p.pitch, int64_t(1) << 26) * kBlockTokens));
     r.n = (r.T + block - 1) / block;
@@ -253,16 +254,6 @@ __device__ __forceinline__ void mma_commit(uint64_t* bar) {
       "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
       "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(
           smem_u32(bar))
-      : "memory");
-}
-
-__device__ __forceinline__ void tma_load_5d(void* dst, const CUtensorMap* map, uint64_t* bar,
-                                            int c0, int c1, int c2, int c3, int c4,
-                                            uint64_t policy) {
-  asm volatile(
-      "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
-      ".L2::cache_hint [%0], [%1, {%3, %4, %5, %6, %7}], [%2], %8;" ::"r"(smem_u32(dst)),
-      "l"(map), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(c4), "l"(policy)
       : "memory");
 }
 
@@ -1330,53 +1321,84 @@ __global__ void __launch_bounds__(Cfg<kFp8>::kThreads, 1)
   }
 }
 
-// One warp per packed row of a cut item: o = sum 2^(lse_c - L) o_c over its
-// parts in key order, lane l holding dims 4l .. 4l+3.
-__global__ void __launch_bounds__(256) merge_kernel(const ChunkParams p) {
+// One warp per packed row of what was cut: o = sum 2^(lse_c - L) o_c over its
+// parts in key order, lane l holding dims 4l .. 4l+3.  at(c): part c's row.
+template <typename At>
+__device__ __forceinline__ void merge_row(const float* lse, const float* part, int parts, At at,
+                                          __nv_bfloat16* out) {
+  const int lane = threadIdx.x & 31;
+  float top = -INFINITY;
+  for (int c = lane; c < parts; c += 32) top = fmaxf(top, __ldcg(lse + at(c)));
+#pragma unroll
+  for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  const float base = top == -INFINITY ? 0.f : top;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  float sum = 0.f;
+#pragma unroll 4
+  for (int c = 0; c < parts; ++c) {
+    const float f = ex2(__ldcg(lse + at(c)) - base);
+    const float4 v = __ldcg(reinterpret_cast<const float4*>(part + at(c) * kHeadDim) + lane);
+    sum += f;
+    acc.x += f * v.x;
+    acc.y += f * v.y;
+    acc.z += f * v.z;
+    acc.w += f * v.w;
+  }
+  const float inv = 1.f / sum;  // 0/0 -> NaN for a token that sees no key
+  uint2 pk;
+  pk.x = pack_bf16(acc.x * inv, acc.y * inv);
+  pk.y = pack_bf16(acc.z * inv, acc.w * inv);
+  *reinterpret_cast<uint2*>(out + lane * 4) = pk;
+}
+
+// Blocks [0, n_long) x grid.y: the items that chunk_kernel's CTAs cut, by the
+// CTA that holds their first keys; the others, the short kernel's units.
+__global__ void __launch_bounds__(256) merge_kernel(const ChunkParams p, const ShortParams q,
+                                                    int n_long, int y_long) {
   pdl_trigger();
   pdl_wait();
-  const int4 d = __ldcg(p.desc + blockIdx.x);
-  if (d.x < 2) return;
-  const int lane = threadIdx.x & 31;
-  const int tpt = kRows / p.group, rows = d.z * p.group;
-  for (int i = blockIdx.y * 8 + (threadIdx.x >> 5); i < rows; i += gridDim.y * 8) {
-    const int tok = i / p.group, head = d.w * p.group + i - tok * p.group;
-    const int prow = (d.z > tpt && tok >= tpt) ? kRows + i - tpt * p.group : i;
-    auto slot = [&](int c) -> int64_t {
-      return ((static_cast<int64_t>(blockIdx.x) + c) * 2 + (c == 0 ? 1 : 0)) * p.part_rows + prow;
-    };
-    float top = -INFINITY;
-    for (int c = lane; c < d.x; c += 32) top = fmaxf(top, __ldcg(p.part_lse + slot(c)));
-#pragma unroll
-    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    const float base = top == -INFINITY ? 0.f : top;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    float sum = 0.f;
-#pragma unroll 4
-    for (int c = 0; c < d.x; ++c) {
-      const float f = ex2(__ldcg(p.part_lse + slot(c)) - base);
-      const float4 v = __ldcg(reinterpret_cast<const float4*>(p.part_o + slot(c) * kHeadDim) + lane);
-      sum += f;
-      acc.x += f * v.x;
-      acc.y += f * v.y;
-      acc.z += f * v.z;
-      acc.w += f * v.w;
+  const int warp = threadIdx.x >> 5;
+  int unit = blockIdx.x - n_long * y_long;
+  if (unit < 0) {
+    const int cta = blockIdx.x / y_long, y = blockIdx.x - cta * y_long;
+    const int4 d = __ldcg(p.desc + cta);
+    if (d.x < 2) return;
+    const int tpt = kRows / p.group, rows = d.z * p.group;
+    for (int i = y * 8 + warp; i < rows; i += y_long * 8) {
+      const int tok = i / p.group, head = d.w * p.group + i - tok * p.group;
+      const int prow = (d.z > tpt && tok >= tpt) ? kRows + i - tpt * p.group : i;
+      merge_row(p.part_lse, p.part_o, d.x,
+                [&](int c) -> int64_t {
+                  return ((static_cast<int64_t>(cta) + c) * 2 + (c == 0 ? 1 : 0)) * p.part_rows + prow;
+                },
+                p.out + static_cast<int64_t>(d.y + tok) * p.o_st + head * p.o_sh);
     }
-    const float inv = 1.f / sum;  // 0/0 -> NaN for a token that sees no key
-    uint2 pk;
-    pk.x = pack_bf16(acc.x * inv, acc.y * inv);
-    pk.y = pack_bf16(acc.z * inv, acc.w * inv);
-    *reinterpret_cast<uint2*>(p.out + static_cast<int64_t>(d.y + tok) * p.o_st + head * p.o_sh +
-                              lane * 4) = pk;
+    return;
+  }
+  const int b = unit / q.hkv, h = unit - b * q.hkv;
+  const ShortRow r = short_row(q, b);
+  if (r.T == 0 || r.nparts < 2) return;
+  for (int i = warp; i < r.T * q.group; i += 8) {
+    const int tok = i / q.group, head = h * q.group + i - tok * q.group;
+    merge_row(q.part_lse, q.part_o, r.nparts,
+              [&](int c) -> int64_t {
+                return (static_cast<int64_t>(unit) * q.max_parts + c) * q.part_rows + i;
+              },
+              q.out + static_cast<int64_t>(r.first + tok) * q.o_st + head * q.o_sh);
   }
 }
 
 // ---------------------------------------------------------------- host
 struct ChunkPlan {
-  int grid, part_rows;
+  int grid, part_rows;                           // chunk_kernel; grid 0: not needed
+  int parts, min_blocks, short_rows;             // short kernel
 };
 
-// One CTA per SM, fewer where the launch's sizes cannot give each kMinStep.
+// chunk_kernel: one CTA per SM, fewer where the launch's sizes cannot give
+// each kMinStep.  Short kernel: enough partitions per (sequence, KV head) for
+// kShortCtas CTAs of at least kShortMinBlocks blocks (two per warp).
+constexpr int kShortCtas = 148 * 2 * 4;
+constexpr int kShortMinBlocks = 8;
 ChunkPlan plan_chunk(int32_t batch, int32_t tokens, int32_t hq, int32_t hkv, int32_t max_kv_len,
                      bool fp8) {
   int dev = 0, sms = 148;
@@ -1384,20 +1406,37 @@ ChunkPlan plan_chunk(int32_t batch, int32_t tokens, int32_t hq, int32_t hkv, int
     cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
   cudaGetLastError();
   const int group = hq / hkv, tpt = kRows / group, tiles = fp8 ? 1 : 2;
-  const int64_t items = (static_cast<int64_t>(tokens) / (tpt * tiles) + batch) * hkv;
-  const int64_t item = kItemCost + static_cast<int64_t>(tiles) * max_kv_len;
-  const int64_t want = items > (int64_t(1) << 40) / item ? sms : (items * item + kMinStep - 1) / kMinStep;
-  ChunkPlan pl;
-  pl.grid = static_cast<int>(want < 1 ? 1 : (want < sms ? want : sms));
-  // rows of a partial: those of one item (tile B starts at row 128)
-  const int64_t most = static_cast<int64_t>(tokens) * group;
-  pl.part_rows = tokens > tpt ? tiles * kRows : static_cast<int>((most + 7) / 8 * 8);
+  ChunkPlan pl{};
+  const int64_t most = static_cast<int64_t>(tokens) * group;  // rows of one sequence
+  if (tokens > kShortRows / group) {
+    const int64_t items = (static_cast<int64_t>(tokens) / (tpt * tiles) +
+                           std::min(batch, tokens / (kShortRows / group + 1))) * hkv;
+    const int64_t item = kItemCost + static_cast<int64_t>(tiles) * max_kv_len;
+    const int64_t want =
+        items > (int64_t(1) << 40) / item ? sms : (items * item + kMinStep - 1) / kMinStep;
+    pl.grid = static_cast<int>(want < 1 ? 1 : (want < sms ? want : sms));
+    // rows of a partial: those of one item (tile B starts at row 128)
+    pl.part_rows = tokens > tpt ? tiles * kRows : static_cast<int>((most + 7) / 8 * 8);
+  }
+  const int64_t units = static_cast<int64_t>(batch) * hkv;
+  const int nblk = max_kv_len / kBlockTokens + 1;
+  int64_t parts = (kShortCtas + units - 1) / units;
+  parts = std::min<int64_t>(parts, std::max(1, nblk / kShortMinBlocks));
+  pl.parts = static_cast<int>(std::min<int64_t>(parts, 64));
+  pl.min_blocks = kShortMinBlocks;
+  pl.short_rows = static_cast<int>(std::min<int64_t>(kShortRows, (most + 7) / 8 * 8));
   return pl;
 }
 
-size_t plan_bytes(const ChunkPlan& pl) {
+// Workspace: descriptors, sums and partials of chunk_kernel, then sums and
+// partials of the short kernel.
+size_t long_bytes(const ChunkPlan& pl) {
   if (pl.grid < 2) return 0;
   return static_cast<size_t>(pl.grid) * (16 + 2 * static_cast<size_t>(pl.part_rows) * (kHeadDim + 1) * 4);
+}
+size_t short_bytes(const ChunkPlan& pl, int64_t units) {
+  if (pl.parts < 2) return 0;
+  return static_cast<size_t>(units) * pl.parts * pl.short_rows * (kHeadDim + 1) * 4;
 }
 
 template <bool kFp8>
@@ -1424,9 +1463,10 @@ bool registers_as_planned() {
 
 size_t chunk_workspace_bytes(int32_t batch, int32_t tokens, int32_t hq, int32_t hkv,
                              int32_t max_kv_len) {
-  const size_t a = plan_bytes(plan_chunk(batch, tokens, hq, hkv, max_kv_len, false));
-  const size_t b = plan_bytes(plan_chunk(batch, tokens, hq, hkv, max_kv_len, true));
-  return a > b ? a : b;
+  const ChunkPlan a = plan_chunk(batch, tokens, hq, hkv, max_kv_len, false);
+  const ChunkPlan b = plan_chunk(batch, tokens, hq, hkv, max_kv_len, true);
+  return std::max(long_bytes(a), long_bytes(b)) +
+         short_bytes(a, static_cast<int64_t>(batch) * hkv);  // the same for both
 }
 
 cudaError_t launch_chunk(const ChunkLaunch& a, cudaStream_t stream) {
@@ -1462,11 +1502,48 @@ cudaError_t launch_chunk(const ChunkLaunch& a, cudaStream_t stream) {
     p.part_lse = reinterpret_cast<float*>(p.desc + pl.grid);
     p.part_o = p.part_lse + static_cast<int64_t>(pl.grid) * 2 * pl.part_rows;
   }
-  const cudaError_t e = fp8 ? launch_chunk_t<true>(p, a.kmap, a.vmap, pl.grid, stream)
-                            : launch_chunk_t<false>(p, a.kmap, a.vmap, pl.grid, stream);
-  if (e != cudaSuccess || pl.grid < 2) return e;
-  const int item_rows = pl.part_rows;
-  return launch_k(merge_kernel, dim3(pl.grid, (item_rows + 15) / 16), dim3(256), 0, stream, p);
+  const int64_t units = static_cast<int64_t>(a.batch) * a.num_kv_heads;
+  ShortParams q{};
+  q.q = p.q;
+  q.q_st = p.q_st;
+  q.q_sh = p.q_sh;
+  q.out = p.out;
+  q.o_st = p.o_st;
+  q.o_sh = p.o_sh;
+  q.kv8 = p.kv8;
+  q.tables = p.tables;
+  q.pitch = p.pitch;
+  q.rows = p.rows;
+  q.q_starts = p.q_starts;
+  q.kv_lens = p.kv_lens;
+  q.tokens = p.tokens;
+  q.hkv = p.hkv;
+  q.group = p.group;
+  q.num_blocks = p.num_blocks;
+  q.causal = p.causal;
+  q.max_parts = pl.parts;
+  q.min_blocks = pl.min_blocks;
+  q.part_rows = pl.short_rows;
+  q.scale_log2 = a.sm_scale * 1.4426950408889634f;
+  q.err = a.err;
+  if (pl.parts > 1) {
+    q.part_lse = reinterpret_cast<float*>(static_cast<uint8_t*>(a.workspace) + long_bytes(pl));
+    q.part_o = q.part_lse + units * pl.parts * pl.short_rows;
+  }
+  if (kShortRows / p.group > 0) {
+    const cudaError_t e = launch_chunk_short(q, a.kmap, a.vmap, a.batch, stream);
+    if (e != cudaSuccess) return e;
+  }
+  if (pl.grid > 0) {
+    const cudaError_t e = fp8 ? launch_chunk_t<true>(p, a.kmap, a.vmap, pl.grid, stream)
+                              : launch_chunk_t<false>(p, a.kmap, a.vmap, pl.grid, stream);
+    if (e != cudaSuccess) return e;
+  }
+  const int n_long = pl.grid > 1 ? pl.grid : 0, y_long = (pl.part_rows + 15) / 16;
+  const int64_t blocks = static_cast<int64_t>(n_long) * y_long + (pl.parts > 1 ? units : 0);
+  if (blocks == 0) return cudaSuccess;
+  return launch_k(merge_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream, p, q,
+                  n_long, y_long);
 }
 
 }  // namespace pkv

@@ -356,7 +356,9 @@ class Split:
     """struct Work and item_role of csrc/chunk.cu."""
 
     def __init__(self, new, kv, group, hkv, fp8, causal):
-        self.new, self.kv, self.hkv, self.causal = new, kv, hkv, causal
+        # sequences of at most 32 rows per KV head are the short kernel's
+        self.new = [t if t > 32 // group else 0 for t in new]
+        self.kv, self.hkv, self.causal = kv, hkv, causal
         self.tpt = 128 // group
         self.wfull = 1 if fp8 else 2
         self.block = self.tpt * self.wfull
@@ -440,6 +442,8 @@ def test_every_key_tile_is_worked_once(seed):
             at += sp.cost(b, i)
         assert sp.head(b) == at
     ctas = rng.choice([2, 11, 148])
+    if not any(sp.new):
+        return
     step, ranges = sp.ranges(ctas)
     work, slots, descs = {}, {}, {}
     for c, (lo, hi) in enumerate(ranges):

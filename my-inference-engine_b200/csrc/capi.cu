@@ -1008,7 +1008,7 @@ static int chunk_common(pkv::ChunkLaunch& a, const void* q, int64_t q_st, int64_
   if (!(sm_scale > 0.f) || !(sm_scale < INFINITY))
     return fail(PKV_ERR_INVALID, "sm_scale must be positive and finite");
   if (static_cast<int64_t>(num_tokens) * num_q_heads > (int64_t(1) << 30) ||
-      static_cast<int64_t>(batch) * num_kv_heads > (int64_t(1) << 24) || batch > 65535 ||
+      static_cast<int64_t>(batch) * num_kv_heads > (int64_t(1) << 24) || batch > 16383 ||
       num_kv_heads > 65535)
     return fail(PKV_ERR_UNSUPPORTED, "too many rows or tokens for one launch");
   const size_t need = pkv::chunk_workspace_bytes(batch, num_tokens, num_q_heads, num_kv_heads, max_kv_len);

@@ -1,6 +1,6 @@
 // Attention of the newest tokens of each sequence over its paged cache, the
 // tokens of all sequences packed (sm_100a: tcgen05 + TMEM).  Sequences of few
-// new tokens are chunk_short.cu's; both leave what they cut to merge_kernel.
+// new tokens, and small calls, are chunk_short.cu's.
 //
 //   o_i = sum_j softmax_j(scale q_i . k_j) v_j      j < kv_len, and, causal,
 //                                                   j <= kv_len - T + i
@@ -22,13 +22,13 @@
 // replays for other lengths.
 //
 // CTA (one per SM), warps:
-//   0, 12  copies of K and of V, a 5-D TMA box of 4 KiB per block, through the
+//   0, 15  copies of K and of V, a 5-D TMA box of 4 KiB per block, through the
 //          block table (FP8: warp 0, one bulk copy of a block's chunk)
 //   1      owns TMEM, issues the Q.K's
 //   2      issues the P.V's
 //   3      walks the range and hands the items out
 //   4-7    softmax of slot A, 8-11 of slot B: a thread owns a tile row
-//   13-15  write the items' Q tiles to shared memory
+//   12-14  write the items' Q tiles to shared memory
 //   12-15  (FP8) do so as f16 of q / 16, and widen K and V to f16 tiles
 // Two slots, each with a P and an O tile in tensor memory, share one S tile:
 // softmax warps take S into registers and free it at once, so the next Q.K
@@ -45,6 +45,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <atomic>
 
 #include "chunk.cuh"
 #include "tc_device.cuh"
@@ -63,8 +64,7 @@ constexpr float kP8Shift = 7.f;   // FP8: P' up to 2^(8 + 7)
 constexpr int kItemCost = 384;
 constexpr int kMinStep = kItemCost + 4 * kKeys;
 constexpr int kItemRing = 3;
-// FP8: e4m3 bytes of a K or V tile, and four copies of its fp32 scales
-constexpr int kRawBytes = kKeys * kHeadDim + 4 * kKeys * 4;
+constexpr int kGroup = 4;  // FP8: blocks to a copy barrier
 // tensor memory columns: S, then each slot's P, then each slot's O
 constexpr uint32_t kColP = 128, kColO = 256;
 
@@ -75,16 +75,16 @@ struct Cfg {
   // 32 KiB tiles; a ring each, so that no barrier is polled by two copiers of
   // whom each sees every second phase only
   static constexpr int kKStages = kFp8 ? 2 : 3, kVStages = 2;
-  static constexpr int kRaw = kFp8 ? 3 : 0;  // FP8 tiles (K or V) read or in flight
+  static constexpr int kRaw = kFp8 ? 3 : 0;  // groups of kGroup chunks in flight
   static constexpr int kOffQ = 0;
   static constexpr int kOffK = kOffQ + kTiles * kOperand;
   static constexpr int kOffV = kOffK + kKStages * kOperand;
   static constexpr int kOffRaw = kOffV + kVStages * kOperand;
-  static constexpr int kOffScale = kOffRaw + kRaw * kRawBytes;  // [4 warps][128] f16 scales
+  static constexpr int kOffScale = kOffRaw + kRaw * kGroup * kFp8HeadBlockBytes;  // [4 warps][128] f16 scales
   static constexpr int kOffMl = kOffScale + (kFp8 ? 4 * kKeys * 8 : 0);  // [2][128] float2
   static constexpr int kOffItem = kOffMl + 2 * kRows * 8;
   static constexpr int kOffBar = kOffItem + kItemRing * 64;
-  static constexpr int kBars = 2 * kItemRing + 2 + 2 * (kKStages + kVStages) + 7 + 3;
+  static constexpr int kBars = 2 * kItemRing + 2 + 2 * (kKStages + kVStages) + 7 + 3 + 2 * kRaw;
   static constexpr int kOffScan = kOffBar + kBars * 8 + 16;  // 16 warp sums, base, row
   static constexpr int kSmem = kOffScan + 18 * 8;
   // setmaxnreg: the warpgroups' shares of the launch's 128 per thread
@@ -94,7 +94,6 @@ struct Cfg {
   static constexpr int kRegsAux = kFp8 ? 72 : 40;    // warps 12-15
   static_assert(kRegsLow + 2 * kRegsSoftmax + kRegsAux <= 4 * kRegsLaunch,
                 "register split exceeds the launch allocation");
-  static_assert(kRaw <= 3, "landed() waits for at most two groups behind the oldest");
   static_assert(kSmem <= 227 * 1024, "shared memory exceeds the per-CTA limit");
 };
 
@@ -111,7 +110,8 @@ struct ChunkParams {
   const int32_t* kv_lens;
   int32_t batch, tokens, hkv, group, num_blocks, causal;
   float scale_log2;
-  int32_t part_rows;  // rows of a partial slot
+  int32_t short_rows;  // sequences of more rows per KV head are this kernel's
+  int32_t part_rows;   // rows of a partial slot
   int4* desc;         // [grid]: parts, first token, tokens, KV head
   float* part_lse;    // [grid][2][part_rows]
   float* part_o;      // [grid][2][part_rows][128]
@@ -161,7 +161,7 @@ struct Work {
     const int s0 = min(max(__ldg(p.q_starts + b), 0), p.tokens);
     const int s1 = min(max(__ldg(p.q_starts + b + 1), s0), p.tokens);
     r.first = s0;
-    r.T = s1 - s0 > kShortRows / p.group ? s1 - s0 : 0;  // else the short kernel's
+    r.T = (s1 - s0) * p.group > p.short_rows ? s1 - s0 : 0;  // else the short kernel's
     r.kv = static_cast<int>(min(static_cast<int64_t>(max(__ldg(p.kv_lens + b), 0)),
                                 min(p.pitch, int64_t(1) << 26) * kBlockTokens));
     r.n = (r.T + block - 1) / block;
@@ -297,7 +297,7 @@ struct Ctx {
   using C = Cfg<kFp8>;
   uint8_t* smem;
   uint64_t *item_full, *item_empty, *q_full, *q_free, *k_full, *k_empty, *v_full, *v_empty, *s_full, *s_free, *p_full,
-      *pv_done, *ml_bar, *ep_bar, *mma_done;
+      *pv_done, *ml_bar, *ep_bar, *mma_done, *raw_full, *raw_empty;
   DevErr err;
 
   __device__ Ctx(uint8_t* s, int32_t* e) : smem(s), err{e} {
@@ -322,6 +322,8 @@ struct Ctx {
     ml_bar = take(1);
     ep_bar = take(1);
     mma_done = take(1);
+    raw_full = take(C::kRaw);
+    raw_empty = take(C::kRaw);
   }
   __device__ uint32_t* tmem_slot() const {
     return reinterpret_cast<uint32_t*>(smem + C::kOffBar + C::kBars * 8);
@@ -768,7 +770,6 @@ struct BlockIds {
     }
     return id;
   }
-  __device__ BlockIds() : trow(nullptr), first(0), count(0), num_blocks(0), cur(0), nxt(0) {}
   __device__ BlockIds(const ChunkParams& p, const Item& it, const DevErr& err)
       : trow(p.tables + static_cast<int64_t>(it.table_row) * p.pitch),
         first(it.t0 * kTileBlocks),
@@ -784,6 +785,28 @@ struct BlockIds {
     nxt = load(i / 32 + 1, err);
   }
 };
+
+// Copies issued by a converged warp (elect.sync in the statement): no branch
+// around each, which with the softmax on the same scheduler is what a copy
+// costs.
+__device__ __forceinline__ void box_load(uint32_t dst, const CUtensorMap* map, uint32_t bar,
+                                         int slot8, int head, uint64_t policy) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+      "@e cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      ".L2::cache_hint [%0], [%1, {%6, %6, %6, %3, %4}], [%2], %5;\n\t}" ::"r"(dst),
+      "l"(map), "r"(bar), "r"(slot8), "r"(head), "l"(policy), "r"(0)
+      : "memory");
+}
+__device__ __forceinline__ void chunk_load(uint32_t dst, const void* src, uint32_t bar,
+                                           uint64_t policy) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+      "@e cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint"
+      " [%0], [%1], %2, [%3], %4;\n\t}" ::"r"(dst),
+      "l"(src), "r"(kFp8HeadBlockBytes), "r"(bar), "l"(policy)
+      : "memory");
+}
 
 // bf16 pool: one warp copies the K tiles, another the V tiles: a
 // thread takes over 100 cycles per box, 16 of them a tile of both.
@@ -810,14 +833,17 @@ __device__ void copy_role(const ChunkParams& p, const Ctx<false>& x, const CUten
         ok = false;
         break;
       }
-      uint8_t* dst = ring + r.st * kOperand;
-      uint64_t* bar = &full[r.st];
-      if (lane == 0) mbar_arrive_expect_tx(bar, nb * 4096);
-      for (int b = 0; b < nb; ++b) {
-        const int id = ids.at(b0 + b);
-        if (lane == 0) tma_load_5d(dst + b * 4096, map, bar, 0, 0, 0, id * 2, it.kvh, keep);
-      }
+      const uint32_t dst = smem_u32(ring) + r.st * kOperand, bar = smem_u32(&full[r.st]);
+      if (lane == 0) mbar_arrive_expect_tx(&full[r.st], nb * 4096);
       __syncwarp();
+      if (nb == kTileBlocks) {
+#pragma unroll
+        for (int b = 0; b < kTileBlocks; ++b)
+          box_load(dst + b * 4096, map, bar, ids.at(b0 + b) * 2, it.kvh, keep);
+      } else {
+        for (int b = 0; b < nb; ++b)
+          box_load(dst + b * 4096, map, bar, ids.at(b0 + b) * 2, it.kvh, keep);
+      }
       r.next();
       ++n_tile;
     }
@@ -826,6 +852,52 @@ __device__ void copy_role(const ChunkParams& p, const Ctx<false>& x, const CUten
     for (uint32_t t = n_tile > kStages ? n_tile - kStages : 0; t < n_tile; ++t)
       x.wait_warp(&full[t % kStages], t / kStages);
   }
+}
+
+// FP8 pool: one bulk copy per block, kGroup blocks to a barrier.
+__device__ void copy_role(const ChunkParams& p, const Ctx<true>& x) {
+  using C = Cfg<true>;
+  const int lane = threadIdx.x & 31;
+  const uint64_t keep = policy_evict_last();
+  const uint64_t stride = static_cast<uint64_t>(p.hkv) * kFp8HeadBlockBytes;
+  RingPos<C::kRaw> r;
+  uint32_t n_group = 0;
+  bool ok = true;
+  for (int n = 0; ok; ++n) {
+    Item it;
+    ok = x.next(n, it);
+    if (!ok || it.t1 < 0) break;
+    if (it.t1 == it.t0) continue;
+    BlockIds ids(p, it, x.err);
+    const uint8_t* from = p.kv8 + static_cast<int64_t>(it.kvh) * kFp8HeadBlockBytes;
+    for (int b0 = 0; b0 < ids.count; b0 += kGroup) {
+      if (b0 && (b0 & 31) == 0) ids.advance(b0, x.err);
+      if (n_group >= C::kRaw && !x.wait_warp(&x.raw_empty[r.st], r.ph ^ 1)) {
+        ok = false;
+        break;
+      }
+      const int nb = min(kGroup, ids.count - b0);
+      const uint32_t dst = smem_u32(x.smem + C::kOffRaw) + r.st * kGroup * kFp8HeadBlockBytes;
+      const uint32_t bar = smem_u32(&x.raw_full[r.st]);
+      if (lane == 0) mbar_arrive_expect_tx(&x.raw_full[r.st], nb * kFp8HeadBlockBytes);
+      __syncwarp();
+      if (nb == kGroup) {
+#pragma unroll
+        for (int b = 0; b < kGroup; ++b)
+          chunk_load(dst + b * kFp8HeadBlockBytes,
+                     from + static_cast<uint32_t>(ids.at(b0 + b)) * stride, bar, keep);
+      } else {
+        for (int b = 0; b < nb; ++b)
+          chunk_load(dst + b * kFp8HeadBlockBytes,
+                     from + static_cast<uint32_t>(ids.at(b0 + b)) * stride, bar, keep);
+      }
+      ++n_group;
+      r.next();
+    }
+  }
+  if (!ok)
+    for (uint32_t g = n_group > C::kRaw ? n_group - C::kRaw : 0; g < n_group; ++g)
+      x.wait_warp(&x.raw_full[g % C::kRaw], g / C::kRaw);
 }
 
 // ---------------------------------------------------------------- FP8 widening
@@ -866,82 +938,13 @@ __device__ __forceinline__ uint32_t keep_pair(uint32_t w, int t, int valid) {
   return t + 1 < valid ? w : (t < valid ? w & 0xffffu : 0u);
 }
 
-// The tiles K(0), V(0), K(1), ... of a CTA's items in order, copied by the
-// widening threads themselves: each brings the very bytes that it widens (and
-// a share of its warp's own copy of the scales), so a copy needs no barrier
-// but the thread's own wait.  (One thread issuing bulk copies for the CTA took
-// 3,900 cycles a tile.)  The copies run ahead of the widening, into items that
-// it has not taken yet: they only look at those.
-struct RawCopies {
-  const ChunkParams& p;
-  const Ctx<true>& x;
-  const uint32_t k_bytes;      // this thread's 16 bytes of a block's K
-  const int c, lane;
-  BlockIds ids{};
-  int kvh = 0, b0 = 0;         // of the item, the next tile's first block in it
-  int n = 0;                   // items looked at
-  bool is_v = false;
-  int slot = 0;
-
-  __device__ RawCopies(const ChunkParams& prm, const Ctx<true>& ctx, uint32_t kb, int thread)
-      : p(prm), x(ctx), k_bytes(kb), c(thread), lane(thread & 31) {}
-
-  static __device__ void copy16(uint32_t dst, const void* src) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-  }
-  __device__ const uint8_t* chunk(int id) const {
-    return p.kv8 + (static_cast<int64_t>(id) * p.hkv + kvh) * kFp8HeadBlockBytes;
-  }
-  // The next tile's copies, as one group; false if no further item is there.
-  __device__ bool issue() {
-    while (b0 >= ids.count) {
-      if (!__all_sync(0xffffffffu, mbar_test(&x.item_full[n % kItemRing], (n / kItemRing) & 1)))
-        return false;
-      const Item& it = *x.item(n);
-      if (it.t1 < 0) return false;  // looked at again on every call
-      ++n;
-      b0 = 0;
-      if (it.t1 > it.t0) {
-        kvh = it.kvh;
-        ids = BlockIds(p, it, x.err);
-      } else {
-        ids.count = 0;
-      }
-    }
-    if (!is_v && b0 && (b0 & 31) == 0) ids.advance(b0, x.err);
-    const int nb = min(kTileBlocks, ids.count - b0);
-    const uint32_t raw = smem_u32(x.smem + Cfg<true>::kOffRaw + slot * kRawBytes);
-    const uint32_t dst = raw + c * 16;
-    const uint32_t at = is_v ? kFp8VOff + c * 16 : k_bytes;
-    const uint32_t stride = p.hkv * kFp8HeadBlockBytes;
-    const uint8_t* from = p.kv8 + kvh * kFp8HeadBlockBytes + at;
-    if (nb == kTileBlocks) {
-#pragma unroll
-      for (int b = 0; b < kTileBlocks; ++b)
-        copy16(dst + b * 2048, from + static_cast<uint64_t>(static_cast<uint32_t>(ids.at(b0 + b))) * stride);
-    } else {
-      for (int b = 0; b < nb; ++b)
-        copy16(dst + b * 2048, from + static_cast<uint64_t>(static_cast<uint32_t>(ids.at(b0 + b))) * stride);
-    }
-    // lane: four tokens' scales of block lane / 4
-    const int id = __shfl_sync(0xffffffffu, ids.cur, (b0 + (lane >> 2)) & 31);
-    if (lane < nb * 4)
-      copy16(raw + kKeys * kHeadDim + (c >> 5) * kKeys * 4 + lane * 16,
-             chunk(id) + (is_v ? kFp8VScaleOff : kFp8KScaleOff) + (lane & 3) * 16);
-    asm volatile("cp.async.commit_group;" ::: "memory");
-    if (is_v) b0 += kTileBlocks;
-    is_v = !is_v;
-    if (++slot == Cfg<true>::kRaw) slot = 0;
-    return true;
-  }
-};
-
 __device__ void widen_role(const ChunkParams& p, const Ctx<true>& x, int tpt) {
   using C = Cfg<true>;
   const int c = threadIdx.x - 384, lane = c & 31;
   const int pair = ((lane >> 4) & 1) + 2 * (c >> 5);
   const int tok = ((pair & 3) + (pair >> 2) * 8) ^ ((lane >> 2) & 1 ? 5 : 0);
   const int grp = (lane & 3) + ((lane >> 3) & 1) * 4;
+  const uint32_t k_src = tok * 128 + ((grp ^ (tok & 7)) << 4);
   const uint32_t k_dst = (grp >> 2) * kRegion + tok * 128;
   const uint32_t k_lo = ((((grp & 3) * 2) ^ (tok & 7)) << 4);
   const uint32_t k_hi = ((((grp & 3) * 2 + 1) ^ (tok & 7)) << 4);
@@ -949,39 +952,13 @@ __device__ void widen_role(const ChunkParams& p, const Ctx<true>& x, int tpt) {
   // of values f16 in order
   uint8_t* scales = x.smem + C::kOffScale + (c >> 5) * kKeys * 8;
   uint32_t key = 0, n_load = 0;  // key tiles, Q tiles so far
-  int slot = 0;                  // of the next raw tile
-  int ahead = 0;                 // raw tiles copied or on their way, not widened
+  RingPos<C::kRaw> g;            // the next copy group
   RingPos<C::kKStages> k;
   RingPos<C::kVStages> v;
-  RawCopies copies(p, x, tok * 128 + ((grp ^ (tok & 7)) << 4), c);
-  auto fill = [&]() {
-    while (ahead < C::kRaw && copies.issue()) ++ahead;
-  };
-  // The next raw tile, once this thread's bytes and its warp's have landed.
-  // (Its item has been taken, so its copies can always be issued.)
-  auto landed = [&]() -> const uint8_t* {
-    if (ahead == 0) fill();
-    if (ahead >= 3)
-      asm volatile("cp.async.wait_group 2;" ::: "memory");
-    else if (ahead == 2)
-      asm volatile("cp.async.wait_group 1;" ::: "memory");
-    else
-      asm volatile("cp.async.wait_group 0;" ::: "memory");
-    __syncwarp();
-    return x.smem + C::kOffRaw + slot * kRawBytes;
-  };
-  // It has been read (its values are stored): the slot's next copies.
-  auto done = [&]() {
-    __syncwarp();
-    if (++slot == C::kRaw) slot = 0;
-    --ahead;
-    fill();
-  };
   Item it;
   for (int n = 0;; ++n) {
     if (!x.next(n, it) || it.t1 < 0) return;
     const int nt = it.t1 - it.t0;
-    fill();
     if (nt) {
       if (n_load && !x.wait_warp(x.q_free, n_load - 1)) return;
       ++n_load;
@@ -995,10 +972,25 @@ __device__ void widen_role(const ChunkParams& p, const Ctx<true>& x, int tpt) {
       const int b0 = (it.t0 + j) * kTileBlocks, nb = min(kTileBlocks, nblk - b0);
       // ---- K tile
       if (key >= C::kKStages && !x.wait_warp(&x.k_empty[k.st], k.ph ^ 1)) return;
-      const uint8_t* src = landed();
+      // block b of the tile is at raw0 (b < kGroup) or raw1 + b * chunk
+      const bool second = nb > kGroup;
+      RingPos<C::kRaw> g2 = g;
+      g2.next();
+      if (!x.wait_warp(&x.raw_full[g.st], g.ph)) return;
+      if (second && !x.wait_warp(&x.raw_full[g2.st], g2.ph)) return;
+      const uint8_t* raw0 = x.smem + C::kOffRaw + g.st * kGroup * kFp8HeadBlockBytes;
+      const uint8_t* raw1 =
+          x.smem + C::kOffRaw + g2.st * kGroup * kFp8HeadBlockBytes - kGroup * kFp8HeadBlockBytes;
+      // lane: four tokens of block lane / 4
+      const uint8_t* mine = ((lane >> 2) < kGroup ? raw0 : raw1) + (lane >> 2) * kFp8HeadBlockBytes +
+                            (lane & 3) * 16;
+      float4 vs = make_float4(0.f, 0.f, 0.f, 0.f);
       {
-        const float4 f = *reinterpret_cast<const float4*>(src + kKeys * kHeadDim +
-                                                          (c >> 5) * kKeys * 4 + lane * 16);
+        float4 f = vs;
+        if ((lane >> 2) < nb) {
+          f = *reinterpret_cast<const float4*>(mine + kFp8KScaleOff);
+          vs = *reinterpret_cast<const float4*>(mine + kFp8VScaleOff);
+        }
         const float v[4] = {f.x, f.y, f.z, f.w};
         uint32_t w[8];
 #pragma unroll
@@ -1015,7 +1007,8 @@ __device__ void widen_role(const ChunkParams& p, const Ctx<true>& x, int tpt) {
       uint8_t* dst = x.smem + C::kOffK + k.st * kOperand + k_dst;
 #pragma unroll 4
       for (int b = 0; b < nb; ++b) {
-        const uint4 raw = *reinterpret_cast<const uint4*>(src + b * 2048 + c * 16);
+        const uint4 raw = *reinterpret_cast<const uint4*>((b < kGroup ? raw0 : raw1) +
+                                                          b * kFp8HeadBlockBytes + k_src);
         const uint2 sc = *reinterpret_cast<const uint2*>(scales + (b * kBlockTokens + tok) * 8);
         uint4 lo, hi;
         widen_k(raw.x, sc.x, sc.y, lo.x, hi.x);
@@ -1029,22 +1022,19 @@ __device__ void widen_role(const ChunkParams& p, const Ctx<true>& x, int tpt) {
       __syncwarp();
       if (lane == 0) mbar_arrive(&x.k_full[k.st]);
       k.next();
-      done();
       // ---- V tile
       if (key >= C::kVStages && !x.wait_warp(&x.v_empty[v.st], v.ph ^ 1)) return;
-      src = landed();
       {
-        const float4 s = *reinterpret_cast<const float4*>(src + kKeys * kHeadDim +
-                                                          (c >> 5) * kKeys * 4 + lane * 16);
         *reinterpret_cast<uint2*>(scales + lane * 8) =
-            make_uint2(pack_f16(s.x, s.y), pack_f16(s.z, s.w));
+            make_uint2(pack_f16(vs.x, vs.y), pack_f16(vs.z, vs.w));
         __syncwarp();
       }
       dst = x.smem + C::kOffV + v.st * kOperand + c * 128;
       const int valid = it.kv - b0 * kBlockTokens;  // positions from the tile's first on
 #pragma unroll 4
       for (int b = 0; b < nb; ++b) {
-        const uint4 raw = *reinterpret_cast<const uint4*>(src + b * 2048 + c * 16);
+        const uint4 raw = *reinterpret_cast<const uint4*>((b < kGroup ? raw0 : raw1) +
+                                                          b * kFp8HeadBlockBytes + kFp8VOff + c * 16);
         const uint4 sl = *reinterpret_cast<const uint4*>(scales + b * 32);
         const uint4 sh = *reinterpret_cast<const uint4*>(scales + b * 32 + 16);
         uint4 lo, hi;
@@ -1073,10 +1063,17 @@ __device__ void widen_role(const ChunkParams& p, const Ctx<true>& x, int tpt) {
       }
       fence_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&x.v_full[v.st]);
+      if (lane == 0) {
+        mbar_arrive(&x.v_full[v.st]);
+        // behind the stores: every load of the chunks has returned by then,
+        // which an arrive right behind the loads would not wait for
+        mbar_arrive(&x.raw_empty[g.st]);
+        if (second) mbar_arrive(&x.raw_empty[g2.st]);
+      }
       v.next();
       ++key;
-      done();
+      g.next();
+      if (second) g.next();
     }
   }
 }
@@ -1174,7 +1171,7 @@ __device__ void q_role(const ChunkParams& p, const Ctx<false>& x, int tpt) {
     if (!x.next(n, it) || it.t1 < 0) return;
     if (it.t1 == 0) continue;
     if (n_load && !x.wait_warp(x.q_free, n_load - 1)) return;
-    load_q(p, x.smem + Cfg<false>::kOffQ, it, tpt, threadIdx.x - 416);
+    load_q(p, x.smem + Cfg<false>::kOffQ, it, tpt, threadIdx.x - 384);
     fence_async_smem();
     __syncwarp();
     if ((threadIdx.x & 31) == 0) mbar_arrive(x.q_full);
@@ -1208,7 +1205,7 @@ __global__ void __launch_bounds__(Cfg<kFp8>::kThreads, 1)
     }
     for (int i = 0; i < kItemRing; ++i) {
       mbar_init(&x.item_full[i], 1);
-      mbar_init(&x.item_empty[i], kFp8 ? 14 : 15);  // the warps that read items
+      mbar_init(&x.item_empty[i], 15);  // every warp but warp 3
     }
     mbar_init(x.q_full, kFp8 ? 4 : 3);
     mbar_init(x.q_free, 1);
@@ -1229,6 +1226,10 @@ __global__ void __launch_bounds__(Cfg<kFp8>::kThreads, 1)
     mbar_init(x.ml_bar, 8);
     mbar_init(x.ep_bar, 8);
     mbar_init(x.mma_done, 2);
+    for (int i = 0; i < C::kRaw; ++i) {
+      mbar_init(&x.raw_full[i], 1);
+      mbar_init(&x.raw_empty[i], 4);
+    }
     fence_mbar_init();
     s_row = p.batch;
     s_base = 0;
@@ -1284,7 +1285,9 @@ __global__ void __launch_bounds__(Cfg<kFp8>::kThreads, 1)
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kRegsLow));
     if (warp == 0) {
-      if constexpr (!kFp8)
+      if constexpr (kFp8)
+        copy_role(p, x);
+      else
         copy_role<C::kKStages>(p, x, &kmap, x.k_full, x.k_empty, smem + C::kOffK);
     } else if (warp == 1) {
       qk_role<kFp8>(p, x, tmem);
@@ -1306,7 +1309,7 @@ __global__ void __launch_bounds__(Cfg<kFp8>::kThreads, 1)
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kRegsAux));
     if constexpr (kFp8) {
       widen_role(p, x, w.tpt);
-    } else if (warp == 12) {
+    } else if (warp == 15) {  // (not on warp 0's scheduler)
       copy_role<C::kVStages>(p, x, &vmap, x.v_full, x.v_empty, smem + C::kOffV);
     } else {
       q_role(p, x, w.tpt);
@@ -1351,92 +1354,90 @@ __device__ __forceinline__ void merge_row(const float* lse, const float* part, i
   *reinterpret_cast<uint2*>(out + lane * 4) = pk;
 }
 
-// Blocks [0, n_long) x grid.y: the items that chunk_kernel's CTAs cut, by the
-// CTA that holds their first keys; the others, the short kernel's units.
-__global__ void __launch_bounds__(256) merge_kernel(const ChunkParams p, const ShortParams q,
-                                                    int n_long, int y_long) {
+// Block (CTA, y): the item that chunk_kernel's CTA cut, where it has its first keys.
+__global__ void __launch_bounds__(256) merge_kernel(const ChunkParams p) {
   pdl_trigger();
   pdl_wait();
-  const int warp = threadIdx.x >> 5;
-  int unit = blockIdx.x - n_long * y_long;
-  if (unit < 0) {
-    const int cta = blockIdx.x / y_long, y = blockIdx.x - cta * y_long;
-    const int4 d = __ldcg(p.desc + cta);
-    if (d.x < 2) return;
-    const int tpt = kRows / p.group, rows = d.z * p.group;
-    for (int i = y * 8 + warp; i < rows; i += y_long * 8) {
-      const int tok = i / p.group, head = d.w * p.group + i - tok * p.group;
-      const int prow = (d.z > tpt && tok >= tpt) ? kRows + i - tpt * p.group : i;
-      merge_row(p.part_lse, p.part_o, d.x,
-                [&](int c) -> int64_t {
-                  return ((static_cast<int64_t>(cta) + c) * 2 + (c == 0 ? 1 : 0)) * p.part_rows + prow;
-                },
-                p.out + static_cast<int64_t>(d.y + tok) * p.o_st + head * p.o_sh);
-    }
-    return;
-  }
-  const int b = unit / q.hkv, h = unit - b * q.hkv;
-  const ShortRow r = short_row(q, b);
-  if (r.T == 0 || r.nparts < 2) return;
-  for (int i = warp; i < r.T * q.group; i += 8) {
-    const int tok = i / q.group, head = h * q.group + i - tok * q.group;
-    merge_row(q.part_lse, q.part_o, r.nparts,
+  const int cta = blockIdx.x;
+  const int4 d = __ldcg(p.desc + cta);
+  if (d.x < 2) return;
+  const int tpt = kRows / p.group, rows = d.z * p.group;
+  for (int i = blockIdx.y * 8 + (threadIdx.x >> 5); i < rows; i += gridDim.y * 8) {
+    const int tok = i / p.group, head = d.w * p.group + i - tok * p.group;
+    const int prow = (d.z > tpt && tok >= tpt) ? kRows + i - tpt * p.group : i;
+    merge_row(p.part_lse, p.part_o, d.x,
               [&](int c) -> int64_t {
-                return (static_cast<int64_t>(unit) * q.max_parts + c) * q.part_rows + i;
+                return ((static_cast<int64_t>(cta) + c) * 2 + (c == 0 ? 1 : 0)) * p.part_rows + prow;
               },
-              q.out + static_cast<int64_t>(r.first + tok) * q.o_st + head * q.o_sh);
+              p.out + static_cast<int64_t>(d.y + tok) * p.o_st + head * p.o_sh);
   }
 }
 
 // ---------------------------------------------------------------- host
+int sm_count() {
+  static std::atomic<int> known[64];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) {
+    cudaGetLastError();
+    return 148;
+  }
+  std::atomic<int>& k = known[dev & 63];
+  int sms = k.load();
+  if (sms == 0) {
+    if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 148;
+    k.store(sms);
+  }
+  return sms;
+}
+
 struct ChunkPlan {
-  int grid, part_rows;                           // chunk_kernel; grid 0: not needed
-  int parts, min_blocks, short_rows;             // short kernel
+  int grid, part_rows;             // chunk_kernel; grid 0: not needed
+  int short_rows, chunks, parts;   // short kernel; short_rows 0: not needed
 };
 
+// Which sequences are the short kernel's: those of at most 16 query rows per
+// KV head over the bf16 pool, 32 over FP8 (where half the bytes and twice the
+// work per byte leave chunk_kernel behind until then), and all of them in a
+// call of at most kSmallRows rows, which then is one launch.
+constexpr int kSmallRows = 128;
+constexpr int kShortCtas = 148 * 2;  // CTAs the short kernel is split into, if long enough
+constexpr int kShortMinBlocks = 8;       // per partition: two per warp
 // chunk_kernel: one CTA per SM, fewer where the launch's sizes cannot give
-// each kMinStep.  Short kernel: enough partitions per (sequence, KV head) for
-// kShortCtas CTAs of at least kShortMinBlocks blocks (two per warp).
-constexpr int kShortCtas = 148 * 2 * 4;
-constexpr int kShortMinBlocks = 8;
+// each kMinStep.
 ChunkPlan plan_chunk(int32_t batch, int32_t tokens, int32_t hq, int32_t hkv, int32_t max_kv_len,
                      bool fp8) {
-  int dev = 0, sms = 148;
-  if (cudaGetDevice(&dev) == cudaSuccess)
-    cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  cudaGetLastError();
   const int group = hq / hkv, tpt = kRows / group, tiles = fp8 ? 1 : 2;
-  ChunkPlan pl{};
   const int64_t most = static_cast<int64_t>(tokens) * group;  // rows of one sequence
-  if (tokens > kShortRows / group) {
-    const int64_t items = (static_cast<int64_t>(tokens) / (tpt * tiles) +
-                           std::min(batch, tokens / (kShortRows / group + 1))) * hkv;
+  ChunkPlan pl{};
+  pl.short_rows = most <= kSmallRows ? kSmallRows : (fp8 ? 32 : 16);
+  pl.chunks = most <= kSmallRows ? static_cast<int>((most + kShortRows - 1) / kShortRows) : 1;
+  if (pl.short_rows < group) pl.short_rows = pl.chunks = 0;  // not one token
+  if (pl.short_rows) {
+    const int64_t units = static_cast<int64_t>(batch) * hkv * pl.chunks;
+    const int nblk = max_kv_len / kBlockTokens + 1;
+    const int64_t want = std::min<int64_t>((kShortCtas + units - 1) / units,
+                                           std::max(1, nblk / kShortMinBlocks));
+    pl.parts = 1;
+    while (pl.parts * 2 <= want && pl.parts < 16) pl.parts *= 2;
+  }
+  if (most > pl.short_rows) {
+    const int64_t longest = std::min<int64_t>(batch, tokens / (pl.short_rows / group + 1));
+    const int64_t items = (static_cast<int64_t>(tokens) / (tpt * tiles) + longest) * hkv;
     const int64_t item = kItemCost + static_cast<int64_t>(tiles) * max_kv_len;
+    const int sms = sm_count();
     const int64_t want =
         items > (int64_t(1) << 40) / item ? sms : (items * item + kMinStep - 1) / kMinStep;
     pl.grid = static_cast<int>(want < 1 ? 1 : (want < sms ? want : sms));
     // rows of a partial: those of one item (tile B starts at row 128)
     pl.part_rows = tokens > tpt ? tiles * kRows : static_cast<int>((most + 7) / 8 * 8);
   }
-  const int64_t units = static_cast<int64_t>(batch) * hkv;
-  const int nblk = max_kv_len / kBlockTokens + 1;
-  int64_t parts = (kShortCtas + units - 1) / units;
-  parts = std::min<int64_t>(parts, std::max(1, nblk / kShortMinBlocks));
-  pl.parts = static_cast<int>(std::min<int64_t>(parts, 64));
-  pl.min_blocks = kShortMinBlocks;
-  pl.short_rows = static_cast<int>(std::min<int64_t>(kShortRows, (most + 7) / 8 * 8));
   return pl;
 }
 
-// Workspace: descriptors, sums and partials of chunk_kernel, then sums and
-// partials of the short kernel.
-size_t long_bytes(const ChunkPlan& pl) {
+// Descriptors, sums and partials of chunk_kernel.
+size_t plan_bytes(const ChunkPlan& pl) {
   if (pl.grid < 2) return 0;
   return static_cast<size_t>(pl.grid) * (16 + 2 * static_cast<size_t>(pl.part_rows) * (kHeadDim + 1) * 4);
-}
-size_t short_bytes(const ChunkPlan& pl, int64_t units) {
-  if (pl.parts < 2) return 0;
-  return static_cast<size_t>(units) * pl.parts * pl.short_rows * (kHeadDim + 1) * 4;
 }
 
 template <bool kFp8>
@@ -1444,8 +1445,16 @@ cudaError_t launch_chunk_t(const ChunkParams& p, const CUtensorMap& kmap, const 
                            int grid, cudaStream_t stream) {
   using C = Cfg<kFp8>;
   auto kern = chunk_kernel<kFp8>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+  static std::atomic<uint64_t> ready{0};  // a bit per device
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
+  const uint64_t bit = uint64_t(1) << (dev & 63);
+  if (!(ready.load() & bit)) {
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+    if (e != cudaSuccess) return e;
+    ready.fetch_or(bit);
+  }
   return launch_k(kern, dim3(grid), dim3(C::kThreads), static_cast<size_t>(C::kSmem), stream, p,
                   kmap, vmap);
 }
@@ -1463,10 +1472,8 @@ bool registers_as_planned() {
 
 size_t chunk_workspace_bytes(int32_t batch, int32_t tokens, int32_t hq, int32_t hkv,
                              int32_t max_kv_len) {
-  const ChunkPlan a = plan_chunk(batch, tokens, hq, hkv, max_kv_len, false);
-  const ChunkPlan b = plan_chunk(batch, tokens, hq, hkv, max_kv_len, true);
-  return std::max(long_bytes(a), long_bytes(b)) +
-         short_bytes(a, static_cast<int64_t>(batch) * hkv);  // the same for both
+  return std::max(plan_bytes(plan_chunk(batch, tokens, hq, hkv, max_kv_len, false)),
+                  plan_bytes(plan_chunk(batch, tokens, hq, hkv, max_kv_len, true)));
 }
 
 cudaError_t launch_chunk(const ChunkLaunch& a, cudaStream_t stream) {
@@ -1502,48 +1509,39 @@ cudaError_t launch_chunk(const ChunkLaunch& a, cudaStream_t stream) {
     p.part_lse = reinterpret_cast<float*>(p.desc + pl.grid);
     p.part_o = p.part_lse + static_cast<int64_t>(pl.grid) * 2 * pl.part_rows;
   }
-  const int64_t units = static_cast<int64_t>(a.batch) * a.num_kv_heads;
-  ShortParams q{};
-  q.q = p.q;
-  q.q_st = p.q_st;
-  q.q_sh = p.q_sh;
-  q.out = p.out;
-  q.o_st = p.o_st;
-  q.o_sh = p.o_sh;
-  q.kv8 = p.kv8;
-  q.tables = p.tables;
-  q.pitch = p.pitch;
-  q.rows = p.rows;
-  q.q_starts = p.q_starts;
-  q.kv_lens = p.kv_lens;
-  q.tokens = p.tokens;
-  q.hkv = p.hkv;
-  q.group = p.group;
-  q.num_blocks = p.num_blocks;
-  q.causal = p.causal;
-  q.max_parts = pl.parts;
-  q.min_blocks = pl.min_blocks;
-  q.part_rows = pl.short_rows;
-  q.scale_log2 = a.sm_scale * 1.4426950408889634f;
-  q.err = a.err;
-  if (pl.parts > 1) {
-    q.part_lse = reinterpret_cast<float*>(static_cast<uint8_t*>(a.workspace) + long_bytes(pl));
-    q.part_o = q.part_lse + units * pl.parts * pl.short_rows;
-  }
-  if (kShortRows / p.group > 0) {
-    const cudaError_t e = launch_chunk_short(q, a.kmap, a.vmap, a.batch, stream);
+  p.short_rows = pl.short_rows;
+  if (pl.short_rows > 0) {
+    ShortParams q{};
+    q.q = p.q;
+    q.q_st = p.q_st;
+    q.q_sh = p.q_sh;
+    q.out = p.out;
+    q.o_st = p.o_st;
+    q.o_sh = p.o_sh;
+    q.kv8 = p.kv8;
+    q.tables = p.tables;
+    q.pitch = p.pitch;
+    q.rows = p.rows;
+    q.q_starts = p.q_starts;
+    q.kv_lens = p.kv_lens;
+    q.tokens = p.tokens;
+    q.hkv = p.hkv;
+    q.group = p.group;
+    q.num_blocks = p.num_blocks;
+    q.causal = p.causal;
+    q.most_rows = pl.short_rows;
+    q.chunks = pl.chunks;
+    q.min_blocks = kShortMinBlocks;
+    q.scale_log2 = a.sm_scale * 1.4426950408889634f;
+    q.err = a.err;
+    const cudaError_t e = launch_chunk_short(q, a.kmap, a.vmap, a.batch, pl.parts, stream);
     if (e != cudaSuccess) return e;
   }
-  if (pl.grid > 0) {
-    const cudaError_t e = fp8 ? launch_chunk_t<true>(p, a.kmap, a.vmap, pl.grid, stream)
-                              : launch_chunk_t<false>(p, a.kmap, a.vmap, pl.grid, stream);
-    if (e != cudaSuccess) return e;
-  }
-  const int n_long = pl.grid > 1 ? pl.grid : 0, y_long = (pl.part_rows + 15) / 16;
-  const int64_t blocks = static_cast<int64_t>(n_long) * y_long + (pl.parts > 1 ? units : 0);
-  if (blocks == 0) return cudaSuccess;
-  return launch_k(merge_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream, p, q,
-                  n_long, y_long);
+  if (pl.grid == 0) return cudaSuccess;
+  const cudaError_t e = fp8 ? launch_chunk_t<true>(p, a.kmap, a.vmap, pl.grid, stream)
+                            : launch_chunk_t<false>(p, a.kmap, a.vmap, pl.grid, stream);
+  if (e != cudaSuccess || pl.grid < 2) return e;
+  return launch_k(merge_kernel, dim3(pl.grid, (pl.part_rows + 15) / 16), dim3(256), 0, stream, p);
 }
 
 }  // namespace pkv

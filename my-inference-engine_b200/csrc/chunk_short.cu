@@ -1,11 +1,14 @@
-// Packed-chunk attention, sequences of few new tokens: T * group <= 32 query
-// rows per KV head (decode rows, checks of drafted tokens).  HBM-bound: every
-// K/V block is read once for all of a sequence's rows of a KV head.
+// Packed-chunk attention, sequences of few new tokens (at most 32 query rows,
+// tokens times heads of a group, per KV head), and small calls altogether, in
+// chunks of 32 rows.  HBM-bound: every K/V block is read once for the chunk.
 //
-//   grid  = (partitions, KV heads, sequences), sequences with more rows leave
-//   block = 4 warps; warp w takes blocks w, w + 4, ... of its partition and
-//           streams them through its own ring of copies (bf16: TMA boxes of K
-//           and V; FP8: one bulk copy of the block's chunk)
+//   grid    = (partitions, KV heads, sequences x chunks)
+//   cluster = the partitions of one unit (up to 16): they join through
+//             distributed shared memory, so a call is one launch and needs no
+//             workspace
+//   block   = 4 warps; warp w takes blocks w, w + 4, ... of its partition and
+//             streams them through its own ring of copies (bf16: TMA boxes of
+//             K and V; FP8: one bulk copy of the block's chunk)
 //
 // One warp, one 16-token block, keys in M and query rows in N (mma.sync
 // m16n8k16; NT tiles of 8 rows: token n / group, head n % group):
@@ -16,11 +19,16 @@
 //                                             ldmatrix.trans
 // FP8: fragments are e4m3 pairs widened to f16 in registers (exact), q / 16 as
 // f16, the key's scale applied to its scores and the value's to its
-// probabilities after the row's sum.  The warps join in shared memory;
-// partitions leave fp32 partials (o / l, log2-sum-exp) for the merge kernel.
-// Every row's partitions follow from its own length, so a captured call
-// replays for other lengths.
+// probabilities after the row's sum.  The warps join in shared memory, then
+// the partitions.  Every row's partitions follow from its own length, so a
+// captured call replays for other lengths.
+//
+// mma.sync runs at about a tenth of the tensor cores' rate: 32 rows of bf16
+// are bound by it (64 sequences of 5 tokens at 6 heads, 347 MB: 112 us here,
+// 71 us in chunk.cu), 16 are not.
 #include <math.h>
+
+#include <atomic>
 
 #include "chunk.cuh"
 
@@ -37,7 +45,9 @@ struct Short {
   static constexpr int kOffQ = kWarps * kStages * kStageBytes;    // [32][128] 16-bit, swizzled
   static constexpr int kOffBar = kOffQ + kShortRows * 256;
   static constexpr int kSmem = kOffBar + kWarps * kStages * 8 + 1024;
-  static_assert(kOffQ >= kWarps * kShortRows * (kHeadDim + 2) * 4,
+  // where the CTA leaves its joined rows for the cluster: [32][128], [32][2]
+  static constexpr int kOffJoin = kWarps * kShortRows * (kHeadDim + 2) * 4;
+  static_assert(kOffQ >= kOffJoin + kShortRows * (kHeadDim + 2) * 4,
                 "the join of the warps reuses the ring");
   static_assert(kSmem <= 113 * 1024, "two CTAs per SM");
 };
@@ -52,8 +62,33 @@ __device__ __forceinline__ void mma16(float (&d)[4], uint32_t a0, uint32_t a1, u
     mma_bf16(d, a0, a1, a2, a3, b0, b1);
 }
 
+// A cluster's barrier, and 16 bytes of another of its CTAs' shared memory.
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::
+                   : "memory");
+}
+__device__ __forceinline__ uint32_t cluster_addr(const void* p, int rank) {
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+  return a;
+}
+__device__ __forceinline__ float4 cluster_ld4(uint32_t a) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(a)
+               : "memory");
+  return v;
+}
+__device__ __forceinline__ float2 cluster_ld2(uint32_t a) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(a) : "memory");
+  return v;
+}
+
 struct ShortItem {
   int first, T, kv;      // packed token, tokens, positions
+  int row0, rows;        // the chunk's rows of the sequence
   int blk0, blk1;        // blocks of this partition
   int part, nparts;
   const int32_t* trow;
@@ -69,7 +104,7 @@ __device__ __forceinline__ void short_part(const ShortParams& p, const CUtensorM
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int g = lane >> 2, t = lane & 3;
   const DevErr err{p.err};
-  const int rows = it.T * p.group;
+  const int rows = it.rows;
   const int span = it.blk1 - it.blk0;
   const int my_n = span > warp ? (span - warp + kWarps - 1) / kWarps : 0;
 
@@ -113,7 +148,7 @@ __device__ __forceinline__ void short_part(const ShortParams& p, const CUtensorM
     const int n = i >> 4, c = i & 15;
     uint4 v = make_uint4(0, 0, 0, 0);
     if (n < rows) {
-      const int tok = n / p.group, head = kvh * p.group + n - tok * p.group;
+      const int tok = (it.row0 + n) / p.group, head = kvh * p.group + it.row0 + n - tok * p.group;
       v = *reinterpret_cast<const uint4*>(p.q + (it.first + tok) * p.q_st + head * p.q_sh + c * 8);
       if constexpr (kFp8) {
         uint32_t* w = reinterpret_cast<uint32_t*>(&v);
@@ -135,9 +170,10 @@ __device__ __forceinline__ void short_part(const ShortParams& p, const CUtensorM
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       const int n = nt * 8 + 2 * t + u;
-      lim[nt][u] = n >= rows ? 0 : (p.causal ? min(it.kv, it.kv - it.T + n / p.group + 1) : it.kv);
+      lim[nt][u] = n >= rows ? 0 : (p.causal ? min(it.kv, it.kv - it.T + (it.row0 + n) / p.group + 1) : it.kv);
     }
-  const int clear = p.causal ? it.kv - it.T + 1 : it.kv;  // keys below are visible to all rows
+  // keys below are visible to all rows
+  const int clear = p.causal ? it.kv - it.T + it.row0 / p.group + 1 : it.kv;
 
   float m[NT][2], l[NT][2], o[NT][8][4];
 #pragma unroll
@@ -363,7 +399,16 @@ __device__ __forceinline__ void short_part(const ShortParams& p, const CUtensorM
     }
   }
   __syncthreads();
-  const int64_t slot = (static_cast<int64_t>(blockIdx.z) * p.hkv + kvh) * p.max_parts + it.part;
+  float* po = reinterpret_cast<float*>(smem + C::kOffJoin);   // [32][128]
+  float* pm = po + kShortRows * kHeadDim;                      // [32] (base, sum)
+  auto store = [&](int n, float4 acc, float sum) {
+    const float inv = 1.f / sum;  // 0/0 -> NaN for a token that sees no key
+    const int tok = (it.row0 + n) / p.group, head = kvh * p.group + it.row0 + n - tok * p.group;
+    uint2 pk;
+    pk.x = pack_bf16(acc.x * inv, acc.y * inv);
+    pk.y = pack_bf16(acc.z * inv, acc.w * inv);
+    *reinterpret_cast<uint2*>(p.out + (it.first + tok) * p.o_st + head * p.o_sh + lane * 4) = pk;
+  };
   for (int n = warp; n < rows; n += kWarps) {  // a warp per row, lane: dims 4l .. 4l + 3
     float M = -INFINITY;
 #pragma unroll
@@ -383,19 +428,36 @@ __device__ __forceinline__ void short_part(const ShortParams& p, const CUtensorM
       acc.w += f * v.w;
     }
     if (it.nparts == 1) {
-      const float inv = 1.f / L;  // 0/0 -> NaN for a token that sees no key
-      const int tok = n / p.group, head = kvh * p.group + n - tok * p.group;
-      uint2 pk;
-      pk.x = pack_bf16(acc.x * inv, acc.y * inv);
-      pk.y = pack_bf16(acc.z * inv, acc.w * inv);
-      *reinterpret_cast<uint2*>(p.out + (it.first + tok) * p.o_st + head * p.o_sh + lane * 4) = pk;
+      store(n, acc, L);
     } else {
-      const float inv = L > 0.f ? 1.f / L : 0.f;
-      *reinterpret_cast<float4*>(p.part_o + (slot * p.part_rows + n) * kHeadDim + lane * 4) =
-          make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
-      if (lane == 0) p.part_lse[slot * p.part_rows + n] = L > 0.f ? base + log2f(L) : -INFINITY;
+      *reinterpret_cast<float4*>(po + n * kHeadDim + lane * 4) = acc;
+      if (lane == 0) *reinterpret_cast<float2*>(pm + 2 * n) = make_float2(M, L);
     }
   }
+  if (it.nparts == 1) return;
+  // ---- join the partitions, in key order; each CTA of the cluster finishes
+  // every nparts-th row (CTAs past the last partition have left)
+  cluster_sync();
+  for (int n = it.part + it.nparts * warp; n < rows; n += it.nparts * kWarps) {
+    float M = -INFINITY;
+    for (int c = 0; c < it.nparts; ++c) M = fmaxf(M, cluster_ld2(cluster_addr(pm + 2 * n, c)).x);
+    const float base = M == -INFINITY ? 0.f : M;
+    float L = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int c = 0; c < it.nparts; ++c) {
+      const float2 ml = cluster_ld2(cluster_addr(pm + 2 * n, c));
+      const float4 v = cluster_ld4(cluster_addr(po + n * kHeadDim + lane * 4, c));
+      const float f = ex2(ml.x - base);
+      L += f * ml.y;
+      acc.x += f * v.x;
+      acc.y += f * v.y;
+      acc.z += f * v.z;
+      acc.w += f * v.w;
+    }
+    store(n, acc, L);
+  }
+  cluster_sync();  // no CTA leaves while another reads its rows
 }
 
 template <bool kFp8>
@@ -408,7 +470,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
                                              ~static_cast<uintptr_t>(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kOffBar);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int b = blockIdx.z, kvh = blockIdx.y;
+  const int b = blockIdx.z / p.chunks, chunk = blockIdx.z - b * p.chunks, kvh = blockIdx.y;
   pdl_trigger();
   if (lane == 0) {
     for (int s = 0; s < C::kStages; ++s) mbar_init(&bars[warp * C::kStages + s], 1);
@@ -420,21 +482,35 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
   }
   __syncwarp();
   pdl_wait();
-  const ShortRow r = short_row(p, b);
-  if (r.T == 0 || static_cast<int>(blockIdx.x) >= r.nparts) return;
-  if (r.cut && blockIdx.x == 0 && kvh == 0 && threadIdx.x == 0)
-    DevErr{p.err}.raise(PKV_DEVERR_POSITION);
+  // (a whole cluster takes the same way here: all of it is one unit)
+  const int s0 = min(max(__ldg(p.q_starts + b), 0), p.tokens);
+  const int s1 = min(max(__ldg(p.q_starts + b + 1), s0), p.tokens);
+  const int len = max(__ldg(p.kv_lens + b), 0);
   ShortItem it;
-  it.first = r.first;
-  it.T = r.T;
-  it.kv = r.kv;
+  it.first = s0;
+  it.T = s1 - s0;
+  it.row0 = chunk * kShortRows;
+  it.rows = min(it.T * p.group - it.row0, kShortRows);
+  if (it.rows <= 0 || it.T * p.group > p.most_rows) return;
+  it.kv = static_cast<int>(min(static_cast<int64_t>(len),
+                               min(p.pitch, int64_t(1) << 26) * kBlockTokens));
+  if (len > it.kv && blockIdx.x == 0 && kvh == 0 && threadIdx.x == 0)
+    DevErr{p.err}.raise(PKV_DEVERR_POSITION);
+  // equal partitions of whole rounds of the four warps; no position: one
+  // empty partition, which writes the NaN rows
+  const int nblk = (it.kv + kBlockTokens - 1) / kBlockTokens;
+  const int np = min(static_cast<int>(gridDim.x), max(1, nblk / p.min_blocks));
+  const int per = max(kWarps, ((nblk + np - 1) / np + kWarps - 1) / kWarps * kWarps);
+  it.nparts = max(1, (nblk + per - 1) / per);
   it.part = blockIdx.x;
-  it.nparts = r.nparts;
-  it.blk0 = it.part * r.per_part;
-  it.blk1 = min(r.nblk, it.blk0 + r.per_part);
+  if (it.part >= it.nparts) return;
+  it.blk0 = it.part * per;
+  it.blk1 = min(nblk, it.blk0 + per);
   it.trow = p.tables + static_cast<int64_t>(p.rows ? p.rows[b] : b) * p.pitch;
-  if (r.T * p.group <= 8)
+  if (it.rows <= 8)
     short_part<kFp8, 1>(p, &kmap, &vmap, smem, bars, it, kvh);
+  else if (it.rows <= 16)
+    short_part<kFp8, 2>(p, &kmap, &vmap, smem, bars, it, kvh);
   else
     short_part<kFp8, kMaxNT>(p, &kmap, &vmap, smem, bars, it, kvh);
 }
@@ -444,18 +520,41 @@ cudaError_t launch_short_t(const ShortParams& p, const CUtensorMap& kmap, const 
                            dim3 grid, cudaStream_t stream) {
   using C = Short<kFp8>;
   auto kern = chunk_short_kernel<kFp8>;
-  const cudaError_t e =
-      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+  static std::atomic<uint64_t> ready{0};  // a bit per device
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
-  return launch_k(kern, grid, dim3(kWarps * 32), static_cast<size_t>(C::kSmem), stream, p, kmap,
-                  vmap);
+  const uint64_t bit = uint64_t(1) << (dev & 63);
+  if (!(ready.load() & bit)) {
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+    if (e == cudaSuccess)
+      e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e != cudaSuccess) return e;
+    ready.fetch_or(bit);
+  }
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(kWarps * 32);
+  cfg.dynamicSmemBytes = C::kSmem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2] = {};
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = grid.x;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl_enabled() ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kern, p, kmap, vmap);
 }
 
 }  // namespace
 
 cudaError_t launch_chunk_short(const ShortParams& p, const CUtensorMap& kmap,
-                               const CUtensorMap& vmap, int32_t batch, cudaStream_t stream) {
-  const dim3 grid(p.max_parts, p.hkv, batch);
+                               const CUtensorMap& vmap, int32_t batch, int32_t parts,
+                               cudaStream_t stream) {
+  const dim3 grid(parts, p.hkv, batch * p.chunks);
   return p.kv8 ? launch_short_t<true>(p, kmap, vmap, grid, stream)
                : launch_short_t<false>(p, kmap, vmap, grid, stream);
 }

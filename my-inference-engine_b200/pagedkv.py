@@ -9,6 +9,7 @@ missing or cannot be loaded, `lib()` raises.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 import threading
 from pathlib import Path
@@ -29,6 +30,7 @@ LINEAR_MAX_ROWS = 256  # PKV_LINEAR_MAX_ROWS
 LAYERS_MAX_ROWS = 32  # PKV_LAYERS_MAX_ROWS
 LAYERS_MAX_LAYERS = 32  # PKV_LAYERS_MAX_LAYERS
 W_ROWMAJOR, W_TILED, W_GATE_UP_PAIRED = 0, 1, 2  # PKV_W_* layouts
+_FP8_BLOCK_BYTES = 4224  # pkv_fp8_block_bytes()
 
 _c_i32p = ctypes.POINTER(ctypes.c_int32)
 _vp = ctypes.c_void_p
@@ -508,13 +510,39 @@ def linear_rope_append(x: torch.Tensor, w_qkv: torch.Tensor, bias: torch.Tensor 
 
 
 # ---------------------------------------------------------------- packed chunks
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def _stream_of(index: int) -> int:
+    """The current stream of device `index` (torch's own handle when it has
+    one to give: an eighth of current_stream's time)."""
+    return _raw_stream(index) if _raw_stream is not None else torch.cuda.current_stream(index).cuda_stream
+
+
+class _OnDevice:
+    """Runs a call with the tensors' device current, if it is not already."""
+
+    __slots__ = ("guard",)
+
+    def __init__(self, index: int):
+        self.guard = None if torch.cuda.current_device() == index else torch.cuda.device(index)
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+
+
 def _int32_vector(t: torch.Tensor, what: str, device: torch.device, n: int | None = None) -> None:
     if t.dtype != torch.int32 or t.dim() != 1 or (n is not None and t.shape[0] != n):
         raise ValueError(f"{what} must be an int32 vector{'' if n is None else f' of {n}'}, "
                          f"got {t.dtype} {tuple(t.shape)}")
     if t.device != device:
         raise ValueError(f"{what} is on {t.device}, expected {device}")
-    if t.shape[0] > 1 and t.stride(0) != 1:
+    if not t.is_contiguous():
         raise ValueError(f"{what} must be contiguous")
 
 
@@ -531,16 +559,17 @@ def _check_tables(tables: torch.Tensor, device: torch.device) -> None:
         raise ValueError("table rows must be contiguous")
 
 
-def _chunk_args(q, tables, rows, q_starts, kv_lens, max_kv_len, out, num_kv_heads, err):
+def _chunk_args(q, tables, rows, q_starts, kv_lens, max_kv_len, out, err):
     """Checks both packed-chunk calls share; returns (tokens, Hq, batch)."""
     dev = q.device
     if dev.type != "cuda":
         raise ValueError("Expected CUDA tensors")
-    if q.dtype != torch.bfloat16 or q.dim() != 3 or q.shape[2] != HEAD_DIM:
-        raise ValueError(f"q must be bf16 [tokens, heads, {HEAD_DIM}], got {q.dtype} {tuple(q.shape)}")
-    if out.dtype != torch.bfloat16 or out.shape != q.shape or out.device != dev:
+    shape = q.shape
+    if q.dtype != torch.bfloat16 or len(shape) != 3 or shape[2] != HEAD_DIM:
+        raise ValueError(f"q must be bf16 [tokens, heads, {HEAD_DIM}], got {q.dtype} {tuple(shape)}")
+    if out.dtype != torch.bfloat16 or out.shape != shape or out.device != dev:
         raise ValueError("out must match q in type, shape and device")
-    if q.numel() and (q.stride(2) != 1 or out.stride(2) != 1):
+    if q.stride(2) != 1 or out.stride(2) != 1:
         raise ValueError("q and out need a contiguous last dimension")
     _int32_vector(kv_lens, "kv_lens", dev)
     batch = kv_lens.shape[0]
@@ -553,15 +582,23 @@ def _chunk_args(q, tables, rows, q_starts, kv_lens, max_kv_len, out, num_kv_head
     _check_err(err, dev)
     if max_kv_len < 0:
         raise ValueError("max_kv_len must not be negative")
-    return q.shape[0], q.shape[1], batch
+    return shape[0], shape[1], batch
 
 
-def _chunk_workspace(batch, tokens, hq, hkv, max_kv_len, device):
-    """Scratch of one packed-chunk call.  Taken from torch's allocator for
-    each call, not kept: calls on two streams, or two captured graphs, then
-    never share it."""
-    need = lib().pkv_chunk_workspace_size(batch, tokens, hq, hkv, max_kv_len)
-    return torch.empty(need, dtype=torch.uint8, device=device) if need else None
+@functools.lru_cache(maxsize=1024)
+def _chunk_workspace_size(index, batch, tokens, hq, hkv, max_kv_len) -> int:
+    return lib().pkv_chunk_workspace_size(batch, tokens, hq, hkv, max_kv_len)
+
+
+def _chunk_workspace(index, batch, tokens, hq, hkv, max_kv_len, device):
+    """Scratch of one packed-chunk call: (pointer, bytes, tensor).  Taken from
+    torch's allocator for each call, not kept: calls on two streams, or two
+    captured graphs, then never share it."""
+    need = _chunk_workspace_size(index, batch, tokens, hq, hkv, max_kv_len)
+    if not need:
+        return None, 0, None
+    ws = torch.empty(need, dtype=torch.uint8, device=device)
+    return ws.data_ptr(), need, ws
 
 
 def paged_chunk(q: torch.Tensor, k_plane: torch.Tensor, v_plane: torch.Tensor,
@@ -570,23 +607,25 @@ def paged_chunk(q: torch.Tensor, k_plane: torch.Tensor, v_plane: torch.Tensor,
                 sm_scale: float, num_kv_heads: int, err: torch.Tensor | None = None) -> None:
     """pkv_paged_chunk.  q, out: [tokens, Hq, 128] packed; q_starts int32
     [B + 1]; the pool planes are [num_slots, Hkv, 128] bf16."""
-    N, Hq, B = _chunk_args(q, tables, rows, q_starts, kv_lens, max_kv_len, out, num_kv_heads, err)
+    N, Hq, B = _chunk_args(q, tables, rows, q_starts, kv_lens, max_kv_len, out, err)
+    dev = q.device
     for name, t in (("k_plane", k_plane), ("v_plane", v_plane)):
         if (t.dtype != torch.bfloat16 or t.dim() != 3 or t.shape[1:] != (num_kv_heads, HEAD_DIM)
-                or not t.is_contiguous() or t.device != q.device):
+                or not t.is_contiguous() or t.device != dev):
             raise ValueError(f"{name} must be contiguous bf16 [slots, {num_kv_heads}, {HEAD_DIM}] on "
-                             f"{q.device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
-    if k_plane.shape != v_plane.shape:
+                             f"{dev}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    if k_plane.shape[0] != v_plane.shape[0]:
         raise ValueError("k_plane and v_plane must have the same shape")
-    with torch.cuda.device(q.device):
-        ws = _chunk_workspace(B, N, Hq, num_kv_heads, max_kv_len, q.device)
+    with _OnDevice(dev.index):
+        ws, ws_bytes, keep = _chunk_workspace(dev.index, B, N, Hq, num_kv_heads, max_kv_len, dev)
         st = lib().pkv_paged_chunk(
-            _ptr(q), q.stride(0), q.stride(1), _ptr(k_plane), _ptr(v_plane), k_plane.shape[0],
-            _ptr(tables), tables.stride(0), _ptr(rows), _ptr(q_starts), _ptr(kv_lens), max_kv_len,
-            B, N, Hq, num_kv_heads, HEAD_DIM, int(causal), sm_scale, _ptr(out), out.stride(0),
-            out.stride(1), _ptr(ws), ws.numel() if ws is not None else 0, _ptr(err),
-            _stream(q.device))
-    _check(st, "pkv_paged_chunk")
+            q.data_ptr(), q.stride(0), q.stride(1), k_plane.data_ptr(), v_plane.data_ptr(),
+            k_plane.shape[0], tables.data_ptr(), tables.stride(0), _ptr(rows), q_starts.data_ptr(),
+            kv_lens.data_ptr(), max_kv_len, B, N, Hq, num_kv_heads, HEAD_DIM, bool(causal), sm_scale,
+            out.data_ptr(), out.stride(0), out.stride(1), ws, ws_bytes, _ptr(err),
+            _stream_of(dev.index))
+    if st:
+        _check(st, "pkv_paged_chunk")
 
 
 def paged_chunk_fp8(q: torch.Tensor, pool8: torch.Tensor, tables: torch.Tensor,
@@ -595,24 +634,22 @@ def paged_chunk_fp8(q: torch.Tensor, pool8: torch.Tensor, tables: torch.Tensor,
                     err: torch.Tensor | None = None) -> None:
     """pkv_paged_chunk_fp8.  q, out: [tokens, Hq, 128] packed; pool8 uint8
     [blocks, Hkv, chunk]."""
-    Hkv = _check_pool8(pool8, q.device)
-    N, Hq, B = _chunk_args(q, tables, rows, q_starts, kv_lens, max_kv_len, out, Hkv, err)
-    with torch.cuda.device(q.device):
-        ws = _chunk_workspace(B, N, Hq, Hkv, max_kv_len, q.device)
+    N, Hq, B = _chunk_args(q, tables, rows, q_starts, kv_lens, max_kv_len, out, err)
+    dev = q.device
+    if (pool8.dtype != torch.uint8 or pool8.dim() != 3 or pool8.shape[2] != _FP8_BLOCK_BYTES
+            or not pool8.is_contiguous() or pool8.device != dev):
+        raise ValueError(f"pool8 must be contiguous uint8 [blocks, Hkv, {_FP8_BLOCK_BYTES}] on {dev}, "
+                         f"got {pool8.dtype} {tuple(pool8.shape)} on {pool8.device}")
+    Hkv = pool8.shape[1]
+    with _OnDevice(dev.index):
+        ws, ws_bytes, keep = _chunk_workspace(dev.index, B, N, Hq, Hkv, max_kv_len, dev)
         st = lib().pkv_paged_chunk_fp8(
-            _ptr(q), q.stride(0), q.stride(1), _ptr(pool8), pool8.shape[0], _ptr(tables),
-            tables.stride(0), _ptr(rows), _ptr(q_starts), _ptr(kv_lens), max_kv_len, B, N, Hq,
-            Hkv, HEAD_DIM, int(causal), sm_scale, _ptr(out), out.stride(0), out.stride(1),
-            _ptr(ws), ws.numel() if ws is not None else 0, _ptr(err), _stream(q.device))
-    _check(st, "pkv_paged_chunk_fp8")
-
-
-def _check_pool8(pool8: torch.Tensor, device: torch.device) -> int:
-    if (pool8.dtype != torch.uint8 or pool8.dim() != 3 or pool8.shape[2] != fp8_block_bytes()
-            or not pool8.is_contiguous() or pool8.device != device):
-        raise ValueError(f"pool8 must be contiguous uint8 [blocks, Hkv, {fp8_block_bytes()}] on "
-                         f"{device}, got {pool8.dtype} {tuple(pool8.shape)} on {pool8.device}")
-    return pool8.shape[1]
+            q.data_ptr(), q.stride(0), q.stride(1), pool8.data_ptr(), pool8.shape[0],
+            tables.data_ptr(), tables.stride(0), _ptr(rows), q_starts.data_ptr(), kv_lens.data_ptr(),
+            max_kv_len, B, N, Hq, Hkv, HEAD_DIM, bool(causal), sm_scale, out.data_ptr(),
+            out.stride(0), out.stride(1), ws, ws_bytes, _ptr(err), _stream_of(dev.index))
+    if st:
+        _check(st, "pkv_paged_chunk_fp8")
 
 
 # ---------------------------------------------------------------- blocks
@@ -627,7 +664,7 @@ def _page_args(pool: torch.Tensor, src: torch.Tensor, dst: torch.Tensor, err):
         if pool.shape[-3] % BLOCK_TOKENS:
             raise ValueError(f"{pool.shape[-3]} slots are not a multiple of {BLOCK_TOKENS}")
         blocks, block_bytes = pool.shape[-3] // BLOCK_TOKENS, BLOCK_TOKENS * pool.shape[-2] * HEAD_DIM * 2
-    elif pool.dtype == torch.uint8 and pool.shape[-1] == fp8_block_bytes():
+    elif pool.dtype == torch.uint8 and pool.shape[-1] == _FP8_BLOCK_BYTES:
         blocks, block_bytes = pool.shape[-3], pool.shape[-2] * pool.shape[-1]
     else:
         raise ValueError(f"not a bf16 or FP8 pool: {pool.dtype} {tuple(pool.shape)}")
@@ -643,10 +680,11 @@ def copy_blocks(pool: torch.Tensor, src: torch.Tensor, dst: torch.Tensor,
     buf or pool8, or one layer of it) receives block src[i].  dst entries are
     distinct and none is the src of another pair."""
     planes, plane, block, blocks, n = _page_args(pool, src, dst, err)
-    with torch.cuda.device(pool.device):
+    with _OnDevice(pool.device.index):
         st = lib().pkv_copy_blocks(_ptr(pool), planes, plane, block, blocks, _ptr(src), _ptr(dst), n,
-                                   _ptr(err), _stream(pool.device))
-    _check(st, "pkv_copy_blocks")
+                                   _ptr(err), _stream_of(pool.device.index))
+    if st:
+        _check(st, "pkv_copy_blocks")
 
 
 def move_blocks(pool: torch.Tensor, src: torch.Tensor, dst: torch.Tensor, tables: torch.Tensor,
@@ -655,11 +693,12 @@ def move_blocks(pool: torch.Tensor, src: torch.Tensor, dst: torch.Tensor, tables
     [rows, columns]) that name a src[i] become dst[i].  src ascends strictly."""
     planes, plane, block, blocks, n = _page_args(pool, src, dst, err)
     _check_tables(tables, pool.device)
-    with torch.cuda.device(pool.device):
+    with _OnDevice(pool.device.index):
         st = lib().pkv_move_blocks(_ptr(pool), planes, plane, block, blocks, _ptr(src), _ptr(dst), n,
                                    _ptr(tables), tables.shape[0], tables.shape[1], tables.stride(0),
-                                   _ptr(err), _stream(pool.device))
-    _check(st, "pkv_move_blocks")
+                                   _ptr(err), _stream_of(pool.device.index))
+    if st:
+        _check(st, "pkv_move_blocks")
 
 
 def default_scale(d: int = HEAD_DIM) -> float:

@@ -3,7 +3,7 @@
 
 Protocol: the roles (copies, the warp that hands out the items, three that
 write Q tiles, one issuing Q.K's and one P.V's, two slots of four softmax
-warps, FP8: four widening warps that also copy their raw bytes and write Q) run as generators under random scheduling; copies
+warps, FP8: four widening warps that also write Q) run as generators under random scheduling; copies
 land in any order, the tensor instructions and commits of one issuer run in
 order but those of the two in any, mbarriers have the hardware's phase parity.  Every read is checked for the tile it was meant for.
 
@@ -24,10 +24,10 @@ def run_kernel(items, seed, fp8, shared_ring=False, merge_wait=True, idle_wait=T
     """items: [(two, nt)].  Raises Race on a wrong read, a lost update or a hang."""
     rng = random.Random(seed)
     k_stages, v_stages = (2, 2) if fp8 else (3, 2)
-    raws = 3  # FP8: tiles copied ahead, by each widening warp for itself
+    raws = 3  # groups of four chunks
     B = {"q_full": Barrier(4 if fp8 else 3), "q_free": Barrier(1), "ml": Barrier(8), "ep": Barrier(8)}
     for i in range(RING):
-        B[f"item_full{i}"], B[f"item_empty{i}"] = Barrier(1), Barrier(14 if fp8 else 15)
+        B[f"item_full{i}"], B[f"item_empty{i}"] = Barrier(1), Barrier(15)
     for i in range(k_stages + v_stages):
         B[f"kv_full{i}"], B[f"kv_empty{i}"] = Barrier(4 if fp8 else 1), Barrier(1)
 
@@ -40,10 +40,12 @@ def run_kernel(items, seed, fp8, shared_ring=False, merge_wait=True, idle_wait=T
     B["s_free"] = Barrier(4)
     for s in range(2):
         B[f"s_full{s}"], B[f"p_full{s}"], B[f"pv_done{s}"] = Barrier(1), Barrier(4), Barrier(1)
+    for i in range(raws):
+        B[f"raw_full{i}"], B[f"raw_empty{i}"] = Barrier(1), Barrier(4)
     item_ring = [None] * RING
     Q = [None] * (4 if fp8 else 3)
     kv = [[None] * 4 for _ in range(k_stages + v_stages)]  # per widening warp; the copy engine writes all four
-    raw = [[None] * raws for _ in range(4)]
+    raw = [None] * raws
     S = [None] * 4
     P = [[None] * 4 for _ in range(2)]
     O = [set(), set()]
@@ -61,7 +63,7 @@ def run_kernel(items, seed, fp8, shared_ring=False, merge_wait=True, idle_wait=T
     def nxt(n):
         yield wait(f"item_full{n % RING}", n // RING)
         it = item_ring[n % RING]
-        need(it is not None and it[0] == n, "item overwritten")
+        need(it[0] == n, "item overwritten")
         B[f"item_empty{n % RING}"].arrive()
         return it[1]
 
@@ -99,76 +101,54 @@ def run_kernel(items, seed, fp8, shared_ring=False, merge_wait=True, idle_wait=T
             if it[1] < 0:
                 return
             for j in range(it[1]):
-                st, use = ring(which, t)
-                if use:
-                    yield wait(f"kv_empty{st}", use - 1)
-                B[f"kv_full{st}"].expect_tx(1)
-                tma.append((kv, st, [("KV"[which], n, j)] * 4, f"kv_full{st}"))
-                t += 1
-                yield None
+                if fp8:
+                    for g in range(2):
+                        st = t % raws
+                        if t >= raws:
+                            yield wait(f"raw_empty{st}", t // raws - 1)
+                        B[f"raw_full{st}"].expect_tx(1)
+                        tma.append((raw, st, (n, j, g), f"raw_full{st}"))
+                        t += 1
+                        yield None
+                else:
+                    st, use = ring(which, t)
+                    if use:
+                        yield wait(f"kv_empty{st}", use - 1)
+                    B[f"kv_full{st}"].expect_tx(1)
+                    tma.append((kv, st, [("KV"[which], n, j)] * 4, f"kv_full{st}"))
+                    t += 1
+                    yield None
             n += 1
 
     def widen_role(w):
-        n = t = n_load = ahead = slot = 0
-        look = [0, 0, 0]  # items looked at, tiles of the last one issued, slot
-        pending = []      # this warp's copies in flight, oldest first
-
-        def issue():
-            """The next tile's copy, if its item is there (never waits)."""
-            while True:
-                if look[0] and look[1] < 2 * look_nt[0]:
-                    break
-                if not B[f"item_full{look[0] % RING}"].test((look[0] // RING) & 1):
-                    return False
-                got = item_ring[look[0] % RING]
-                need(got[0] == look[0], "item looked at")
-                if got[1][1] < 0:
-                    return False
-                look_nt[0] = got[1][1]
-                look[0] += 1
-                look[1] = 0
-            tile = (look[0] - 1, look[1] // 2, "KV"[look[1] % 2])
-            pending.append((look[2], tile))
-            look[1] += 1
-            look[2] = (look[2] + 1) % raws
-            return True
-
-        look_nt = [0]
+        n = r = n_load = 0
         while True:
             it = yield from nxt(n)
             if it[1] < 0:
                 return
-            while ahead < raws and issue():
-                ahead += 1
             if it[1]:
                 yield from q_write(n, [w], n_load)
                 n_load += 1
             for j in range(it[1]):
                 for what in "KV":
-                    st, use = ring("KV".index(what), t // 2)
+                    st, use = ring("KV".index(what), r // 2)
                     if use:
                         yield wait(f"kv_empty{st}", use - 1)
-                    if ahead == 0:
-                        while ahead < raws and issue():
-                            ahead += 1
-                    need(ahead > 0, "a tile of a taken item can be copied")
-                    while len(pending) > ahead - 1:  # the oldest copies land
-                        s_, tile = pending.pop(0)
-                        raw[w][s_] = tile
-                    if rng.random() < 0.3:
-                        yield None
-                    if pending and rng.random() < 0.5:  # others land whenever they like
-                        s_, tile = pending.pop(0)
-                        raw[w][s_] = tile
-                    need(raw[w][slot] == (n, j, what), f"raw tile {raw[w][slot]} for {(n, j, what)}")
+                    for g in range(2):
+                        rs = (r + g) % raws
+                        if what == "K":
+                            yield wait(f"raw_full{rs}", (r + g) // raws)
+                        need(raw[rs] == (n, j, g), "raw chunks")
+                        if rng.random() < 0.2:
+                            yield None
+                        need(raw[rs] == (n, j, g), "raw chunks while read")
                     kv[st][w] = (what, n, j)
                     yield None
                     B[f"kv_full{st}"].arrive()
-                    slot = (slot + 1) % raws
-                    ahead -= 1
-                    t += 1
-                    while ahead < raws and issue():
-                        ahead += 1
+                    if what == "V":
+                        for g in range(2):
+                            B[f"raw_empty{(r + g) % raws}"].arrive()
+                r += 2
             n += 1
 
     def qk_role():
@@ -284,7 +264,7 @@ def run_kernel(items, seed, fp8, shared_ring=False, merge_wait=True, idle_wait=T
             O[slot].add((n, j))
 
     actors = [items_role(), qk_role(), pv_role()]
-    actors += [] if fp8 else [copy_role(0), copy_role(1)] + [q_role(w) for w in range(3)]
+    actors += [copy_role(None)] if fp8 else [copy_role(0), copy_role(1)] + [q_role(w) for w in range(3)]
     actors += [softmax(s, q) for s in range(2) for q in range(4)]
     if fp8:
         actors += [widen_role(w) for w in range(4)]
@@ -356,8 +336,8 @@ class Split:
     """struct Work and item_role of csrc/chunk.cu."""
 
     def __init__(self, new, kv, group, hkv, fp8, causal):
-        # sequences of at most 32 rows per KV head are the short kernel's
-        self.new = [t if t > 32 // group else 0 for t in new]
+        # sequences of few rows per KV head are the short kernel's
+        self.new = [t if t * group > (32 if fp8 else 16) else 0 for t in new]
         self.kv, self.hkv, self.causal = kv, hkv, causal
         self.tpt = 128 // group
         self.wfull = 1 if fp8 else 2

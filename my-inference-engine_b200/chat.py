@@ -23,6 +23,11 @@ it overlaps the prefill), and nothing is allocated or started at import --
 `KV_CACHE` is created on first use and the worker thread on the first
 message (`init()` sets both up explicitly).
 
+`Chat.fork` starts a chat that continues another one's conversation on its own
+(a regenerated or alternative reply): when its first message is admitted it
+shares the K/V blocks of the common history instead of prefilling it, if the
+chat that it came from is still resident.
+
 Not provided, being outside the attention path: weight loading from a
 checkpoint directory and the single-sequence `generate` loop of the
 reference (chat.py:39-46, :72-88).  A caller builds the model itself
@@ -214,7 +219,27 @@ def _evict(chat):
     _resident.remove(chat)
 
 
+def _share_history(chat):
+    """A forked chat's sequence, before its first message is admitted: the
+    resident history of the chat it came from.  Left to the prefill if that
+    chat was evicted, or its ids changed."""
+    parent, chat.parent = chat.parent, None
+    cache = _kv()
+    with _cache_lock:
+        if chat.seq is not None or parent.seq is None:
+            return
+        n = min(len(chat.ids), cache.length(parent.seq))
+        if cache.free_block_count() == 0:
+            n -= n % cache.block_size  # no block for a copy: whole blocks only
+        if n == 0 or parent.ids[:n] != chat.ids[:n]:
+            return
+        chat.seq = cache.fork(parent.seq, n)
+        _resident.append(chat)
+
+
 def _make_room(job):
+    if job.chat.parent is not None:
+        _share_history(job.chat)
     busy = {j.chat for j in active} | {j.chat for j, _ in _mixed} | {job.chat}
     with _cache_lock:
         while _blocks_needed(job) > _kv().free_block_count():
@@ -438,6 +463,7 @@ class Chat:
         self.pending = []      # submitted user texts not yet admitted
         self.in_progress = None  # the reply being streamed, if any
         self.listeners = []    # queues receiving the streamed reply pieces
+        self.parent = None     # the chat a fork shares its history with, until it is admitted
         self.eos_id = tokenizer.encoder["<|endoftext|>"]
 
     def release(self):
@@ -447,6 +473,18 @@ class Chat:
             if self.seq is None:
                 return
             _evict(self)
+
+    def fork(self):
+        """A new chat with this one's history so far; from here on the two
+        go on separately.  Refused while a message of this chat is queued or
+        in progress."""
+        if self.pending or self.in_progress is not None:
+            raise RuntimeError("cannot fork a chat while its message is in flight")
+        child = Chat(self.tokenizer)
+        child.ids = list(self.ids)
+        child.messages = list(self.messages)
+        child.parent = self if self.parent is None else self.parent
+        return child
 
     def submit(self, model, text):
         """Queue a message without starting the worker thread; returns the

@@ -989,7 +989,11 @@ size_t pkv_chunk_workspace_size(int32_t batch, int32_t num_tokens, int32_t num_q
 }
 
 // What both pool formats check of a packed-chunk call; fills `a` but its pool.
-static int chunk_common(pkv::ChunkLaunch& a, const void* q, int64_t q_st, int64_t q_sh,
+// The checks and the launch that both pools share.  k_pool, v_pool: the bf16
+// planes, whose tensor maps are made once every argument has passed (nullptr
+// for the FP8 pool, which is read by pointer).
+static int chunk_common(const void* k_pool, const void* v_pool, int64_t num_slots,
+                        pkv::ChunkLaunch& a, const void* q, int64_t q_st, int64_t q_sh,
                         const int32_t* block_tables, int64_t table_pitch, const int32_t* seq_rows,
                         const int32_t* q_starts, const int32_t* kv_lens, int32_t max_kv_len,
                         int32_t batch, int32_t num_tokens, int32_t num_q_heads,
@@ -1018,6 +1022,10 @@ static int chunk_common(pkv::ChunkLaunch& a, const void* q, int64_t q_st, int64_
                   workspace ? workspace_bytes : (size_t)0);
     if (!aligned16(workspace)) return fail(PKV_ERR_ALIGN, "workspace not 16-byte aligned");
   }
+  if (k_pool) {
+    if ((st = encode_blocks(&a.kmap, k_pool, num_slots, num_kv_heads))) return st;
+    if ((st = encode_blocks(&a.vmap, v_pool, num_slots, num_kv_heads))) return st;
+  }
   a.q = q; a.q_st = q_st; a.q_sh = q_sh;
   a.out = out; a.o_st = o_st; a.o_sh = o_sh;
   a.tables = block_tables; a.pitch = table_pitch; a.rows = seq_rows;
@@ -1040,11 +1048,9 @@ int pkv_paged_chunk(const void* q, int64_t q_st, int64_t q_sh, const void* k_poo
   if (st) return st;
   if ((st = check_pool(k_pool, v_pool, num_slots, block_tables, table_pitch))) return st;
   pkv::ChunkLaunch a{};
-  if ((st = encode_blocks(&a.kmap, k_pool, num_slots, num_kv_heads))) return st;
-  if ((st = encode_blocks(&a.vmap, v_pool, num_slots, num_kv_heads))) return st;
   a.num_blocks = static_cast<int32_t>(num_slots / 16);
-  return chunk_common(a, q, q_st, q_sh, block_tables, table_pitch, seq_rows, q_starts, kv_lens,
-                      max_kv_len, batch, num_tokens, num_q_heads, num_kv_heads, causal, sm_scale,
+  return chunk_common(k_pool, v_pool, num_slots, a, q, q_st, q_sh, block_tables, table_pitch,
+                      seq_rows, q_starts, kv_lens, max_kv_len, batch, num_tokens, num_q_heads, num_kv_heads, causal, sm_scale,
                       out, o_st, o_sh, workspace, workspace_bytes, err_flag, stream);
 }
 
@@ -1061,8 +1067,8 @@ int pkv_paged_chunk_fp8(const void* q, int64_t q_st, int64_t q_sh, const void* k
   pkv::ChunkLaunch a{};
   a.kv8 = kv8_pool;
   a.num_blocks = static_cast<int32_t>(num_blocks);
-  return chunk_common(a, q, q_st, q_sh, block_tables, table_pitch, seq_rows, q_starts, kv_lens,
-                      max_kv_len, batch, num_tokens, num_q_heads, num_kv_heads, causal, sm_scale,
+  return chunk_common(nullptr, nullptr, 0, a, q, q_st, q_sh, block_tables, table_pitch,
+                      seq_rows, q_starts, kv_lens, max_kv_len, batch, num_tokens, num_q_heads, num_kv_heads, causal, sm_scale,
                       out, o_st, o_sh, workspace, workspace_bytes, err_flag, stream);
 }
 

@@ -16,7 +16,9 @@ K and V may be
     the device block table (no gather copy) -- the engine's path;
   * dense [B, Hkv, S, D] tensors, as the reference's own test passes them
     (kernels/test_fa2.py:44-52).
-T == 1 runs the split-K decode kernel, T > 1 the prefill kernel.  There is no
+T == 1 runs the split-K decode kernel, T > 1 the prefill kernel.
+`packed_attention` takes a step whose rows hold different numbers of new
+tokens (KVCache.prepare_packed) in one launch, over either pool.  There is no
 SDPA/CPU fallback: non-CUDA inputs fail the reference's first assertion.
 """
 from __future__ import annotations
@@ -26,7 +28,7 @@ import math
 import torch
 
 import pagedkv
-from kv_cache import PagedKV
+from kv_cache import PackedStep, PagedKV
 
 
 def flash_attention(Q, K, V, is_causal=False, kv_lens=None, out=None):
@@ -57,6 +59,7 @@ def flash_attention(Q, K, V, is_causal=False, kv_lens=None, out=None):
     if batch_size == 0 or seq_len == 0:
         return out
     if paged:
+        assert not isinstance(K.step, PackedStep), "a packed step's tokens go through packed_attention"
         assert isinstance(V, PagedKV) and V.step is K.step, "K and V handles come from one read()"
         cache, step = K.cache, K.step
         if cache.fp8:
@@ -97,6 +100,37 @@ def flash_attention(Q, K, V, is_causal=False, kv_lens=None, out=None):
     pagedkv.dense_attention(Q, K, V, kv_lens, tgt, bool(is_causal), sm_scale)
     if tgt is not out:
         out.copy_(tgt)
+    return out
+
+
+def packed_attention(Q, K, V, is_causal=True, out=None):
+    """Attention of a packed step: Q [N, Hq, D] bf16 holds the new tokens of all
+    rows end to end, K and V are the PagedKV handles of a prepare_packed step
+    (the new tokens' K/V already appended).  Token i of a row with n new tokens
+    and kv_len keys sees keys up to kv_len - n + i (all kv_len of them unless
+    is_causal).  The FP8 pool is read in place.  Returns O [N, Hq, D]."""
+    assert isinstance(K, PagedKV) and isinstance(V, PagedKV) and V.step is K.step, \
+        "K and V handles come from one read()"
+    cache, step = K.cache, K.step
+    assert isinstance(step, PackedStep), "packed_attention needs a step from prepare_packed"
+    assert Q.is_cuda and Q.dtype == torch.bfloat16, "Expected CUDA bf16 Q"
+    N, num_heads, d = Q.shape
+    assert N == sum(step.new_lens), "Q holds the step's new tokens"
+    assert num_heads % K.shape[1] == 0, "num_heads must be a multiple of num_kv_heads (GQA)"
+    assert d == pagedkv.HEAD_DIM, "head_dim must be 128 (paged kernels)"
+    if out is None:
+        out = torch.empty((N, num_heads, d), device=Q.device, dtype=Q.dtype)
+    if N == 0:
+        return out
+    sm_scale = 1.0 / math.sqrt(d)
+    if cache.fp8:
+        pagedkv.paged_chunk_fp8(Q, cache.pool8[K.layer_idx], cache.block_tables, step.rows,
+                                step.q_starts, step.kv_lens, step.max_kv_len, out, bool(is_causal),
+                                sm_scale, cache.err_flag)
+    else:
+        pagedkv.paged_chunk(Q, K.plane, V.plane, cache.block_tables, step.rows, step.q_starts,
+                            step.kv_lens, step.max_kv_len, out, bool(is_causal), sm_scale,
+                            K.shape[1], cache.err_flag)
     return out
 
 

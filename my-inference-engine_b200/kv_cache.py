@@ -15,9 +15,20 @@ What moves to the device:
   * `prepare(seqs, T)` uploads one int32 [3, B] array (table row, start,
     kv_len per batch row) and returns a `PagedStep` in the two positions the
     reference returns slot_mapping and gather_idx.
+  * `prepare_packed(seqs, new_lens)` does the same for a step whose rows hold
+    different numbers of new tokens, laid end to end without padding.
   * `write()` scatters through the table on the GPU; `read()` returns
     zero-copy `PagedKV` handles instead of a dense gathered copy;
     `append()` fuses RoPE on q and k with the write.
+
+Beyond the reference, off until called (no decision above changes):
+  * `fork`/`fork_many` start sequences that share a prefix's full blocks with
+    the sequence they come from (a count per shared block; only the last,
+    partly filled block is copied), `truncate` takes a sequence back to an
+    earlier length, `compact` moves the live blocks to the low end of the pool.
+  * A block that another sequence holds too is never written: shared blocks are
+    full ones below a sequence's length, and `truncate` copies the block that a
+    shortened sequence would go on writing in.
 
 `buf` keeps the reference layout [NUM_LAYERS, 2, num_blocks*16, NUM_KV_HEADS,
 HEAD_DIM] (kv_cache.py:20-22), so code that inspects it (bytes per token in
@@ -53,6 +64,17 @@ class PagedStep:
     @property
     def batch(self) -> int:
         return len(self.starts_host)
+
+
+@dataclass
+class PackedStep(PagedStep):
+    """Device description of one forward step whose rows hold different numbers
+    of new tokens, packed end to end (built by prepare_packed).  T is the
+    largest number; `tokens` describes the same step as one row per token, for
+    the append kernels."""
+    new_lens: list = None
+    q_starts: torch.Tensor = None  # int32 [B + 1] first packed token of each row, then their number
+    tokens: PagedStep = None       # [N] rows of one token
 
 
 class PagedKV:
@@ -125,6 +147,7 @@ class BlockTables:
         self._row_of = {}  # seq id -> table row
         self._free_rows = list(range(self.max_seqs - 1, -1, -1))
         self._pending = {}  # (row, col) -> block id not yet on the device (last write wins)
+        self._shared = {}  # block id -> sequences holding it, for blocks held by two or more
 
     def free_block_count(self):
         return len(self._free_blocks)
@@ -147,7 +170,7 @@ class BlockTables:
 
     def free(self, seq):
         """Return every block (and the table row) this sequence holds."""
-        self._free_blocks.extend(self._block_tables.pop(seq))
+        self._release(self._block_tables.pop(seq))
         del self._lengths[seq]
         self._free_rows.append(self._row_of.pop(seq))
 
@@ -181,8 +204,116 @@ class BlockTables:
         """Give back any blocks past the one holding seq's last written token."""
         table = self._block_tables[seq]
         keep = math.ceil(self._lengths[seq] / self.block_size)
-        self._free_blocks.extend(table[keep:])
+        self._release(table[keep:])
         del table[keep:]
+
+    def _release(self, blocks):
+        """One holder of each of `blocks` less; those without another one are free."""
+        if not self._shared:
+            self._free_blocks.extend(blocks)
+            return
+        for b in blocks:
+            n = self._shared.get(b)
+            if n is None:
+                self._free_blocks.append(b)
+            elif n > 2:
+                self._shared[b] = n - 1
+            else:
+                del self._shared[b]
+
+    def _copy(self, src, dst):
+        """Copy the K/V of blocks src to blocks dst (nothing to copy on the host)."""
+
+    def _move(self, src, dst):
+        """_copy, and the device tables' entries src become dst."""
+
+    # ---- sharing, roll-back and compaction (not in the reference) ----
+    def fork(self, seq, length=None):
+        """A new sequence that holds the first `length` tokens (default: all) of seq."""
+        return self.fork_many([seq], None if length is None else [length])[0]
+
+    def fork_many(self, seqs, lengths=None):
+        """A new sequence for each of `seqs` (an id may repeat), holding its
+        first lengths[i] tokens (default: all it has).  Full blocks are shared;
+        the block that a new sequence will write next, if those tokens fill it
+        in part, is a copy.  All copies are one launch.  Raises RuntimeError, with
+        nothing changed, when rows or blocks run out."""
+        seqs = list(seqs)
+        lens = [self._lengths[s] for s in seqs] if lengths is None else list(lengths)
+        if len(lens) != len(seqs):
+            raise ValueError(f"{len(seqs)} sequences, {len(lens)} lengths")
+        for s, n in zip(seqs, lens):
+            if not 0 <= n <= self._lengths[s]:
+                raise ValueError(f"seq {s} holds {self._lengths[s]} tokens, cannot fork at {n}")
+        bs = self.block_size
+        need = sum(1 for n in lens if n % bs)
+        if need > len(self._free_blocks):
+            raise RuntimeError(f"KV cache exhausted: {len(seqs)} forks need {need} blocks, only "
+                               f"{len(self._free_blocks)} free")
+        if len(seqs) > len(self._free_rows):
+            raise RuntimeError(f"KV cache exhausted: {len(seqs)} forks, only "
+                               f"{len(self._free_rows)} sequence rows free")
+        new, src, dst = [], [], []
+        for s, n in zip(seqs, lens):
+            f = self.alloc()
+            table = self._block_tables[s][:n // bs]
+            for b in table:
+                self._shared[b] = self._shared.get(b, 1) + 1
+            if n % bs:
+                src.append(self._block_tables[s][n // bs])
+                dst.append(self._free_blocks.pop())
+                table.append(dst[-1])
+            self._block_tables[f] = table
+            self._lengths[f] = n
+            row = self._row_of[f]
+            self._pending.update(((row, c), b) for c, b in enumerate(table))
+            new.append(f)
+        if src:
+            self._copy(src, dst)
+        return new
+
+    def truncate(self, seq, length):
+        """Forget seq's tokens from position `length` on (drafted tokens that
+        were rejected, a reply to be generated anew) and give back its blocks
+        past them, reserved ones too.  A block that the next token goes into
+        and another sequence holds as well is replaced by a copy; RuntimeError,
+        with nothing changed, if there is no block for it."""
+        if not 0 <= length <= self._lengths[seq]:
+            raise ValueError(f"seq {seq} holds {self._lengths[seq]} tokens, cannot truncate to {length}")
+        bs, table = self.block_size, self._block_tables[seq]
+        keep = math.ceil(length / bs)
+        copied = length % bs != 0 and table[keep - 1] in self._shared
+        if copied and not self._free_blocks and all(b in self._shared for b in table[keep:]):
+            raise RuntimeError(f"KV cache exhausted: truncating seq {seq} to {length} needs a block")
+        self._lengths[seq] = length
+        self._release(table[keep:])
+        del table[keep:]
+        if copied:
+            old, new = table[-1], self._free_blocks.pop()
+            self._release([old])
+            table[-1] = new
+            self._pending[(self._row_of[seq], keep - 1)] = new
+            self._copy([old], [new])
+
+    def compact(self):
+        """Move the K/V of blocks in use above the number of blocks in use into
+        free blocks below it, so that the sequences hold exactly the blocks
+        0 .. n - 1; the free blocks then go out in ascending order.  Sequences,
+        lengths and shared blocks stay as they are.  Returns n."""
+        free = set(self._free_blocks)
+        n = self.num_blocks - len(free)
+        src = [b for b in range(n, self.num_blocks) if b not in free]
+        dst = sorted(b for b in free if b < n)
+        self._free_blocks = list(range(self.num_blocks - 1, n - 1, -1))
+        if not src:
+            return n
+        to = dict(zip(src, dst))
+        for table in self._block_tables.values():
+            table[:] = [to.get(b, b) for b in table]
+        self._shared = {to.get(b, b): c for b, c in self._shared.items()}
+        self._pending = {cell: to.get(b, b) for cell, b in self._pending.items()}
+        self._move(src, dst)
+        return n
 
     def advance(self, seqs, T):
         """Record that every seq in `seqs` now holds T more tokens (after all layers wrote)."""
@@ -224,6 +355,29 @@ class BlockTables:
             if start + T > len(tables[s]) * bs:  # otherwise ensure_capacity adds nothing
                 self.ensure_capacity(s, start + T)
         return starts, [self._row_of[s] for s in seqs]
+
+
+    def packed_rows(self, seqs, new_lens):
+        """Host part of prepare_packed(): check, reserve blocks, return (starts, rows)."""
+        if len(seqs) != len(new_lens):
+            raise ValueError(f"{len(seqs)} sequences, {len(new_lens)} numbers of new tokens")
+        if len(set(seqs)) != len(seqs):
+            raise ValueError("a sequence appears twice in one packed step")
+        if any(n < 0 for n in new_lens):
+            raise ValueError("negative number of new tokens")
+        starts = [self._lengths[s] for s in seqs]
+        need = sum(self.blocks_needed(s, start + n) for s, start, n in zip(seqs, starts, new_lens))
+        if need > len(self._free_blocks):
+            raise RuntimeError(f"KV cache exhausted: the packed step needs {need} more blocks, only "
+                               f"{len(self._free_blocks)} free")
+        for s, start, n in zip(seqs, starts, new_lens):
+            self.ensure_capacity(s, start + n)
+        return starts, [self._row_of[s] for s in seqs]
+
+    def advance_packed(self, seqs, new_lens):
+        """Record that seqs[i] now holds new_lens[i] more tokens."""
+        for s, n in zip(seqs, new_lens):
+            self._lengths[s] += n
 
 
 class _PinnedUpload:
@@ -317,6 +471,48 @@ class KVCache(BlockTables):
         dev = self._step_up.send(host.reshape(-1), self.device).view(3, B)
         step = PagedStep(self, T, starts, dev[0], dev[1], dev[2], max(starts) + T)
         return starts, step, step
+
+    def prepare_packed(self, seqs, new_lens):
+        """Set up one forward step that appends new_lens[i] tokens (0 and up) to
+        seqs[i], the step's tokens packed end to end in that order.  Returns
+        (starts, step): lengths before the step as plain ints and a PackedStep."""
+        new_lens = [int(n) for n in new_lens]
+        starts, rows = self.packed_rows(seqs, new_lens)
+        self.flush_tables()
+        B, N = len(seqs), sum(new_lens)
+        # rows, starts, kv_lens [B] | q_starts [B + 1] | row, position, position + 1 of each token
+        host = np.empty(4 * B + 1 + 3 * N, dtype=np.int32)
+        lens = np.array(new_lens, dtype=np.int32)
+        host[:B], host[B:2 * B] = rows, starts
+        np.add(host[B:2 * B], lens, out=host[2 * B:3 * B])
+        host[3 * B] = 0
+        np.cumsum(lens, out=host[3 * B + 1:4 * B + 1])
+        tok = host[4 * B + 1:].reshape(3, N)
+        tok[0] = np.repeat(host[:B], lens)
+        tok[1] = np.arange(N) + np.repeat(host[B:2 * B] - host[3 * B:4 * B], lens)
+        np.add(tok[1], 1, out=tok[2])
+        dev = self._step_up.send(host, self.device)
+        row = dev[:3 * B].view(3, B)
+        tok = dev[4 * B + 1:].view(3, N)
+        longest = max((a + n for a, n in zip(starts, new_lens)), default=0)
+        tokens = PagedStep(self, 1, [], tok[0], tok[1], tok[2], longest)
+        step = PackedStep(self, max(new_lens, default=0), starts, row[0], row[1], row[2], longest,
+                          new_lens=new_lens, q_starts=dev[3 * B:4 * B + 1], tokens=tokens)
+        return starts, step
+
+    def _pairs(self, src, dst):
+        return self._step_up.send(np.array([src, dst], dtype=np.int32).reshape(-1),
+                                  self.device).view(2, -1)
+
+    def _copy(self, src, dst):
+        pairs = self._pairs(src, dst)
+        pagedkv.copy_blocks(self.pool8 if self.fp8 else self.buf, pairs[0], pairs[1], self.err_flag)
+
+    def _move(self, src, dst):
+        self.flush_tables()
+        pairs = self._pairs(src, dst)
+        pagedkv.move_blocks(self.pool8 if self.fp8 else self.buf, pairs[0], pairs[1],
+                            self.block_tables, self.err_flag)
 
     @property
     def fp8(self) -> bool:

@@ -251,15 +251,19 @@ class Qwen2ForCausalLM(torch.nn.Module):
 
         segs: row segments [(first row, B, T, PagedStep, causal)] that share
         the GEMMs but append and attend separately (a mixed prefill + decode
-        step); default one segment (0, B, T, step, is_causal)."""
+        step); default one segment (0, B, T, step, is_causal).  A PackedStep's
+        segment is (0, N, T, step, causal), N its tokens: appended as N rows of
+        one token, attended in one packed launch."""
         import pagedkv
-        from kernels.fa2 import flash_attention
+        from kernels.fa2 import flash_attention, packed_attention
+        from kv_cache import PackedStep
 
         N = xs.shape[0]
         if segs is None:
             segs = [(0, B, T, step, is_causal)]
-        if (self.persistent_decode and len(segs) == 1 and segs[0][2] == 1
-                and 0 < N <= pagedkv.LAYERS_MAX_ROWS and not cache.fp8
+        packed = isinstance(segs[0][3], PackedStep)
+        if (self.persistent_decode and not packed and len(segs) == 1
+                and segs[0][2] == 1 and 0 < N <= pagedkv.LAYERS_MAX_ROWS and not cache.fp8
                 and segs[0][3].q_lens is None and len(self.layers) <= pagedkv.LAYERS_MAX_LAYERS):
             # a small decode step: every layer in one persistent launch
             st = segs[0][3]
@@ -271,6 +275,7 @@ class Qwen2ForCausalLM(torch.nn.Module):
         # the q/k/v GEMM's fused RoPE + append epilogue writes the bf16 pool;
         # an FP8 pool takes the separate quantising append
         fused_qkv = use["qkv"] and len(segs) == 1 and not cache.fp8
+        rope_step = step.tokens if packed else step
         err = cache.err_flag
         m = None
         last = len(self.layers) - 1
@@ -281,15 +286,16 @@ class Qwen2ForCausalLM(torch.nn.Module):
                 pagedkv.linear_rope_append(
                     h, at.qkv_weight, at.qkv_bias, cos, sin,
                     q_rot.view(B, T, NUM_HEADS, HEAD_DIM).transpose(1, 2), cache.buf[li, 0],
-                    cache.buf[li, 1], cache.block_tables, step.rows, step.starts, NUM_KV_HEADS,
-                    err=err, q_lens=step.q_lens)
+                    cache.buf[li, 1], cache.block_tables, rope_step.rows, rope_step.starts,
+                    NUM_KV_HEADS, err=err, q_lens=rope_step.q_lens)
             else:
                 qkv = (pagedkv.linear(h, at.qkv_weight, at.qkv_bias, err=err) if use["qkv"]
                        else F.linear(h, at.qkv_weight, at.qkv_bias))
                 qkv = qkv.view(N, NUM_HEADS + 2 * NUM_KV_HEADS, HEAD_DIM)
                 for r0, Bs, Ts, st, _ in segs:
                     part = qkv[r0:r0 + Bs * Ts].view(Bs, Ts, NUM_HEADS + 2 * NUM_KV_HEADS, HEAD_DIM)
-                    cache.append(li, st, part[:, :, :NUM_HEADS].transpose(1, 2),
+                    cache.append(li, st.tokens if packed else st,
+                                 part[:, :, :NUM_HEADS].transpose(1, 2),
                                  part[:, :, NUM_HEADS:NUM_HEADS + NUM_KV_HEADS].transpose(1, 2),
                                  part[:, :, NUM_HEADS + NUM_KV_HEADS:].transpose(1, 2), cos, sin,
                                  q_rot[r0:r0 + Bs * Ts].view(Bs, Ts, NUM_HEADS, HEAD_DIM)
@@ -297,6 +303,9 @@ class Qwen2ForCausalLM(torch.nn.Module):
             out = torch.empty(N, NUM_HEADS, HEAD_DIM, device=xs.device, dtype=xs.dtype)
             for r0, Bs, Ts, st, causal in segs:
                 k_blocks, v_blocks = cache.read(li, st)
+                if packed:
+                    packed_attention(q_rot, k_blocks, v_blocks, causal, out=out)
+                    continue
                 qs = q_rot[r0:r0 + Bs * Ts].view(Bs, Ts, NUM_HEADS, HEAD_DIM).transpose(1, 2)
                 os_ = out[r0:r0 + Bs * Ts].view(Bs, Ts, NUM_HEADS, HEAD_DIM).transpose(1, 2)
                 flash_attention(qs, k_blocks, v_blocks, causal, st.kv_lens, out=os_)
@@ -377,6 +386,38 @@ class Qwen2ForCausalLM(torch.nn.Module):
         hl = pagedkv.add_rmsnorm(m[last], xs[last], self.norm.weight, RMS_NORM_EPS)
         cache.advance([prefill_seq], T)
         cache.advance(decode_seqs, 1)
+        return hl @ self.embed_tokens.weight.T
+
+    def forward_packed(self, input_ids, cache, seqs, new_lens, all_logits=False):
+        """One forward over rows with different numbers of new tokens: input_ids
+        [N] holds new_lens[i] >= 1 tokens for each seqs[i], end to end (drafted
+        tokens to check, prompts' suffixes after a shared prefix and single
+        decode tokens may share a step).  Every projection, norm and SwiGLU runs
+        once over the N tokens and attention is one launch per layer, on either
+        pool.  Returns logits [B, vocab] of each row's last token, or with
+        all_logits [N, vocab] of every token (what a check of drafted tokens
+        compares them with; KVCache.truncate then forgets the rejected ones).
+        Needs the fused weights (fuse_weights_)."""
+        import pagedkv
+
+        if any(n < 1 for n in new_lens):
+            raise ValueError("every row of a packed forward needs a new token")
+        if input_ids.dim() != 1 or input_ids.shape[0] != sum(new_lens):
+            raise ValueError(f"input_ids must be [{sum(new_lens)}], got {tuple(input_ids.shape)}")
+        if not seqs:
+            raise ValueError("a packed forward needs a row")
+        self.fuse_weights_()
+        _, step = cache.prepare_packed(seqs, new_lens)
+        N = input_ids.shape[0]
+        x = self.embed_tokens(input_ids.to(cache.device, non_blocking=True))
+        cos, sin = self.rope_tables(cache.table_pitch * cache.block_size, x.dtype, x.device)
+        h = pagedkv.add_rmsnorm(x, None, self.layers[0].input_layernorm.weight, RMS_NORM_EPS)
+        m = self._fused_layers(h, x, N, 1, cos, sin, True, None, cache, step)
+        if not all_logits:
+            last = step.q_starts[1:].long() - 1
+            m, x = m[last], x[last]
+        hl = pagedkv.add_rmsnorm(m, x, self.norm.weight, RMS_NORM_EPS)
+        cache.advance_packed(seqs, new_lens)
         return hl @ self.embed_tokens.weight.T
 
     @staticmethod

@@ -71,10 +71,10 @@ constexpr uint32_t kColP = 128, kColO = 256;
 template <bool kFp8>
 struct Cfg {
   static constexpr int kThreads = 512;
-  static constexpr int kTiles = kFp8 ? 1 : 2;   // tiles of a full item
+  static constexpr int kTiles = 2;              // tiles of a full item
   // 32 KiB tiles; a ring each, so that no barrier is polled by two copiers of
   // whom each sees every second phase only
-  static constexpr int kKStages = kFp8 ? 2 : 3, kVStages = 2;
+  static constexpr int kKStages = kFp8 ? 2 : 3, kVStages = kFp8 ? 1 : 2;
   static constexpr int kRaw = kFp8 ? 3 : 0;  // groups of kGroup chunks in flight
   static constexpr int kOffQ = 0;
   static constexpr int kOffK = kOffQ + kTiles * kOperand;
@@ -679,7 +679,7 @@ __device__ void qk_role(const ChunkParams& p, const Ctx<kFp8>& x, uint32_t tmem)
         tc_fence_after();
         if constexpr (kFp8)
           mma_ss8<kHiKMajor, kHiKMajor, (kRegion >> 4) - 6, (kRegion >> 4) - 6, 2>(
-              tmem, sq, b, Tensor<kFp8>::kIdesc);
+              tmem, sq + t * (kOperand >> 4), b, Tensor<kFp8>::kIdesc);
         else
           mma_ss8<kHiKMajor, kHiBoxK, (kRegion >> 4) - 6, (1024 >> 4) - 6, 2>(
               tmem, sq + t * (kOperand >> 4), b, Tensor<kFp8>::kIdesc);
@@ -1406,7 +1406,7 @@ constexpr int kShortMinBlocks = 8;       // per partition: two per warp
 // each kMinStep.
 ChunkPlan plan_chunk(int32_t batch, int32_t tokens, int32_t hq, int32_t hkv, int32_t max_kv_len,
                      bool fp8) {
-  const int group = hq / hkv, tpt = kRows / group, tiles = fp8 ? 1 : 2;
+  const int group = hq / hkv, tpt = kRows / group, tiles = 2;
   const int64_t most = static_cast<int64_t>(tokens) * group;  // rows of one sequence
   ChunkPlan pl{};
   pl.short_rows = most <= kSmallRows ? kSmallRows : (fp8 ? 32 : 16);
@@ -1510,6 +1510,11 @@ cudaError_t launch_chunk(const ChunkLaunch& a, cudaStream_t stream) {
     p.part_o = p.part_lse + static_cast<int64_t>(pl.grid) * 2 * pl.part_rows;
   }
   p.short_rows = pl.short_rows;
+  cudaError_t e = cudaSuccess;
+  if (pl.grid > 0)
+    e = fp8 ? launch_chunk_t<true>(p, a.kmap, a.vmap, pl.grid, stream)
+            : launch_chunk_t<false>(p, a.kmap, a.vmap, pl.grid, stream);
+  if (e != cudaSuccess) return e;
   if (pl.short_rows > 0) {
     ShortParams q{};
     q.q = p.q;
@@ -1532,15 +1537,13 @@ cudaError_t launch_chunk(const ChunkLaunch& a, cudaStream_t stream) {
     q.most_rows = pl.short_rows;
     q.chunks = pl.chunks;
     q.min_blocks = kShortMinBlocks;
+    q.beside = pl.grid > 0;
     q.scale_log2 = a.sm_scale * 1.4426950408889634f;
     q.err = a.err;
-    const cudaError_t e = launch_chunk_short(q, a.kmap, a.vmap, a.batch, pl.parts, stream);
+    e = launch_chunk_short(q, a.kmap, a.vmap, a.batch, pl.parts, stream);
     if (e != cudaSuccess) return e;
   }
-  if (pl.grid == 0) return cudaSuccess;
-  const cudaError_t e = fp8 ? launch_chunk_t<true>(p, a.kmap, a.vmap, pl.grid, stream)
-                            : launch_chunk_t<false>(p, a.kmap, a.vmap, pl.grid, stream);
-  if (e != cudaSuccess || pl.grid < 2) return e;
+  if (pl.grid < 2) return cudaSuccess;
   return launch_k(merge_kernel, dim3(pl.grid, (pl.part_rows + 15) / 16), dim3(256), 0, stream, p);
 }
 

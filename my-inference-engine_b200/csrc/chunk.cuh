@@ -24,6 +24,7 @@ struct ShortParams {
   int32_t most_rows;   // sequences of more rows per KV head are not its
   int32_t chunks;      // of kShortRows rows, for each sequence
   int32_t min_blocks;  // a partition holds at least this many
+  int32_t beside;      // launched right behind chunk.cu's kernel, to run beside it
   float scale_log2;
   int32_t* err;
 };

@@ -460,28 +460,11 @@ __device__ __forceinline__ void short_part(const ShortParams& p, const CUtensorM
   cluster_sync();  // no CTA leaves while another reads its rows
 }
 
+// The CTA's partition of (sequence b, its chunk of rows, KV head), if it has one.
 template <bool kFp8>
-__global__ void __launch_bounds__(kWarps * 32, 2)
-    chunk_short_kernel(const ShortParams p, const __grid_constant__ CUtensorMap kmap,
-                       const __grid_constant__ CUtensorMap vmap) {
-  using C = Short<kFp8>;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
-                                             ~static_cast<uintptr_t>(1023));
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kOffBar);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int b = blockIdx.z / p.chunks, chunk = blockIdx.z - b * p.chunks, kvh = blockIdx.y;
-  pdl_trigger();
-  if (lane == 0) {
-    for (int s = 0; s < C::kStages; ++s) mbar_init(&bars[warp * C::kStages + s], 1);
-    fence_mbar_init();
-    if (warp == 0 && !kFp8) {
-      prefetch_tmap(&kmap);
-      prefetch_tmap(&vmap);
-    }
-  }
-  __syncwarp();
-  pdl_wait();
+__device__ __forceinline__ void short_unit(const ShortParams& p, const CUtensorMap* kmap,
+                                           const CUtensorMap* vmap, uint8_t* smem, uint64_t* bars,
+                                           int b, int chunk, int kvh) {
   // (a whole cluster takes the same way here: all of it is one unit)
   const int s0 = min(max(__ldg(p.q_starts + b), 0), p.tokens);
   const int s1 = min(max(__ldg(p.q_starts + b + 1), s0), p.tokens);
@@ -508,11 +491,41 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
   it.blk1 = min(nblk, it.blk0 + per);
   it.trow = p.tables + static_cast<int64_t>(p.rows ? p.rows[b] : b) * p.pitch;
   if (it.rows <= 8)
-    short_part<kFp8, 1>(p, &kmap, &vmap, smem, bars, it, kvh);
+    short_part<kFp8, 1>(p, kmap, vmap, smem, bars, it, kvh);
   else if (it.rows <= 16)
-    short_part<kFp8, 2>(p, &kmap, &vmap, smem, bars, it, kvh);
+    short_part<kFp8, 2>(p, kmap, vmap, smem, bars, it, kvh);
   else
-    short_part<kFp8, kMaxNT>(p, &kmap, &vmap, smem, bars, it, kvh);
+    short_part<kFp8, kMaxNT>(p, kmap, vmap, smem, bars, it, kvh);
+}
+
+template <bool kFp8>
+__global__ void __launch_bounds__(kWarps * 32, 2)
+    chunk_short_kernel(const ShortParams p, const __grid_constant__ CUtensorMap kmap,
+                       const __grid_constant__ CUtensorMap vmap) {
+  using C = Short<kFp8>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~static_cast<uintptr_t>(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kOffBar);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int b = blockIdx.z / p.chunks, chunk = blockIdx.z - b * p.chunks, kvh = blockIdx.y;
+  pdl_trigger();
+  if (lane == 0) {
+    for (int s = 0; s < C::kStages; ++s) mbar_init(&bars[warp * C::kStages + s], 1);
+    fence_mbar_init();
+    if (warp == 0 && !kFp8) {
+      prefetch_tmap(&kmap);
+      prefetch_tmap(&vmap);
+    }
+  }
+  __syncwarp();
+  // Beside chunk.cu's kernel (launched just before): that one has waited for
+  // the stream's earlier work before it let this one start, so the two run at
+  // the same time; waiting for it at the end keeps the stream's order for
+  // what comes after.
+  if (!p.beside) pdl_wait();
+  short_unit<kFp8>(p, &kmap, &vmap, smem, bars, b, chunk, kvh);
+  if (p.beside) pdl_wait();
 }
 
 template <bool kFp8>

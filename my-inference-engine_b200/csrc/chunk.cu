@@ -114,7 +114,7 @@ struct ChunkParams {
   int32_t part_rows;   // rows of a partial slot
   int4* desc;         // [grid]: parts, first token, tokens, KV head
   float* part_lse;    // [grid][2][part_rows]
-  float* part_o;      // [grid][2][part_rows][128]
+  float* part_o;      // [grid][2][dims / 4][part_rows][4]
   int32_t* err;
 };
 
@@ -284,8 +284,8 @@ __device__ __forceinline__ uint64_t now_ns() {
 template <int N>
 struct RingPos {
   uint32_t st = 0, ph = 0;
-  __device__ void next() {
-    if (++st == N) {
+  __device__ void next(uint32_t n = N) {
+    if (++st == n) {
       st = 0;
       ph ^= 1;
     }
@@ -334,16 +334,16 @@ struct Ctx {
   // A whole warp waits for a phase: false after kWaitNs (a role may wait for
   // a whole item, nothing waits seconds).
   __device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t phase) const {
-    if (__all_sync(0xffffffffu, suspend_on(bar, phase & 1))) return true;
-    return __all_sync(0xffffffffu, keep_waiting(bar, phase & 1));
-  }
-  __device__ bool keep_waiting(uint64_t* bar, uint32_t parity) const {
-    const uint64_t t0 = now_ns();
-    do {
-      if (suspend_on(bar, parity)) return true;
-    } while (now_ns() - t0 < kWaitNs);
-    err.raise(PKV_DEVERR_TIMEOUT);
-    return false;
+    uint64_t since = 0;
+    while (!__all_sync(0xffffffffu, suspend_on(bar, phase & 1))) {
+      const uint64_t t = now_ns();
+      if (since == 0) since = t;
+      if (t - since > kWaitNs) {
+        err.raise(PKV_DEVERR_TIMEOUT);
+        return false;
+      }
+    }
+    return true;
   }
   // Item n, read by a whole warp; false after a wait that ran out.
   __device__ bool next(int n, Item& it) const {
@@ -363,27 +363,45 @@ struct Ctx {
 // The item's rows, 16-byte chunk c of row r at chunk c ^ (r & 7) of its
 // 128-byte line (K-major, 128B swizzle).  Rows past the item's are not
 // written: they only reach their own rows of S and O.
-struct QRows {
-  int rows, per_tile;  // rows of the item and of a full tile
-  __device__ const __nv_bfloat16* src(const ChunkParams& p, const Item& it, int i) const {
-    const int r = i >> 4, tok = r / p.group, head = it.kvh * p.group + r - tok * p.group;
-    return p.q + (it.first + tok) * p.q_st + head * p.q_sh + (i & 15) * 8;
+// A thread takes one 16-byte chunk of every kThreads / 16th row; heads and
+// tokens advance without a division (one per 16 bytes made the Q tiles of an
+// item take 9k cycles, which nothing hides in its first tiles).
+template <int kThreads>
+struct QWalk {
+  const __nv_bfloat16* src;
+  int64_t step, wrap;  // elements to the next row, and from past a token's last head
+  int r, rows, head, dhead, group, per_tile, c;
+  __device__ QWalk(const ChunkParams& p, const Item& it, int tpt, int thread)
+      : r(thread >> 4), rows(it.ntok * p.group), group(p.group), per_tile(tpt * p.group), c(thread & 15) {
+    constexpr int kRowStep = kThreads / 16;
+    const int dtok = kRowStep / group, tok = r / group;
+    dhead = kRowStep - dtok * group;
+    head = r - tok * group;
+    step = dtok * p.q_st + dhead * p.q_sh;
+    wrap = p.q_st - group * p.q_sh;
+    src = p.q + static_cast<int64_t>(it.first + tok) * p.q_st + (it.kvh * group + head) * p.q_sh + c * 8;
   }
-  __device__ uint32_t dst(int i) const {
-    int r = i >> 4;
-    const int c = i & 15;
-    const uint32_t tile = r >= per_tile ? kOperand : 0;
-    if (tile) r -= per_tile;
-    return tile + (c >> 3) * kRegion + swz128(r, c & 7);
+  __device__ bool more() const { return r < rows; }
+  __device__ uint32_t dst() const {
+    const bool b = r >= per_tile;
+    return (b ? kOperand : 0) + (c >> 3) * kRegion + swz128(b ? r - per_tile : r, c & 7);
+  }
+  __device__ void next() {
+    r += kThreads / 16;
+    src += step;
+    head += dhead;
+    if (head >= group) {
+      head -= group;
+      src += wrap;
+    }
   }
 };
 
 // bf16 pool: three warps, asynchronous copies, all in flight at once.
 __device__ void load_q(const ChunkParams& p, uint8_t* tiles, const Item& it, int tpt, int thread) {
-  const QRows q{it.ntok * p.group, tpt * p.group};
-  for (int i = thread; i < q.rows * 16; i += 96)
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(tiles) + q.dst(i)),
-                 "l"(q.src(p, it, i))
+  const uint32_t base = smem_u32(tiles);
+  for (QWalk<96> q(p, it, tpt, thread); q.more(); q.next())
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(base + q.dst()), "l"(q.src)
                  : "memory");
   asm volatile("cp.async.wait_all;" ::: "memory");
 }
@@ -392,48 +410,89 @@ __device__ void load_q(const ChunkParams& p, uint8_t* tiles, const Item& it, int
 // f16's range; it is exact from 2^-10 up, below that off by at most 2^-21.)
 __device__ void load_q_f16(const ChunkParams& p, uint8_t* tiles, const Item& it, int tpt,
                            int thread) {
-  const QRows q{it.ntok * p.group, tpt * p.group};
   constexpr int kBatch = 4;
-  for (int base = thread; base < q.rows * 16; base += 128 * kBatch) {
+  QWalk<128> q(p, it, tpt, thread);
+  while (q.more()) {
     uint4 v[kBatch];
-#pragma unroll
-    for (int k = 0; k < kBatch; ++k)
-      if (base + k * 128 < q.rows * 16)
-        v[k] = *reinterpret_cast<const uint4*>(q.src(p, it, base + k * 128));
+    uint32_t at[kBatch];
 #pragma unroll
     for (int k = 0; k < kBatch; ++k) {
-      if (base + k * 128 < q.rows * 16) {
+      at[k] = q.more() ? q.dst() : ~0u;
+      if (q.more()) v[k] = *reinterpret_cast<const uint4*>(q.src);
+      q.next();
+    }
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      if (at[k] != ~0u) {
         uint32_t* w = reinterpret_cast<uint32_t*>(&v[k]);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const float2 f = __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&w[e]));
           w[e] = pack_f16(f.x * 0.0625f, f.y * 0.0625f);
         }
-        *reinterpret_cast<uint4*>(tiles + q.dst(base + k * 128)) = v[k];
+        *reinterpret_cast<uint4*>(tiles + at[k]) = v[k];
       }
     }
   }
 }
 
 // ---------------------------------------------------------------- epilogue
-// Columns [c0, c0 + 32 * N) of a row of O (already divided by its sum): bf16 to out or fp32
-// to the row's partial.
-__device__ __forceinline__ void store_cols(const float (&v)[32], __nv_bfloat16* out, float* part) {
-  if (out) {
+// A thread holds a row, and a store whose lanes lie in 32 rows takes 32 cycles
+// whatever its width, so four lanes exchange their 16-byte vectors and each
+// store then covers 64 bytes of eight rows (the epilogue of an item took 4k
+// cycles a tile, 8k of fp32, with a store per thread).
+struct OutRows {
+  __nv_bfloat16* row[4];  // the rows of this lane's group of four
+  bool live[4];
+  __device__ OutRows(__nv_bfloat16* mine, bool is_live) {
+    const int lane = threadIdx.x & 31;
+    const unsigned mask = __ballot_sync(0xffffffffu, is_live);
 #pragma unroll
-    for (int e = 0; e < 32; e += 8) {
-      uint4 pk;
-      pk.x = pack_bf16(v[e + 0], v[e + 1]);
-      pk.y = pack_bf16(v[e + 2], v[e + 3]);
-      pk.z = pack_bf16(v[e + 4], v[e + 5]);
-      pk.w = pack_bf16(v[e + 6], v[e + 7]);
-      *reinterpret_cast<uint4*>(out + e) = pk;
+    for (int j = 0; j < 4; ++j) {
+      const int from = (lane & ~3) + j;
+      row[j] = reinterpret_cast<__nv_bfloat16*>(
+          __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(mine), from));
+      live[j] = (mask >> from) & 1;
     }
-  } else {
-#pragma unroll
-    for (int e = 0; e < 32; e += 4)
-      *reinterpret_cast<float4*>(part + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
   }
+  // Columns [col, col + 32) as bf16, by a whole warp.
+  __device__ __forceinline__ void store(const float (&v)[32], int col) const {
+    const int q = threadIdx.x & 3;
+    uint32_t w[4][4];  // this row's four 16-byte vectors
+#pragma unroll
+    for (int i = 0; i < 16; ++i) w[i >> 2][i & 3] = pack_bf16(v[2 * i], v[2 * i + 1]);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {  // 4 x 4 transpose of the vectors among four lanes
+#pragma unroll
+      for (int i = 0; i < 4; i += 2) {
+        const uint32_t got = __shfl_xor_sync(0xffffffffu, (q & 1) ? w[i][e] : w[i + 1][e], 1);
+        if (q & 1)
+          w[i][e] = got;
+        else
+          w[i + 1][e] = got;
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const uint32_t got = __shfl_xor_sync(0xffffffffu, (q & 2) ? w[i][e] : w[i + 2][e], 2);
+        if (q & 2)
+          w[i][e] = got;
+        else
+          w[i + 2][e] = got;
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (live[j])
+        *reinterpret_cast<uint4*>(row[j] + col + q * 8) = make_uint4(w[j][0], w[j][1], w[j][2], w[j][3]);
+  }
+};
+
+// The same columns as fp32 to a partial, whose rows are its fast axis.
+__device__ __forceinline__ void store_part(const float (&v)[32], float* part, int part_rows, int col) {
+#pragma unroll
+  for (int e = 0; e < 32; e += 4)
+    *reinterpret_cast<float4*>(part + static_cast<int64_t>(col + e) * part_rows) =
+        make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
 }
 
 // ---------------------------------------------------------------- softmax
@@ -571,20 +630,22 @@ __device__ void softmax_role(const ChunkParams& p, const Ctx<kFp8>& x, uint32_t 
     const bool direct = it.slot < 0;
     const int prow = r + (whole ? slot * kRows : 0);
     const int64_t pslot = static_cast<int64_t>(blockIdx.x) * 2 + max(it.slot, 0);
-    __nv_bfloat16* out = direct ? p.out + (it.first + (live ? tok : 0)) * p.o_st + head * p.o_sh
-                                : nullptr;
-    float* part = direct ? nullptr : p.part_o + (pslot * p.part_rows + prow) * kHeadDim;
+    const OutRows out(p.out + (it.first + (live ? tok : 0)) * p.o_st + head * p.o_sh, live);
+    float* part = p.part_o + pslot * p.part_rows * kHeadDim + prow * 4;
     if (whole) {
       if (busy) {
         // a token without a visible key: NaN, but 0 in a partial (its weight is 0)
         const float inv = (direct || l > 0.f) ? 1.f / l : 0.f;
-#pragma unroll
+#pragma unroll 1
         for (int c = 0; c < 4; ++c) {
           float v[32];
           tmem_ld32_sync(col_o + c * 32, v);
 #pragma unroll
           for (int i = 0; i < 32; ++i) v[i] = (direct || l > 0.f) ? v[i] * inv : 0.f;
-          if (live) store_cols(v, out ? out + c * 32 : nullptr, part + c * 32);
+          if (direct)
+            out.store(v, c * 32);
+          else if (live)
+            store_part(v, part, p.part_rows, c * 32);
         }
         if (live && !direct)
           p.part_lse[pslot * p.part_rows + prow] = l > 0.f ? base + log2f(l) : -INFINITY;
@@ -607,7 +668,7 @@ __device__ void softmax_role(const ChunkParams& p, const Ctx<kFp8>& x, uint32_t 
         const float inv = (direct || sum > 0.f) ? 1.f / sum : 0.f;
         // a slot without a tile never wrote its O (t1 - t0 = 1)
         const bool has_b = it.t1 - it.t0 > 1;
-#pragma unroll
+#pragma unroll 1
         for (int c = 0; c < 2; ++c) {
           float v[32], w[32];
           const uint32_t at = lane_addr + kColO + slot * 64 + c * 32;
@@ -624,8 +685,10 @@ __device__ void softmax_role(const ChunkParams& p, const Ctx<kFp8>& x, uint32_t 
 #pragma unroll
             for (int i = 0; i < 32; ++i) v[i] = 0.f;
           }
-          if (live)
-            store_cols(v, out ? out + slot * 64 + c * 32 : nullptr, part + slot * 64 + c * 32);
+          if (direct)
+            out.store(v, slot * 64 + c * 32);
+          else if (live)
+            store_part(v, part, p.part_rows, slot * 64 + c * 32);
         }
         if (live && !direct && slot == 0)
           p.part_lse[pslot * p.part_rows + prow] = sum > 0.f ? top + log2f(sum) : -INFINITY;
@@ -673,6 +736,7 @@ __device__ void qk_role(const ChunkParams& p, const Ctx<kFp8>& x, uint32_t tmem)
     for (int j = 0; j < nt; ++j) {
       if (!x.wait_warp(&x.k_full[k.st], k.ph)) return;
       const uint32_t b = sk + k.st * (kOperand >> 4);
+#pragma unroll 1
       for (int t = 0; t <= (it.two ? 1 : 0); ++t) {
         if (n_s && !x.wait_warp(x.s_free, n_s - 1)) return;
         ++n_s;
@@ -725,6 +789,7 @@ __device__ void pv_role(const ChunkParams& p, const Ctx<kFp8>& x, uint32_t tmem)
         }
       }
       const uint32_t b = sv + v.st * (kOperand >> 4);
+#pragma unroll 1
       for (int t = 0; t <= (it.two ? 1 : 0); ++t) {
         const int slot = it.two ? t : j & 1;
         uint32_t& np = slot ? n_p1 : n_p0;
@@ -740,6 +805,7 @@ __device__ void pv_role(const ChunkParams& p, const Ctx<kFp8>& x, uint32_t tmem)
             mma_ts8<kHiBoxV, 256, 256>(d, a, b, kIdesc, more);
         } else {
           const int nb = (left + kBlockTokens - 1) / kBlockTokens;
+#pragma unroll 1
           for (int kb = 0; kb < nb; ++kb)
             mma_ts1(d, a + kb * 8,
                     b + (kFp8 ? (kb >> 2) * (kRegion >> 4) + (kb & 3) * 2 : kb * 256),
@@ -810,12 +876,11 @@ __device__ __forceinline__ void chunk_load(uint32_t dst, const void* src, uint32
 
 // bf16 pool: one warp copies the K tiles, another the V tiles: a
 // thread takes over 100 cycles per box, 16 of them a tile of both.
-template <int kStages>
 __device__ void copy_role(const ChunkParams& p, const Ctx<false>& x, const CUtensorMap* map,
-                          uint64_t* full, uint64_t* empty, uint8_t* ring) {
+                          uint64_t* full, uint64_t* empty, uint8_t* ring, uint32_t stages) {
   const int lane = threadIdx.x & 31;
   const uint64_t keep = policy_evict_last();
-  RingPos<kStages> r;
+  RingPos<0> r;
   uint32_t n_tile = 0;
   bool ok = true;
   for (int n = 0; ok; ++n) {
@@ -829,7 +894,7 @@ __device__ void copy_role(const ChunkParams& p, const Ctx<false>& x, const CUten
       const int b0 = j * kTileBlocks;
       if (j && (b0 & 31) == 0) ids.advance(b0, x.err);
       const int nb = min(kTileBlocks, ids.count - b0);
-      if (n_tile >= kStages && !x.wait_warp(&empty[r.st], r.ph ^ 1)) {
+      if (n_tile >= stages && !x.wait_warp(&empty[r.st], r.ph ^ 1)) {
         ok = false;
         break;
       }
@@ -841,16 +906,17 @@ __device__ void copy_role(const ChunkParams& p, const Ctx<false>& x, const CUten
         for (int b = 0; b < kTileBlocks; ++b)
           box_load(dst + b * 4096, map, bar, ids.at(b0 + b) * 2, it.kvh, keep);
       } else {
+#pragma unroll 1
         for (int b = 0; b < nb; ++b)
           box_load(dst + b * 4096, map, bar, ids.at(b0 + b) * 2, it.kvh, keep);
       }
-      r.next();
+      r.next(stages);
       ++n_tile;
     }
   }
   if (!ok) {  // copies still in flight get a bounded time to land before the CTA ends
-    for (uint32_t t = n_tile > kStages ? n_tile - kStages : 0; t < n_tile; ++t)
-      x.wait_warp(&full[t % kStages], t / kStages);
+    for (uint32_t t = n_tile > stages ? n_tile - stages : 0; t < n_tile; ++t)
+      x.wait_warp(&full[t % stages], t / stages);
   }
 }
 
@@ -1129,10 +1195,10 @@ __device__ void item_role(const ChunkParams& p, const Ctx<kFp8>& x, const Work& 
         const int wt = w.weight(r, i), ke = w.key_end(r, i);
         const int64_t end = s + kItemCost + static_cast<int64_t>(wt) * ke;
         const int kt = (ke + kKeys - 1) / kKeys;
-        // tiles before a boundary inside the item
+        // tiles before a boundary inside the item (128 or 256 of cost each)
         auto cut = [&](int64_t at) -> int {
           const int64_t d = at - s - kItemCost;
-          return d <= 0 ? 0 : static_cast<int>(min(static_cast<int64_t>(kt), d / (wt * kKeys)));
+          return d <= 0 ? 0 : static_cast<int>(min(static_cast<int64_t>(kt), d >> (6 + wt)));
         };
         Item it;
         it.t0 = lo <= s ? 0 : cut(lo);
@@ -1285,10 +1351,7 @@ __global__ void __launch_bounds__(Cfg<kFp8>::kThreads, 1)
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kRegsLow));
     if (warp == 0) {
-      if constexpr (kFp8)
-        copy_role(p, x);
-      else
-        copy_role<C::kKStages>(p, x, &kmap, x.k_full, x.k_empty, smem + C::kOffK);
+      if constexpr (kFp8) copy_role(p, x);
     } else if (warp == 1) {
       qk_role<kFp8>(p, x, tmem);
       // every tensor instruction has retired before TMEM is freed (after a
@@ -1309,10 +1372,15 @@ __global__ void __launch_bounds__(Cfg<kFp8>::kThreads, 1)
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kRegsAux));
     if constexpr (kFp8) {
       widen_role(p, x, w.tpt);
-    } else if (warp == 15) {  // (not on warp 0's scheduler)
-      copy_role<C::kVStages>(p, x, &vmap, x.v_full, x.v_empty, smem + C::kOffV);
-    } else {
+    } else if (warp < 15) {
       q_role(p, x, w.tpt);
+    }
+  }
+  if constexpr (!kFp8) {  // (not on one scheduler)
+    if (warp == 0 || warp == 15) {
+      const bool k = warp == 0;
+      copy_role(p, x, k ? &kmap : &vmap, k ? x.k_full : x.v_full, k ? x.k_empty : x.v_empty,
+                smem + (k ? C::kOffK : C::kOffV), k ? C::kKStages : C::kVStages);
     }
   }
   __syncwarp();
@@ -1324,52 +1392,49 @@ __global__ void __launch_bounds__(Cfg<kFp8>::kThreads, 1)
   }
 }
 
-// One warp per packed row of what was cut: o = sum 2^(lse_c - L) o_c over its
-// parts in key order, lane l holding dims 4l .. 4l+3.  at(c): part c's row.
-template <typename At>
-__device__ __forceinline__ void merge_row(const float* lse, const float* part, int parts, At at,
-                                          __nv_bfloat16* out) {
-  const int lane = threadIdx.x & 31;
-  float top = -INFINITY;
-  for (int c = lane; c < parts; c += 32) top = fmaxf(top, __ldcg(lse + at(c)));
-#pragma unroll
-  for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  const float base = top == -INFINITY ? 0.f : top;
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  float sum = 0.f;
-#pragma unroll 4
-  for (int c = 0; c < parts; ++c) {
-    const float f = ex2(__ldcg(lse + at(c)) - base);
-    const float4 v = __ldcg(reinterpret_cast<const float4*>(part + at(c) * kHeadDim) + lane);
-    sum += f;
-    acc.x += f * v.x;
-    acc.y += f * v.y;
-    acc.z += f * v.z;
-    acc.w += f * v.w;
-  }
-  const float inv = 1.f / sum;  // 0/0 -> NaN for a token that sees no key
-  uint2 pk;
-  pk.x = pack_bf16(acc.x * inv, acc.y * inv);
-  pk.y = pack_bf16(acc.z * inv, acc.w * inv);
-  *reinterpret_cast<uint2*>(out + lane * 4) = pk;
-}
-
-// Block (CTA, y): the item that chunk_kernel's CTA cut, where it has its first keys.
+// What was cut, joined in key order: o = sum 2^(lse_c - L) o_c.  Block (CTA,
+// y): the item that chunk_kernel's CTA cut, where it has its first keys; eight
+// rows at a time, warp w their dims [16 w, 16 w + 16), lane (row, four dims).
 __global__ void __launch_bounds__(256) merge_kernel(const ChunkParams p) {
   pdl_trigger();
   pdl_wait();
   const int cta = blockIdx.x;
   const int4 d = __ldcg(p.desc + cta);
   if (d.x < 2) return;
+  const int lane = threadIdx.x & 31, dims = ((threadIdx.x >> 5) * 4 + (lane >> 3)) * 4;
   const int tpt = kRows / p.group, rows = d.z * p.group;
-  for (int i = blockIdx.y * 8 + (threadIdx.x >> 5); i < rows; i += gridDim.y * 8) {
+  for (int i0 = blockIdx.y * 8; i0 < rows; i0 += gridDim.y * 8) {
+    const int i = min(i0 + (lane & 7), rows - 1);
     const int tok = i / p.group, head = d.w * p.group + i - tok * p.group;
     const int prow = (d.z > tpt && tok >= tpt) ? kRows + i - tpt * p.group : i;
-    merge_row(p.part_lse, p.part_o, d.x,
-              [&](int c) -> int64_t {
-                return ((static_cast<int64_t>(cta) + c) * 2 + (c == 0 ? 1 : 0)) * p.part_rows + prow;
-              },
-              p.out + static_cast<int64_t>(d.y + tok) * p.o_st + head * p.o_sh);
+    auto slot = [&](int c) -> int64_t {  // part c's, in rows
+      return ((static_cast<int64_t>(cta) + c) * 2 + (c == 0 ? 1 : 0)) * p.part_rows;
+    };
+    float top = -INFINITY;
+#pragma unroll 4
+    for (int c = lane >> 3; c < d.x; c += 4) top = fmaxf(top, __ldcg(p.part_lse + slot(c) + prow));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+    const float base = top == -INFINITY ? 0.f : top;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    float sum = 0.f;
+#pragma unroll 4
+    for (int c = 0; c < d.x; ++c) {
+      const float f = ex2(__ldcg(p.part_lse + slot(c) + prow) - base);
+      const float4 v = __ldcg(reinterpret_cast<const float4*>(
+          p.part_o + slot(c) * kHeadDim + static_cast<int64_t>(dims) * p.part_rows + prow * 4));
+      sum += f;
+      acc.x += f * v.x;
+      acc.y += f * v.y;
+      acc.z += f * v.z;
+      acc.w += f * v.w;
+    }
+    const float inv = 1.f / sum;  // 0/0 -> NaN for a token that sees no key
+    uint2 pk;
+    pk.x = pack_bf16(acc.x * inv, acc.y * inv);
+    pk.y = pack_bf16(acc.z * inv, acc.w * inv);
+    if (i0 + (lane & 7) < rows)
+      *reinterpret_cast<uint2*>(p.out + static_cast<int64_t>(d.y + tok) * p.o_st + head * p.o_sh + dims) = pk;
   }
 }
 

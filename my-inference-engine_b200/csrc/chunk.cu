@@ -561,8 +561,13 @@ __device__ void softmax_role(const ChunkParams& p, const Ctx<kFp8>& x, uint32_t 
         const int left = lim - j * kKeys;  // visible keys of this tile
         if (left < kKeys) {
 #pragma unroll
-          for (int i = 0; i < 128; ++i)
-            if (i >= left) s[i] = -INFINITY;
+          for (int c = 0; c < 4; ++c) {
+            const int n = left - c * 32;
+            const uint32_t seen = n <= 0 ? 0u : (n >= 32 ? ~0u : (1u << n) - 1u);
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (!(seen >> i & 1)) s[c * 32 + i] = -INFINITY;
+          }
         }
         float pm[4];
 #pragma unroll
@@ -603,7 +608,7 @@ __device__ void softmax_role(const ChunkParams& p, const Ctx<kFp8>& x, uint32_t 
         }
         l = l * alpha + ((ps[0] + ps[1]) + (ps[2] + ps[3]));
         if (!first && __any_sync(0xffffffffu, alpha != 1.f)) {
-#pragma unroll
+#pragma unroll 1
           for (int c = 0; c < 4; ++c) {
             float v[32];
             tmem_ld32_sync(col_o + c * 32, v);
@@ -901,15 +906,9 @@ __device__ void copy_role(const ChunkParams& p, const Ctx<false>& x, const CUten
       const uint32_t dst = smem_u32(ring) + r.st * kOperand, bar = smem_u32(&full[r.st]);
       if (lane == 0) mbar_arrive_expect_tx(&full[r.st], nb * 4096);
       __syncwarp();
-      if (nb == kTileBlocks) {
-#pragma unroll
-        for (int b = 0; b < kTileBlocks; ++b)
-          box_load(dst + b * 4096, map, bar, ids.at(b0 + b) * 2, it.kvh, keep);
-      } else {
-#pragma unroll 1
-        for (int b = 0; b < nb; ++b)
-          box_load(dst + b * 4096, map, bar, ids.at(b0 + b) * 2, it.kvh, keep);
-      }
+#pragma unroll 1  // (the warp has time: unrolled by 8 it costs others their instruction cache)
+      for (int b = 0; b < nb; ++b)
+        box_load(dst + b * 4096, map, bar, ids.at(b0 + b) * 2, it.kvh, keep);
       r.next(stages);
       ++n_tile;
     }

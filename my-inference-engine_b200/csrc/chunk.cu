@@ -42,6 +42,7 @@
 // of S the scales cost every softmax thread 96 loads a tile).  f16's range is
 // used up to 2^(8 + 7): base = maximum - 7, so a term keeps 11 bits down to
 // 2^-21 of the largest and is off by at most 2^-32 of it below.
+#include <limits.h>
 #include <math.h>
 
 #include <algorithm>
@@ -544,7 +545,12 @@ __device__ void softmax_role(const ChunkParams& p, const Ctx<kFp8>& x, uint32_t 
       }
       continue;
     }
-    const int lim = !live ? 0 : (p.causal ? min(it.kv, it.lim0 + tok) : it.kv);
+    // A row of no token is never masked and its maximum stays 0: whatever it
+    // holds reaches only its own P and O, and it must not send its warp
+    // through the mask or the rescale (two such rows of 128, with groups of 6,
+    // made every tile's mask run: 340 us instead of 310 for 2048 tokens on a
+    // 30k cache).
+    const int lim = !live ? INT_MAX : (p.causal ? min(it.kv, it.lim0 + tok) : it.kv);
     const bool busy = __any_sync(0xffffffffu, live);
     float m = -INFINITY, l = 0.f;
     bool first = true;
@@ -577,7 +583,7 @@ __device__ void softmax_role(const ChunkParams& p, const Ctx<kFp8>& x, uint32_t 
 #pragma unroll
           for (int u = 0; u < 4; ++u) pm[u] = fmaxf(fmaxf(pm[u], s[i + u]), s[i + u + 4]);
         float mx = fmaxf(fmaxf(pm[0], pm[1]), fmaxf(pm[2], pm[3]));
-        mx *= p.scale_log2;
+        mx = live ? mx * p.scale_log2 : 0.f;
         // the running maximum moves only by more than 2^8
         const float mn = (mx > m + kLazyLog2 || m == -INFINITY) ? mx : m;
         const float alpha = mn == m ? 1.f : ex2(m - mn);  // 0 from m = -inf

@@ -30,6 +30,9 @@
 //   4-7    softmax of slot A, 8-11 of slot B: a thread owns a tile row
 //   12-14  write the items' Q tiles to shared memory
 //   12-15  (FP8) do so as f16 of q / 16, and widen K and V to f16 tiles
+// The loops of these roles together are near what the instruction cache holds,
+// so code is kept small where it costs nothing: loops rolled, one copy of a
+// loop that two warps run (2048 tokens on a 30k cache 377 -> 340 us).
 // Two slots, each with a P and an O tile in tensor memory, share one S tile:
 // softmax warps take S into registers and free it at once, so the next Q.K
 // (the other slot's) runs under their exponentials.  An item of more than 128
@@ -61,11 +64,12 @@ constexpr int kRegion = kRows * 128;               // 128 rows x 64 elements
 constexpr int kOperand = 2 * kRegion;              // 32 KiB
 constexpr float kP8Shift = 7.f;   // FP8: P' up to 2^(8 + 7)
 // cost model, in keys of one tile: what an item costs besides its keys, and
-// the least a CTA is given
-constexpr int kItemCost = 384;
-constexpr int kMinStep = kItemCost + 4 * kKeys;
+// the least a CTA is given (384 and 896: 512 tokens without a cache 25.3 us
+// instead of 22.4, 24 ragged suffixes 150 us either way)
+constexpr int kItemCost = 512;
+constexpr int kMinStep = kItemCost + 2 * kKeys;
 constexpr int kItemRing = 3;
-constexpr int kGroup = 4;  // FP8: blocks to a copy barrier
+constexpr int kGroup = 2;  // FP8: blocks to a copy barrier
 // tensor memory columns: S, then each slot's P, then each slot's O
 constexpr uint32_t kColP = 128, kColO = 256;
 
@@ -75,14 +79,13 @@ struct Cfg {
   static constexpr int kTiles = 2;              // tiles of a full item
   // 32 KiB tiles; a ring each, so that no barrier is polled by two copiers of
   // whom each sees every second phase only
-  static constexpr int kKStages = kFp8 ? 2 : 3, kVStages = kFp8 ? 1 : 2;
+  static constexpr int kKStages = kFp8 ? 2 : 3, kVStages = 2;
   static constexpr int kRaw = kFp8 ? 3 : 0;  // groups of kGroup chunks in flight
   static constexpr int kOffQ = 0;
   static constexpr int kOffK = kOffQ + kTiles * kOperand;
   static constexpr int kOffV = kOffK + kKStages * kOperand;
   static constexpr int kOffRaw = kOffV + kVStages * kOperand;
-  static constexpr int kOffScale = kOffRaw + kRaw * kGroup * kFp8HeadBlockBytes;  // [4 warps][128] f16 scales
-  static constexpr int kOffMl = kOffScale + (kFp8 ? 4 * kKeys * 8 : 0);  // [2][128] float2
+  static constexpr int kOffMl = kOffRaw + kRaw * kGroup * kFp8HeadBlockBytes;  // [2][128] float2
   static constexpr int kOffItem = kOffMl + 2 * kRows * 8;
   static constexpr int kOffBar = kOffItem + kItemRing * 64;
   static constexpr int kBars = 2 * kItemRing + 2 + 2 * (kKStages + kVStages) + 7 + 3 + 2 * kRaw;
@@ -976,8 +979,10 @@ __device__ void copy_role(const ChunkParams& p, const Ctx<true>& x) {
 // A key's scale is two f16 terms: rounded to one it would move all of the
 // key's products, and so its score, by up to 2^-12 together, where their own
 // roundings average out.  For a value it is one more rounding among many.
-// These warps share the schedulers with the softmax, so what counts is the
-// number of instructions: the scales are rounded once per tile and warp.
+// One thread's chain of load, convert, scale and store is what bounds a group,
+// so its two blocks go through without a branch or a barrier between them and
+// every thread rounds the scales it needs (2 x 1024 tokens on a 15k cache
+// 344 -> 322 us; with a copy of the scales in shared memory 324 us).
 // K: one 16-byte group (token t, dims 16g ..) per block and thread; the lanes
 // of a quarter-warp take tokens t and t ^ 5 with four groups each, which keeps
 // the two stores (chunk 2g + h ^ t) free of bank conflicts.  V is stored by
@@ -1019,9 +1024,6 @@ __device__ void widen_role(const ChunkParams& p, const Ctx<true>& x, int tpt) {
   const uint32_t k_dst = (grp >> 2) * kRegion + tok * 128;
   const uint32_t k_lo = ((((grp & 3) * 2) ^ (tok & 7)) << 4);
   const uint32_t k_hi = ((((grp & 3) * 2 + 1) ^ (tok & 7)) << 4);
-  // this warp's copy of the tile's scales: of keys both terms, twice each,
-  // of values f16 in order
-  uint8_t* scales = x.smem + C::kOffScale + (c >> 5) * kKeys * 8;
   uint32_t key = 0, n_load = 0;  // key tiles, Q tiles so far
   RingPos<C::kRaw> g;            // the next copy group
   RingPos<C::kKStages> k;
@@ -1041,86 +1043,54 @@ __device__ void widen_role(const ChunkParams& p, const Ctx<true>& x, int tpt) {
     const int nblk = (it.key_end + kBlockTokens - 1) / kBlockTokens;
     for (int j = 0; j < nt; ++j) {
       const int b0 = (it.t0 + j) * kTileBlocks, nb = min(kTileBlocks, nblk - b0);
-      // ---- K tile
       if (key >= C::kKStages && !x.wait_warp(&x.k_empty[k.st], k.ph ^ 1)) return;
-      // block b of the tile is at raw0 (b < kGroup) or raw1 + b * chunk
-      const bool second = nb > kGroup;
-      RingPos<C::kRaw> g2 = g;
-      g2.next();
-      if (!x.wait_warp(&x.raw_full[g.st], g.ph)) return;
-      if (second && !x.wait_warp(&x.raw_full[g2.st], g2.ph)) return;
-      const uint8_t* raw0 = x.smem + C::kOffRaw + g.st * kGroup * kFp8HeadBlockBytes;
-      const uint8_t* raw1 =
-          x.smem + C::kOffRaw + g2.st * kGroup * kFp8HeadBlockBytes - kGroup * kFp8HeadBlockBytes;
-      // lane: four tokens of block lane / 4
-      const uint8_t* mine = ((lane >> 2) < kGroup ? raw0 : raw1) + (lane >> 2) * kFp8HeadBlockBytes +
-                            (lane & 3) * 16;
-      float4 vs = make_float4(0.f, 0.f, 0.f, 0.f);
-      {
-        float4 f = vs;
-        if ((lane >> 2) < nb) {
-          f = *reinterpret_cast<const float4*>(mine + kFp8KScaleOff);
-          vs = *reinterpret_cast<const float4*>(mine + kFp8VScaleOff);
-        }
-        const float v[4] = {f.x, f.y, f.z, f.w};
-        uint32_t w[8];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const __half2 s = __float2half2_rn(v[i]);
-          w[2 * i] = as_u32(s);
-          w[2 * i + 1] = as_u32(__float2half2_rn(v[i] - __low2float(s)));
-        }
-        uint4* at = reinterpret_cast<uint4*>(scales + lane * 32);
-        at[0] = make_uint4(w[0], w[1], w[2], w[3]);
-        at[1] = make_uint4(w[4], w[5], w[6], w[7]);
-        __syncwarp();
-      }
-      uint8_t* dst = x.smem + C::kOffK + k.st * kOperand + k_dst;
-#pragma unroll 4
-      for (int b = 0; b < nb; ++b) {
-        const uint4 raw = *reinterpret_cast<const uint4*>((b < kGroup ? raw0 : raw1) +
-                                                          b * kFp8HeadBlockBytes + k_src);
-        const uint2 sc = *reinterpret_cast<const uint2*>(scales + (b * kBlockTokens + tok) * 8);
-        uint4 lo, hi;
-        widen_k(raw.x, sc.x, sc.y, lo.x, hi.x);
-        widen_k(raw.y, sc.x, sc.y, lo.y, hi.y);
-        widen_k(raw.z, sc.x, sc.y, lo.z, hi.z);
-        widen_k(raw.w, sc.x, sc.y, lo.w, hi.w);
-        *reinterpret_cast<uint4*>(dst + b * 2048 + k_lo) = lo;
-        *reinterpret_cast<uint4*>(dst + b * 2048 + k_hi) = hi;
-      }
-      fence_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&x.k_full[k.st]);
-      k.next();
-      // ---- V tile
       if (key >= C::kVStages && !x.wait_warp(&x.v_empty[v.st], v.ph ^ 1)) return;
-      {
-        *reinterpret_cast<uint2*>(scales + lane * 8) =
-            make_uint2(pack_f16(vs.x, vs.y), pack_f16(vs.z, vs.w));
+      uint8_t* k_tile = x.smem + C::kOffK + k.st * kOperand + k_dst;
+      uint8_t* v_tile = x.smem + C::kOffV + v.st * kOperand + c * 128;
+      for (int first = 0; first < nb; first += kGroup) {
+        if (!x.wait_warp(&x.raw_full[g.st], g.ph)) return;
+        const uint8_t* raw = x.smem + C::kOffRaw + g.st * kGroup * kFp8HeadBlockBytes;
+#pragma unroll
+        for (int i = 0; i < kGroup; ++i) {
+          const int b = first + i;  // (past the item's last block: rows that nothing uses)
+          const uint4 kr = *reinterpret_cast<const uint4*>(raw + i * kFp8HeadBlockBytes + k_src);
+          const uint4 vr =
+              *reinterpret_cast<const uint4*>(raw + i * kFp8HeadBlockBytes + kFp8VOff + c * 16);
+          const float* fs = reinterpret_cast<const float*>(raw + i * kFp8HeadBlockBytes + kFp8KScaleOff);
+          const __half2 top = __float2half2_rn(fs[tok]);
+          const uint2 sc = make_uint2(as_u32(top), as_u32(__float2half2_rn(fs[tok] - __low2float(top))));
+          const float4* fv = reinterpret_cast<const float4*>(raw + i * kFp8HeadBlockBytes + kFp8VScaleOff);
+          const float4 f0 = fv[0], f1 = fv[1], f2 = fv[2], f3 = fv[3];
+          const uint4 sl = make_uint4(pack_f16(f0.x, f0.y), pack_f16(f0.z, f0.w), pack_f16(f1.x, f1.y),
+                                      pack_f16(f1.z, f1.w));
+          const uint4 sh = make_uint4(pack_f16(f2.x, f2.y), pack_f16(f2.z, f2.w), pack_f16(f3.x, f3.y),
+                                      pack_f16(f3.z, f3.w));
+          uint4 lo, hi;
+          widen_k(kr.x, sc.x, sc.y, lo.x, hi.x);
+          widen_k(kr.y, sc.x, sc.y, lo.y, hi.y);
+          widen_k(kr.z, sc.x, sc.y, lo.z, hi.z);
+          widen_k(kr.w, sc.x, sc.y, lo.w, hi.w);
+          *reinterpret_cast<uint4*>(k_tile + b * 2048 + k_lo) = lo;
+          *reinterpret_cast<uint4*>(k_tile + b * 2048 + k_hi) = hi;
+          widen_v(vr.x, sl.x, sh.x, lo.x, hi.x);
+          widen_v(vr.y, sl.y, sh.y, lo.y, hi.y);
+          widen_v(vr.z, sl.z, sh.z, lo.z, hi.z);
+          widen_v(vr.w, sl.w, sh.w, lo.w, hi.w);
+          uint8_t* row = v_tile + (b >> 2) * kRegion;
+          *reinterpret_cast<uint4*>(row + ((((b & 3) * 2) ^ (c & 7)) << 4)) = lo;
+          *reinterpret_cast<uint4*>(row + ((((b & 3) * 2 + 1) ^ (c & 7)) << 4)) = hi;
+        }
+        // behind the stores: every load of the chunks has returned by then,
+        // which an arrive right behind the loads would not wait for
         __syncwarp();
+        if (lane == 0) mbar_arrive(&x.raw_empty[g.st]);
+        g.next();
       }
-      dst = x.smem + C::kOffV + v.st * kOperand + c * 128;
       const int valid = it.kv - b0 * kBlockTokens;  // positions from the tile's first on
-#pragma unroll 4
-      for (int b = 0; b < nb; ++b) {
-        const uint4 raw = *reinterpret_cast<const uint4*>((b < kGroup ? raw0 : raw1) +
-                                                          b * kFp8HeadBlockBytes + kFp8VOff + c * 16);
-        const uint4 sl = *reinterpret_cast<const uint4*>(scales + b * 32);
-        const uint4 sh = *reinterpret_cast<const uint4*>(scales + b * 32 + 16);
-        uint4 lo, hi;
-        widen_v(raw.x, sl.x, sh.x, lo.x, hi.x);
-        widen_v(raw.y, sl.y, sh.y, lo.y, hi.y);
-        widen_v(raw.z, sl.z, sh.z, lo.z, hi.z);
-        widen_v(raw.w, sl.w, sh.w, lo.w, hi.w);
-        uint8_t* row = dst + (b >> 2) * kRegion;
-        *reinterpret_cast<uint4*>(row + ((((b & 3) * 2) ^ (c & 7)) << 4)) = lo;
-        *reinterpret_cast<uint4*>(row + ((((b & 3) * 2 + 1) ^ (c & 7)) << 4)) = hi;
-      }
       if (valid < nb * kBlockTokens) {
         // no positions at the end of the last block: zeros for P's zeros
         const int b = nb - 1, t = valid - b * kBlockTokens;
-        uint8_t* row = dst + (b >> 2) * kRegion;
+        uint8_t* row = v_tile + (b >> 2) * kRegion;
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
           uint4* at = reinterpret_cast<uint4*>(row + ((((b & 3) * 2 + half) ^ (c & 7)) << 4));
@@ -1135,16 +1105,12 @@ __device__ void widen_role(const ChunkParams& p, const Ctx<true>& x, int tpt) {
       fence_async_smem();
       __syncwarp();
       if (lane == 0) {
+        mbar_arrive(&x.k_full[k.st]);
         mbar_arrive(&x.v_full[v.st]);
-        // behind the stores: every load of the chunks has returned by then,
-        // which an arrive right behind the loads would not wait for
-        mbar_arrive(&x.raw_empty[g.st]);
-        if (second) mbar_arrive(&x.raw_empty[g2.st]);
       }
+      k.next();
       v.next();
       ++key;
-      g.next();
-      if (second) g.next();
     }
   }
 }
@@ -1466,9 +1432,13 @@ struct ChunkPlan {
 };
 
 // Which sequences are the short kernel's: those of at most 16 query rows per
-// KV head over the bf16 pool, 32 over FP8 (where half the bytes and twice the
-// work per byte leave chunk_kernel behind until then), and all of them in a
-// call of at most kSmallRows rows, which then is one launch.
+// KV head (up to 32 rows of bf16 the tensor cores win: 64 sequences of up to 30
+// rows 73 us there, 83 us here); 32 over FP8, where widening K and V costs
+// chunk_kernel as much for few rows as for many (96 sequences of 24 rows on 6k
+// caches: 91 us here, 127 us there), unless the call's sequences have more on
+// average, so that it runs anyway and takes the others along (24 sequences
+// of up to 60 rows on 3k caches: 30 us, with the short kernel beside it 47 us);
+// and all sequences of a call of at most kSmallRows rows, which is one launch.
 constexpr int kSmallRows = 128;
 constexpr int kShortCtas = 148 * 2;  // CTAs the short kernel is split into, if long enough
 constexpr int kShortMinBlocks = 8;       // per partition: two per warp
@@ -1479,7 +1449,8 @@ ChunkPlan plan_chunk(int32_t batch, int32_t tokens, int32_t hq, int32_t hkv, int
   const int group = hq / hkv, tpt = kRows / group, tiles = 2;
   const int64_t most = static_cast<int64_t>(tokens) * group;  // rows of one sequence
   ChunkPlan pl{};
-  pl.short_rows = most <= kSmallRows ? kSmallRows : (fp8 ? 32 : 16);
+  const bool few = static_cast<int64_t>(tokens) * group <= int64_t(32) * batch;
+  pl.short_rows = most <= kSmallRows ? kSmallRows : (fp8 && few ? 32 : 16);
   pl.chunks = most <= kSmallRows ? static_cast<int>((most + kShortRows - 1) / kShortRows) : 1;
   if (pl.short_rows < group) pl.short_rows = pl.chunks = 0;  // not one token
   if (pl.short_rows) {

@@ -24,8 +24,8 @@
 // captured call replays for other lengths.
 //
 // mma.sync runs at about a tenth of the tensor cores' rate: 32 rows of bf16
-// are bound by it (64 sequences of 5 tokens at 6 heads, 347 MB: 112 us here,
-// 71 us in chunk.cu), 16 are not.
+// are bound by it (64 sequences of up to 5 tokens at 6 heads, 347 MB: 83 us
+// here, 73 us in chunk.cu), 16 are not.
 #include <math.h>
 
 #include <atomic>

@@ -23,8 +23,8 @@ RING = 3
 def run_kernel(items, seed, fp8, shared_ring=False, merge_wait=True, idle_wait=True):
     """items: [(two, nt)].  Raises Race on a wrong read, a lost update or a hang."""
     rng = random.Random(seed)
-    k_stages, v_stages = (2, 1) if fp8 else (3, 2)
-    raws = 3  # groups of four chunks
+    k_stages, v_stages = (2, 2) if fp8 else (3, 2)
+    raws = 3  # groups of two chunks
     B = {"q_full": Barrier(4 if fp8 else 3), "q_free": Barrier(1), "ml": Barrier(8), "ep": Barrier(8)}
     for i in range(RING):
         B[f"item_full{i}"], B[f"item_empty{i}"] = Barrier(1), Barrier(15)
@@ -102,7 +102,7 @@ def run_kernel(items, seed, fp8, shared_ring=False, merge_wait=True, idle_wait=T
                 return
             for j in range(it[1]):
                 if fp8:
-                    for g in range(2):
+                    for g in range(4):
                         st = t % raws
                         if t >= raws:
                             yield wait(f"raw_empty{st}", t // raws - 1)
@@ -130,25 +130,24 @@ def run_kernel(items, seed, fp8, shared_ring=False, merge_wait=True, idle_wait=T
                 yield from q_write(n, [w], n_load)
                 n_load += 1
             for j in range(it[1]):
-                for what in "KV":
-                    st, use = ring("KV".index(what), r // 2)
+                places = [ring(i, r // 4) for i in range(2)]
+                for st, use in places:
                     if use:
                         yield wait(f"kv_empty{st}", use - 1)
-                    for g in range(2):
-                        rs = (r + g) % raws
-                        if what == "K":
-                            yield wait(f"raw_full{rs}", (r + g) // raws)
-                        need(raw[rs] == (n, j, g), "raw chunks")
-                        if rng.random() < 0.2:
-                            yield None
-                        need(raw[rs] == (n, j, g), "raw chunks while read")
-                    kv[st][w] = (what, n, j)
-                    yield None
+                for g in range(4):
+                    rs = r % raws
+                    yield wait(f"raw_full{rs}", r // raws)
+                    need(raw[rs] == (n, j, g), "raw chunks")
+                    if rng.random() < 0.2:
+                        yield None
+                    need(raw[rs] == (n, j, g), "raw chunks while read")
+                    for what, (st, _) in zip("KV", places):  # a tile is whole with its last group
+                        kv[st][w] = (what, n, j) if g == 3 else (what, n, j, g)
+                    B[f"raw_empty{rs}"].arrive()
+                    r += 1
+                yield None
+                for st, _ in places:
                     B[f"kv_full{st}"].arrive()
-                    if what == "V":
-                        for g in range(2):
-                            B[f"raw_empty{(r + g) % raws}"].arrive()
-                r += 2
             n += 1
 
     def qk_role():
@@ -329,7 +328,7 @@ def test_the_model_sees_a_ring_with_two_copiers():
 
 
 # ---------------------------------------------------------------- work split
-ITEM, STEP, KEYS = 384, 384 + 4 * 128, 128
+ITEM, STEP, KEYS = 512, 512 + 2 * 128, 128
 
 
 class Split:
@@ -337,7 +336,8 @@ class Split:
 
     def __init__(self, new, kv, group, hkv, fp8, causal):
         # sequences of few rows per KV head are the short kernel's
-        self.new = [t if t * group > (32 if fp8 else 16) else 0 for t in new]
+        short = 32 if fp8 and sum(new) * group <= 32 * len(new) else 16
+        self.new = [t if t * group > short else 0 for t in new]
         self.kv, self.hkv, self.causal = kv, hkv, causal
         self.tpt = 128 // group
         self.wfull = 2

@@ -521,7 +521,9 @@ int pkv_paged_chunk(const void* q, int64_t q_st, int64_t q_sh,
 
 /*
  * pkv_paged_chunk over the FP8 pool: blocks are read in place (no dense bf16
- * copy), K and V as e4m3 * scale.
+ * copy), K and V as e4m3 * scale.  The products are f16: keys must stay
+ * within 65504, values within 1023 and |q| below 2^20; keys are kept to 2^-12
+ * of themselves or 2^-16, values to 2^-11 or 2^-22, whichever is more.
  */
 int pkv_paged_chunk_fp8(const void* q, int64_t q_st, int64_t q_sh,
                         const void* kv8_pool, int64_t num_blocks,

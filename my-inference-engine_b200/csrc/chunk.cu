@@ -63,6 +63,7 @@ constexpr int kTileBlocks = kKeys / kBlockTokens;  // 8
 constexpr int kRegion = kRows * 128;               // 128 rows x 64 elements
 constexpr int kOperand = 2 * kRegion;              // 32 KiB
 constexpr float kP8Shift = 7.f;   // FP8: P' up to 2^(8 + 7)
+constexpr float kV8Up = 64.f;     // FP8: the value tiles hold the values times this
 // cost model, in keys of one tile: what an item costs besides its keys, and
 // the least a CTA is given (384 and 896: 512 tokens without a cache 25.3 us
 // instead of 22.4, 24 ragged suffixes 150 us either way)
@@ -649,7 +650,7 @@ __device__ void softmax_role(const ChunkParams& p, const Ctx<kFp8>& x, uint32_t 
     if (whole) {
       if (busy) {
         // a token without a visible key: NaN, but 0 in a partial (its weight is 0)
-        const float inv = (direct || l > 0.f) ? 1.f / l : 0.f;
+        const float inv = (direct || l > 0.f) ? (kFp8 ? 1.f / kV8Up : 1.f) / l : 0.f;
 #pragma unroll 1
         for (int c = 0; c < 4; ++c) {
           float v[32];
@@ -679,7 +680,7 @@ __device__ void softmax_role(const ChunkParams& p, const Ctx<kFp8>& x, uint32_t 
         const float fa = A.y > 0.f ? ex2(A.x - top) : 0.f;
         const float fb = B.y > 0.f ? ex2(B.x - top) : 0.f;
         const float sum = A.y * fa + B.y * fb;
-        const float inv = (direct || sum > 0.f) ? 1.f / sum : 0.f;
+        const float inv = (direct || sum > 0.f) ? (kFp8 ? 1.f / kV8Up : 1.f) / sum : 0.f;
         // a slot without a tile never wrote its O (t1 - t0 = 1)
         const bool has_b = it.t1 - it.t0 > 1;
 #pragma unroll 1
@@ -978,11 +979,15 @@ __device__ void copy_role(const ChunkParams& p, const Ctx<true>& x) {
 // Warps 12-15: e4m3 * scale as f16 (the chunks hold 4 bits, f16 holds 11).
 // A key's scale is two f16 terms: rounded to one it would move all of the
 // key's products, and so its score, by up to 2^-12 together, where their own
-// roundings average out.  For a value it is one more rounding among many.
+// roundings average out.  For a value it is one more rounding among many;
+// it is taken times 2^6, so that rows down to 4e-4 have a scale in f16's
+// normal range, and O is divided by that at its end (values up to 1023;
+// 2 x 1024 tokens on a 15k cache 335 us, 324 without it, 353 with scales
+// that adapt to any range).
 // One thread's chain of load, convert, scale and store is what bounds a group,
 // so its two blocks go through without a branch or a barrier between them and
-// every thread rounds the scales it needs (2 x 1024 tokens on a 15k cache
-// 344 -> 322 us; with a copy of the scales in shared memory 324 us).
+// every thread rounds the scales it needs (344 -> 322 us; with a copy of the
+// scales in shared memory 324 us).
 // K: one 16-byte group (token t, dims 16g ..) per block and thread; the lanes
 // of a quarter-warp take tokens t and t ^ 5 with four groups each, which keeps
 // the two stores (chunk 2g + h ^ t) free of bank conflicts.  V is stored by
@@ -1061,10 +1066,9 @@ __device__ void widen_role(const ChunkParams& p, const Ctx<true>& x, int tpt) {
           const uint2 sc = make_uint2(as_u32(top), as_u32(__float2half2_rn(fs[tok] - __low2float(top))));
           const float4* fv = reinterpret_cast<const float4*>(raw + i * kFp8HeadBlockBytes + kFp8VScaleOff);
           const float4 f0 = fv[0], f1 = fv[1], f2 = fv[2], f3 = fv[3];
-          const uint4 sl = make_uint4(pack_f16(f0.x, f0.y), pack_f16(f0.z, f0.w), pack_f16(f1.x, f1.y),
-                                      pack_f16(f1.z, f1.w));
-          const uint4 sh = make_uint4(pack_f16(f2.x, f2.y), pack_f16(f2.z, f2.w), pack_f16(f3.x, f3.y),
-                                      pack_f16(f3.z, f3.w));
+          auto pair = [](float x, float y) { return pack_f16(x * kV8Up, y * kV8Up); };
+          const uint4 sl = make_uint4(pair(f0.x, f0.y), pair(f0.z, f0.w), pair(f1.x, f1.y), pair(f1.z, f1.w));
+          const uint4 sh = make_uint4(pair(f2.x, f2.y), pair(f2.z, f2.w), pair(f3.x, f3.y), pair(f3.z, f3.w));
           uint4 lo, hi;
           widen_k(kr.x, sc.x, sc.y, lo.x, hi.x);
           widen_k(kr.y, sc.x, sc.y, lo.y, hi.y);

@@ -19,7 +19,10 @@
 //                                             ldmatrix.trans
 // FP8: fragments are e4m3 pairs widened to f16 in registers (exact), q / 16 as
 // f16, the key's scale applied to its scores and the value's to its
-// probabilities after the row's sum.  The warps join in shared memory, then
+// probabilities after the row's sum, relative to the largest scale so far (a
+// warp's `cap`): the product then is a f16 of up to 2^15 and is off by at most
+// 2^-32 of the largest term when it falls below f16's normal range, so that
+// thousands of small terms of a long cache keep their weight.  The warps join in shared memory, then
 // the partitions.  Every row's partitions follow from its own length, so a
 // captured call replays for other lengths.
 //
@@ -183,6 +186,7 @@ __device__ __forceinline__ void short_part(const ShortParams& p, const CUtensorM
 #pragma unroll
     for (int mt = 0; mt < 8; ++mt) o[nt][mt][0] = o[nt][mt][1] = o[nt][mt][2] = o[nt][mt][3] = 0.f;
   }
+  float cap = 0.f, unit = 0.f;  // FP8: O is kept in units of cap / 128; unit = 128 / cap
   const uint32_t sqa = smem_u32(sq);
   // ldmatrix lane roles
   const int a_row = (lane & 7) + ((lane >> 3) & 1) * 8, a_chk = lane >> 4;  // K rows
@@ -261,7 +265,7 @@ __device__ __forceinline__ void short_part(const ShortParams& p, const CUtensorM
       v0 = sc[16 + g];
       v1 = sc[24 + g];
     }
-    bool over = false;
+    bool over = kFp8 && fmaxf(v0, v1) > cap;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       s[nt][0] *= k0;
@@ -278,6 +282,19 @@ __device__ __forceinline__ void short_part(const ShortParams& p, const CUtensorM
               fmaxf(s[nt][1], s[nt][3]) > m[nt][1] + kLazyLog2;
     }
     if (__any_sync(0xffffffffu, over)) {
+      float to_unit = 1.f;  // from the old unit of O to the new one
+      if constexpr (kFp8) {
+        float top = fmaxf(v0, v1);
+#pragma unroll
+        for (int off = 4; off < 32; off <<= 1)
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+        if (top > cap) {
+          const float next = 4.f * top;  // (some room, so that scales a little larger pass)
+          to_unit = cap / next;
+          cap = next;
+          unit = 128.f / next;
+        }
+      }
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -290,13 +307,18 @@ __device__ __forceinline__ void short_part(const ShortParams& p, const CUtensorM
           const float al = ex2(m[nt][u] - (mn == -INFINITY ? 0.f : mn));
           l[nt][u] *= al;
           m[nt][u] = mn;
+          const float ao = kFp8 ? al * to_unit : al;
 #pragma unroll
           for (int mt = 0; mt < 8; ++mt) {
-            o[nt][mt][u] *= al;
-            o[nt][mt][2 + u] *= al;
+            o[nt][mt][u] *= ao;
+            o[nt][mt][2 + u] *= ao;
           }
         }
       }
+    }
+    if constexpr (kFp8) {
+      v0 *= unit;
+      v1 *= unit;
     }
     uint32_t pb[NT][2];
 #pragma unroll
@@ -373,6 +395,15 @@ __device__ __forceinline__ void short_part(const ShortParams& p, const CUtensorM
 #pragma unroll
       for (int off = 4; off < 32; off <<= 1)
         l[nt][u] += __shfl_xor_sync(0xffffffffu, l[nt][u], off);
+
+  if constexpr (kFp8) {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int mt = 0; mt < 8; ++mt)
+#pragma unroll
+        for (int u = 0; u < 4; ++u) o[nt][mt][u] *= cap * (1.f / 128.f);
+  }
 
   // ---- join the four warps (in the ring's memory)
   __syncthreads();

@@ -24,10 +24,11 @@ pytestmark = pytest.mark.gpu
 SCALE = 1.0 / math.sqrt(128)
 
 
-def make(device, new, kv, hq, hkv, fmt="bf16", seed=0, poison=True, spare_rows=0, amp=1.0):
+def make(device, new, kv, hq, hkv, fmt="bf16", seed=0, poison=True, spare_rows=0, amp=1.0, edit=None):
     """Pool, tables, packed q of rows with `new` tokens and `kv` positions.
     Everything that belongs to no position (other blocks, the tail of the last
-    block) holds NaN when `poison`."""
+    block) holds NaN when `poison`.  edit(keys, values) changes a sequence's
+    before they are stored."""
     import pagedkv
 
     g = torch.Generator(device=device).manual_seed(seed)
@@ -52,6 +53,8 @@ def make(device, new, kv, hq, hkv, fmt="bf16", seed=0, poison=True, spare_rows=0
         kk = torch.randn(n, hkv, 128, generator=g, device=device) * amp
         vv = torch.randn(n, hkv, 128, generator=g, device=device)
         vv *= torch.exp(torch.randn(n, hkv, 1, generator=g, device=device))
+        if edit is not None:
+            edit(kk, vv)
         k[slot], v[slot] = kk, vv
         dense.append(slot)
     k, v = k.to(torch.bfloat16), v.to(torch.bfloat16)
@@ -221,6 +224,25 @@ def test_no_token_at_all(cuda, fmt):
 def test_large_scores(cuda, fmt):
     """Scores of several hundred: one key takes a row, then another moves the maximum."""
     check(make(cuda, [30, 2], [900, 3000], 12, 2, fmt, seed=5, amp=60.0))
+
+
+@FMT
+@pytest.mark.parametrize("new", [[1], [5], [40], [2, 40]])
+@pytest.mark.parametrize("value", [1e-4, 1.0, 90.0])
+def test_small_terms_of_a_long_cache_keep_their_weight(cuda, fmt, new, value):
+    """One key far above the others (e^12.5) and 30000 that together weigh a
+    tenth of it: neither the small terms nor values as small as f16's least
+    normal numbers may be lost to a narrow format."""
+    def edit(kk, vv):
+        kk *= 0.02
+        kk[5] = 12.5 / SCALE / 128
+        vv.fill_(value)
+        vv[5] = -value
+
+    c = make(cuda, new, [30000] * len(new), 12, 2, fmt, seed=6, edit=edit)
+    c["q"].fill_(1.0)
+    out = check(c)
+    assert float(out.max()) > -0.95 * value  # the tail counts
 
 
 @FMT

@@ -500,6 +500,9 @@ int pkv_decode_layers(const pkv_layer_weights* layers, int32_t num_layers, const
  * capacity; shorter rows cost nothing).  A token that sees no position is a
  * NaN row, as 0/0 is everywhere in this library; a row with T_b = 0 writes
  * nothing, and out rows that belong to no sequence are left as they were.
+ * Keys and values of cached positions must be finite; what lies in a block
+ * past a sequence's last position, or in other blocks, may be anything.
+ * At most 16383 sequences and num_tokens * Hq <= 2^30.
  * workspace: >= pkv_chunk_workspace_size() bytes, 16-byte aligned, contents
  * irrelevant before and after; calls that may overlap on the GPU need one
  * each.

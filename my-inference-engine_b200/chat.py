@@ -262,11 +262,12 @@ def _admit(job):
     chat, model, text = job.chat, job.model, job.text
     cache = _kv()
     reserve_len = _reserve_len(job)
-    chat.pending.remove(text)
-    chat.messages.append(("user", text))
-    chat.ids.extend(job.new_ids)
-    chat.listeners = [job.out_queue]
-    chat.in_progress = ""
+    with _cache_lock:  # Chat.fork must not see a message half taken over
+        chat.pending.remove(text)
+        chat.messages.append(("user", text))
+        chat.ids.extend(job.new_ids)
+        chat.listeners = [job.out_queue]
+        chat.in_progress = ""
     if chat.seq is None:
         chat.seq = cache.alloc()
     prefill_ids = chat.ids[cache.length(chat.seq):]
@@ -307,8 +308,9 @@ def _finish(job):
     with _cache_lock:
         _kv().trim(chat.seq)
     _touch(chat)
-    chat.messages.append(("assistant", chat.in_progress))
-    chat.in_progress = None
+    with _cache_lock:
+        chat.messages.append(("assistant", chat.in_progress))
+        chat.in_progress = None
     for q in chat.listeners:
         q.put(None)
     chat.listeners = []
@@ -478,13 +480,14 @@ class Chat:
         """A new chat with this one's history so far; from here on the two
         go on separately.  Refused while a message of this chat is queued or
         in progress."""
-        if self.pending or self.in_progress is not None:
-            raise RuntimeError("cannot fork a chat while its message is in flight")
-        child = Chat(self.tokenizer)
-        child.ids = list(self.ids)
-        child.messages = list(self.messages)
-        child.parent = self if self.parent is None else self.parent
-        return child
+        with _cache_lock:
+            if self.pending or self.in_progress is not None:
+                raise RuntimeError("cannot fork a chat while its message is in flight")
+            child = Chat(self.tokenizer)
+            child.ids = list(self.ids)
+            child.messages = list(self.messages)
+            child.parent = self if self.parent is None else self.parent
+            return child
 
     def submit(self, model, text):
         """Queue a message without starting the worker thread; returns the

@@ -371,6 +371,10 @@ class BlockTables:
             raise RuntimeError(f"KV cache exhausted: the packed step needs {need} more blocks, only "
                                f"{len(self._free_blocks)} free")
         for s, start, n in zip(seqs, starts, new_lens):
+            if start + n > self.table_pitch * self.block_size:
+                raise RuntimeError(f"KV cache exhausted: seq {s} would hold {start + n} tokens, the "
+                                   f"device table holds {self.table_pitch} blocks per sequence")
+        for s, start, n in zip(seqs, starts, new_lens):
             self.ensure_capacity(s, start + n)
         return starts, [self._row_of[s] for s in seqs]
 

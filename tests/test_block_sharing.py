@@ -213,6 +213,12 @@ def test_a_packed_step_is_refused_as_a_whole():
     with pytest.raises(RuntimeError, match="exhausted"):
         bt.packed_rows([a, b], [40, 20])
     assert _state(bt) == state
+    wide = BlockTables(8, 16, max_blocks_per_seq=2)  # the second row outgrows its table row
+    c, d = wide.alloc(), wide.alloc()
+    before = _state(wide)
+    with pytest.raises(RuntimeError, match="device table"):
+        wide.packed_rows([c, d], [16, 33])
+    assert _state(wide) == before
     assert bt.packed_rows([a, b], [40, 16]) == ([0, 0], [bt.table_row(a), bt.table_row(b)])
 
 
@@ -333,5 +339,26 @@ def test_a_chat_with_a_message_in_flight_does_not_fork(engine):
     chat_mod._tick(block=False)
     with pytest.raises(RuntimeError, match="in flight"):
         a.fork()
+    chat_mod.run_until_idle()
+    a.fork()
+
+
+def test_a_message_is_taken_over_in_one_piece(engine):
+    """A fork on another thread waits while the worker turns a queued message
+    into history, or sees it still queued; it never copies half of it."""
+    chat_mod, install = engine
+    install(64)
+    a = chat_mod.Chat(FakeTokenizer())
+    seen = []
+
+    class Ids(list):
+        def extend(self, new):
+            seen.append(chat_mod._cache_lock.locked())
+            super().extend(new)
+
+    a.ids = Ids()
+    a.submit(FakeModel([]), "hello")
+    chat_mod._tick(block=False)
+    assert seen[0]
     chat_mod.run_until_idle()
     a.fork()

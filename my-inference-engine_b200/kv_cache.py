@@ -539,6 +539,8 @@ class KVCache(BlockTables):
     def append(self, layer_idx, step, q, k, v, rope_cos, rope_sin, q_out):
         """Fused apply_rope(q, k) + write (model.py:92-96): roped q goes to
         q_out, roped k and v into the pool.  rope_cos/sin: bf16 [positions, 128]."""
+        if k.numel() == 0:  # a packed step of idle rows
+            return
         if self.fp8:
             pagedkv.append_rope_fp8(q, k, v, rope_cos, rope_sin, q_out, self.pool8[layer_idx],
                                     self.block_tables, step.rows, step.starts, self.err_flag,

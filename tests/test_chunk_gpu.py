@@ -12,7 +12,14 @@ relatively, and ex2, the sums over keys and the running rescale add a few
 The FP8 kernel takes e4m3 * scale as f16.  A key element is off by at most
 2^-12 of itself (one rounding to 11 bits; the scale is held in two terms), so a
 score by 2^-12 S and p by twice that relatively; a value element by 2^-12 for
-its scale and 2^-12 for the product, 2^-11 A in all.
+its scale and 2^-12 for the product, 2^-11 A in all.  The kernel holds values
+times 2^6, so one of less than 2^-20 lies below f16's normal range there and is
+off by at most half its least step, 2^-25 / 2^6 = 2^-31 (weights sum to 1, so
+the result by no more).  Its products take p_j as f16 too: one that has fallen
+below f16's normal range is off by half its least step, 2^-25, of a number that
+holds the largest p as 2^7, so by 2^-32 of the largest; the short kernel rounds
+p_j times its row's scale, relative to four times the largest scale, 2^-30 of
+the largest value.  Over n keys that is at most n 2^-30 max |v|.
 """
 import math
 
@@ -134,7 +141,10 @@ def plain(c, causal=True):
             rel = 2.0 ** -8 + 2.0 ** -16 + 2 * 130 * 2.0 ** -24 * S
             if c["fmt"] == "fp8":
                 rel = rel + 2 * 2.0 ** -12 * S + 2.0 ** -11
-            tol[at + a:at + z] = 2.0 ** -8 * oo.abs() + rel * A
+            least = 0.0
+            if c["fmt"] == "fp8":
+                least = 2.0 ** -31 + n * 2.0 ** -30 * v.abs().amax((0, 2))[None, :, None]
+            tol[at + a:at + z] = 2.0 ** -8 * oo.abs() + rel * A + least
         at += t
     return o, tol
 

@@ -138,6 +138,7 @@ def test_a_run_of_sharing_attending_rolling_back_and_moving(cuda, fmt):
     r.step([a, b], [200, 37])               # two prompts
     f, g, h = r.fork([a, a, b], [200, 128, 37])
     r.step([f, a, g, h, b], [3, 1, 20, 0, 1])  # checks, a decode token, a suffix, an idle row
+    r.step([f, a], [0, 0])                  # nothing to do in a whole step
     r.truncate(f, 201)
     r.truncate(a, 64)                       # whole shared blocks dropped
     r.truncate(g, 100)                      # into a block that a held too: copied

@@ -524,9 +524,13 @@ int pkv_paged_chunk(const void* q, int64_t q_st, int64_t q_sh,
 
 /*
  * pkv_paged_chunk over the FP8 pool: blocks are read in place (no dense bf16
- * copy), K and V as e4m3 * scale.  The products are f16: keys must stay
- * within 65504, values within 1023 and |q| below 2^20; keys are kept to 2^-12
- * of themselves or 2^-16, values to 2^-11 or 2^-22, whichever is more.
+ * copy), K and V as e4m3 * scale, of any size.  The products are f16, keys and
+ * values relative to the largest scale of the sequence: a key is kept to 2^-11
+ * of itself or 2^-30 of the sequence's largest (448 times its largest scale; a
+ * row of zeros is stored with scale 1), a value to 2^-10 or 2^-30, a probability
+ * to 2^-11, or 2^-30 of the row's largest (times the largest value),
+ * whichever is more.  q is taken as f16 of q / 16, as pkv_paged_decode_fp8 does:
+ * |q| below 2^20, elements below 2^-13 off by up to 2^-21.
  */
 int pkv_paged_chunk_fp8(const void* q, int64_t q_st, int64_t q_sh,
                         const void* kv8_pool, int64_t num_blocks,

@@ -41,10 +41,12 @@
 //
 // P, as 16-bit pairs, is the A operand from tensor memory: bf16, and f16 over
 // the FP8 pool, whose e4m3 keys and values are widened to f16 with their scale
-// applied (a score or probability then needs no scale of its own; as columns
-// of S the scales cost every softmax thread 96 loads a tile).  f16's range is
+// applied, relative to a power of two for the tile (a score or probability then
+// needs no scale of its own; as columns of S the scales cost every softmax
+// thread 96 loads a tile).  f16's range is
 // used up to 2^(8 + 7): base = maximum - 7, so a term keeps 11 bits down to
 // 2^-21 of the largest and is off by at most 2^-32 of it below.
+#include <float.h>
 #include <limits.h>
 #include <math.h>
 
@@ -63,7 +65,6 @@ constexpr int kTileBlocks = kKeys / kBlockTokens;  // 8
 constexpr int kRegion = kRows * 128;               // 128 rows x 64 elements
 constexpr int kOperand = 2 * kRegion;              // 32 KiB
 constexpr float kP8Shift = 7.f;   // FP8: P' up to 2^(8 + 7)
-constexpr float kV8Up = 64.f;     // FP8: the value tiles hold the values times this
 // cost model, in keys of one tile: what an item costs besides its keys, and
 // the least a CTA is given (384 and 896: 512 tokens without a cache 25.3 us
 // instead of 22.4, 24 ragged suffixes 150 us either way)
@@ -71,6 +72,7 @@ constexpr int kItemCost = 512;
 constexpr int kMinStep = kItemCost + 2 * kKeys;
 constexpr int kItemRing = 3;
 constexpr int kGroup = 2;  // FP8: blocks to a copy barrier
+constexpr int kUnitRing = 4;  // FP8: tiles whose units are published (3 would do, see widen_role)
 // tensor memory columns: S, then each slot's P, then each slot's O
 constexpr uint32_t kColP = 128, kColO = 256;
 
@@ -88,7 +90,9 @@ struct Cfg {
   static constexpr int kOffRaw = kOffV + kVStages * kOperand;
   static constexpr int kOffMl = kOffRaw + kRaw * kGroup * kFp8HeadBlockBytes;  // [2][128] float2
   static constexpr int kOffItem = kOffMl + 2 * kRows * 8;
-  static constexpr int kOffBar = kOffItem + kItemRing * 64;
+  // FP8: the tiles' units, float2 (key, value), and each slot's at an item's end
+  static constexpr int kOffUnit = kOffItem + kItemRing * 64;
+  static constexpr int kOffBar = kOffUnit + (kFp8 ? kUnitRing * 8 + 2 * 4 : 0);
   static constexpr int kBars = 2 * kItemRing + 2 + 2 * (kKStages + kVStages) + 7 + 3 + 2 * kRaw;
   static constexpr int kOffScan = kOffBar + kBars * 8 + 16;  // 16 warp sums, base, row
   static constexpr int kSmem = kOffScan + 18 * 8;
@@ -336,6 +340,12 @@ struct Ctx {
   __device__ Item* item(int n) const {
     return reinterpret_cast<Item*>(smem + C::kOffItem + (n % kItemRing) * 64);
   }
+  __device__ float2* unit(uint32_t key_tile) const {
+    return reinterpret_cast<float2*>(smem + C::kOffUnit) + key_tile % kUnitRing;
+  }
+  __device__ float* slot_unit(int slot) const {
+    return reinterpret_cast<float*>(smem + C::kOffUnit + kUnitRing * 8) + slot;
+  }
   // A whole warp waits for a phase: false after kWaitNs (a role may wait for
   // a whole item, nothing waits seconds).
   __device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t phase) const {
@@ -521,6 +531,11 @@ __device__ __forceinline__ void mul2(float& x0, float& x1, float a) {
       : "f"(a));
 }
 
+// a / b of two powers of two.
+__device__ __forceinline__ float exp2i_ratio(float a, float b) {
+  return __int_as_float(max(__float_as_int(a) - __float_as_int(b) + (127 << 23), 0));
+}
+
 template <bool kFp8>
 __device__ void softmax_role(const ChunkParams& p, const Ctx<kFp8>& x, uint32_t tmem, int slot,
                              int tpt) {
@@ -533,6 +548,7 @@ __device__ void softmax_role(const ChunkParams& p, const Ctx<kFp8>& x, uint32_t 
   const int rtok = r / p.group, rhead = r - rtok * p.group;
   float2* ml = reinterpret_cast<float2*>(x.smem + C::kOffMl);
   uint32_t n_tile = 0, n_ml = 0;  // tiles of this slot, joins of the two slots so far
+  uint32_t n_key = 0;             // key tiles of the items so far
   for (int n = 0;; ++n) {
     Item it;
     if (!x.next(n, it) || it.t1 < 0) return;
@@ -557,6 +573,7 @@ __device__ void softmax_role(const ChunkParams& p, const Ctx<kFp8>& x, uint32_t 
     const int lim = !live ? INT_MAX : (p.causal ? min(it.kv, it.lim0 + tok) : it.kv);
     const bool busy = __any_sync(0xffffffffu, live);
     float m = -INFINITY, l = 0.f;
+    float unit = 1.f;  // O is kept in this unit (FP8: the last tile's value unit)
     bool first = true;
     for (int j = it.t0 + (whole ? 0 : slot); j < it.t1; j += whole ? 1 : 2) {
       if (!x.wait_warp(&x.s_full[slot], n_tile)) return;
@@ -565,6 +582,16 @@ __device__ void softmax_role(const ChunkParams& p, const Ctx<kFp8>& x, uint32_t 
         tc_fence_after();
         float s[128];
         tmem_ld32x4_sync(lane_addr, s);
+        // FP8: S and this tile's part of O are in the tile's units
+        float scale = p.scale_log2, to_unit = 1.f;
+        if constexpr (kFp8) {
+          float2 u = *x.unit(n_key + (j - it.t0));
+          u.x = __shfl_sync(0xffffffffu, u.x, 0);  // (loaded before the arrival below)
+          scale = fmaxf(scale * u.x, FLT_MIN);     // (0 * -inf is no mask)
+          // powers of two, never falling within an item
+          if (!first && u.y != unit) to_unit = exp2i_ratio(unit, u.y);
+          unit = u.y;
+        }
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(x.s_free);
@@ -587,10 +614,11 @@ __device__ void softmax_role(const ChunkParams& p, const Ctx<kFp8>& x, uint32_t 
 #pragma unroll
           for (int u = 0; u < 4; ++u) pm[u] = fmaxf(fmaxf(pm[u], s[i + u]), s[i + u + 4]);
         float mx = fmaxf(fmaxf(pm[0], pm[1]), fmaxf(pm[2], pm[3]));
-        mx = live ? mx * p.scale_log2 : 0.f;
+        mx = live ? mx * scale : 0.f;
         // the running maximum moves only by more than 2^8
         const float mn = (mx > m + kLazyLog2 || m == -INFINITY) ? mx : m;
         const float alpha = mn == m ? 1.f : ex2(m - mn);  // 0 from m = -inf
+        const float alpha_o = kFp8 ? alpha * to_unit : alpha;
         const float base = mn == -INFINITY ? 0.f : (kFp8 ? mn - kP8Shift : mn);
         m = mn;
         float ps[4] = {0.f, 0.f, 0.f, 0.f};
@@ -601,8 +629,8 @@ __device__ void softmax_role(const ChunkParams& p, const Ctx<kFp8>& x, uint32_t 
 #pragma unroll
           for (int i = 0; i < 32; i += 4) {
             float* e = s + c * 32 + i;
-            fma2(e[0], e[1], p.scale_log2, p.scale_log2, -base, -base);
-            fma2(e[2], e[3], p.scale_log2, p.scale_log2, -base, -base);
+            fma2(e[0], e[1], scale, scale, -base, -base);
+            fma2(e[2], e[3], scale, scale, -base, -base);
 #pragma unroll
             for (int u = 0; u < 4; ++u) e[u] = ex2(e[u]);
             add2(ps[0], ps[1], e[0], e[1]);
@@ -617,13 +645,13 @@ __device__ void softmax_role(const ChunkParams& p, const Ctx<kFp8>& x, uint32_t 
           tmem_st16u(col_p + c * 16, pk);
         }
         l = l * alpha + ((ps[0] + ps[1]) + (ps[2] + ps[3]));
-        if (!first && __any_sync(0xffffffffu, alpha != 1.f)) {
+        if (!first && __any_sync(0xffffffffu, alpha_o != 1.f)) {
 #pragma unroll 1
           for (int c = 0; c < 4; ++c) {
             float v[32];
             tmem_ld32_sync(col_o + c * 32, v);
 #pragma unroll
-            for (int i = 0; i < 32; i += 2) mul2(v[i], v[i + 1], alpha);
+            for (int i = 0; i < 32; i += 2) mul2(v[i], v[i + 1], alpha_o);
             tmem_st32(col_o + c * 32, v);
           }
         }
@@ -650,7 +678,7 @@ __device__ void softmax_role(const ChunkParams& p, const Ctx<kFp8>& x, uint32_t 
     if (whole) {
       if (busy) {
         // a token without a visible key: NaN, but 0 in a partial (its weight is 0)
-        const float inv = (direct || l > 0.f) ? (kFp8 ? 1.f / kV8Up : 1.f) / l : 0.f;
+        const float inv = (direct || l > 0.f) ? unit / l : 0.f;
 #pragma unroll 1
         for (int c = 0; c < 4; ++c) {
           float v[32];
@@ -669,6 +697,7 @@ __device__ void softmax_role(const ChunkParams& p, const Ctx<kFp8>& x, uint32_t 
       // the slots' halves of the keys: exchange (base, l), then slot s
       // finishes columns [64 s, 64 s + 64) of both O tiles
       ml[slot * kRows + r] = make_float2(m == -INFINITY ? -INFINITY : base, l);
+      if (kFp8 && busy && lane == 0) *x.slot_unit(slot) = unit;
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(x.ml_bar);
@@ -677,10 +706,14 @@ __device__ void softmax_role(const ChunkParams& p, const Ctx<kFp8>& x, uint32_t 
       if (busy) {
         const float2 A = ml[r], B = ml[kRows + r];
         const float top = fmaxf(A.x, B.x);
-        const float fa = A.y > 0.f ? ex2(A.x - top) : 0.f;
-        const float fb = B.y > 0.f ? ex2(B.x - top) : 0.f;
+        float fa = A.y > 0.f ? ex2(A.x - top) : 0.f;
+        float fb = B.y > 0.f ? ex2(B.x - top) : 0.f;
         const float sum = A.y * fa + B.y * fb;
-        const float inv = (direct || sum > 0.f) ? (kFp8 ? 1.f / kV8Up : 1.f) / sum : 0.f;
+        const float inv = (direct || sum > 0.f) ? 1.f / sum : 0.f;
+        if constexpr (kFp8) {
+          fa *= *x.slot_unit(0);
+          fb *= *x.slot_unit(1);
+        }
         // a slot without a tile never wrote its O (t1 - t0 = 1)
         const bool has_b = it.t1 - it.t0 > 1;
 #pragma unroll 1
@@ -715,6 +748,7 @@ __device__ void softmax_role(const ChunkParams& p, const Ctx<kFp8>& x, uint32_t 
       if (!x.wait_warp(x.ep_bar, n_ml)) return;
       ++n_ml;
     }
+    n_key += it.t1 - it.t0;
     tc_fence_before();
   }
 }
@@ -977,13 +1011,21 @@ __device__ void copy_role(const ChunkParams& p, const Ctx<true>& x) {
 
 // ---------------------------------------------------------------- FP8 widening
 // Warps 12-15: e4m3 * scale as f16 (the chunks hold 4 bits, f16 holds 11).
+// f16 spans 30 powers of two and fp32 scales many more, so a tile holds its
+// keys, and its values, in a unit, a power of two: unit = cap / 128, where the
+// cap lies above every scale of the item so far (128 * 448 is within f16) and
+// is raised when a group brings one that is not below it; what the tile holds
+// by then is brought down to the new unit.  (2 x 1024 tokens on a 15k cache 367 us;
+// with a fixed unit, which loses values past 1023 and keys past 65504, 335 us.)  The softmax folds the key unit into its scale, keeps O in the value
+// unit of its last tile (units never fall within an item) and multiplies by it
+// at the end.  What is much smaller than the largest scale so far is off by
+// f16's least steps, at most 2^-30 of the largest key or value.  A tile's units
+// go through a ring: entry n is written again for tile n + kUnitRing, after
+// Q.K(n + kUnitRing - 2) has freed its K buffer, which was issued after all of
+// S(n + kUnitRing - 3) had been taken, and the units are read before that.
 // A key's scale is two f16 terms: rounded to one it would move all of the
-// key's products, and so its score, by up to 2^-12 together, where their own
-// roundings average out.  For a value it is one more rounding among many;
-// it is taken times 2^6, so that rows down to 4e-4 have a scale in f16's
-// normal range, and O is divided by that at its end (values up to 1023;
-// 2 x 1024 tokens on a 15k cache 335 us, 324 without it, 353 with scales
-// that adapt to any range).
+// key's products, and so its score, by up to 2^-11 together, where their own
+// roundings average out.  For a value it is one more rounding among many.
 // One thread's chain of load, convert, scale and store is what bounds a group,
 // so its two blocks go through without a branch or a barrier between them and
 // every thread rounds the scales it needs (344 -> 322 us; with a copy of the
@@ -1012,6 +1054,35 @@ __device__ __forceinline__ void widen_v(uint32_t four, uint32_t s_lo, uint32_t s
   e4m3x4_to_f16x2x2(four, a, b);
   lo = as_u32(__hmul2(as_half2(a), as_half2(s_lo)));
   hi = as_u32(__hmul2(as_half2(b), as_half2(s_hi)));
+}
+
+// The unit of one tile ring's keys or values: the cap's biased exponent.
+struct Unit {
+  static constexpr int kLeast = 27;  // 2^-100: scales far below it count as 0
+  int exp;
+  float up;  // 128 / cap
+  __device__ Unit() {
+    exp = kLeast;
+    up = __int_as_float((261 - kLeast) << 23);
+  }
+  // The cap above `scale` (a positive float's bits); its former unit over the new one.
+  __device__ __forceinline__ __half2 raise(uint32_t scale) {
+    const int to = min(max(static_cast<int>(scale >> 23) + 1, exp), 250);
+    const int by = to - exp;
+    exp = to;
+    up = __int_as_float((261 - to) << 23);
+    return __float2half2_rn(by < 100 ? __int_as_float((127 - by) << 23) : 0.f);
+  }
+  __device__ __forceinline__ bool holds(uint32_t scale) const { return scale < static_cast<uint32_t>(exp) << 23; }
+  __device__ __forceinline__ float value() const { return __int_as_float((exp - 7) << 23); }
+};
+__device__ __forceinline__ void scale8(uint8_t* at, __half2 by) {
+  uint4 w = *reinterpret_cast<uint4*>(at);
+  w.x = as_u32(__hmul2(as_half2(w.x), by));
+  w.y = as_u32(__hmul2(as_half2(w.y), by));
+  w.z = as_u32(__hmul2(as_half2(w.z), by));
+  w.w = as_u32(__hmul2(as_half2(w.w), by));
+  *reinterpret_cast<uint4*>(at) = w;
 }
 
 // The 16-bit halves of a pair (tokens t, t + 1) that lie before `valid`.
@@ -1046,6 +1117,8 @@ __device__ void widen_role(const ChunkParams& p, const Ctx<true>& x, int tpt) {
       if (lane == 0) mbar_arrive(x.q_full);
     }
     const int nblk = (it.key_end + kBlockTokens - 1) / kBlockTokens;
+    const int positions = min(it.kv, nblk * kBlockTokens);
+    Unit ku, vu;  // the same in every thread
     for (int j = 0; j < nt; ++j) {
       const int b0 = (it.t0 + j) * kTileBlocks, nb = min(kTileBlocks, nblk - b0);
       if (key >= C::kKStages && !x.wait_warp(&x.k_empty[k.st], k.ph ^ 1)) return;
@@ -1055,6 +1128,24 @@ __device__ void widen_role(const ChunkParams& p, const Ctx<true>& x, int tpt) {
       for (int first = 0; first < nb; first += kGroup) {
         if (!x.wait_warp(&x.raw_full[g.st], g.ph)) return;
         const uint8_t* raw = x.smem + C::kOffRaw + g.st * kGroup * kFp8HeadBlockBytes;
+        // the group's scales, lane: one of its 32 positions
+        const float* mine = reinterpret_cast<const float*>(
+            raw + (lane >> 4) * kFp8HeadBlockBytes + kFp8KScaleOff + (lane & 15) * 4);
+        const bool held = (b0 + first) * kBlockTokens + lane < positions;
+        const uint32_t k_top = __reduce_max_sync(0xffffffffu, held ? __float_as_uint(mine[0]) : 0u);
+        const uint32_t v_top = __reduce_max_sync(
+            0xffffffffu, held ? __float_as_uint(mine[(kFp8VScaleOff - kFp8KScaleOff) / 4]) : 0u);
+        if (!ku.holds(k_top) || !vu.holds(v_top)) {
+          const __half2 k_by = ku.raise(k_top), v_by = vu.raise(v_top);
+#pragma unroll 1
+          for (int b = 0; b < first; ++b) {  // (what this thread wrote itself)
+            scale8(k_tile + b * 2048 + k_lo, k_by);
+            scale8(k_tile + b * 2048 + k_hi, k_by);
+            uint8_t* row = v_tile + (b >> 2) * kRegion;
+            scale8(row + ((((b & 3) * 2) ^ (c & 7)) << 4), v_by);
+            scale8(row + ((((b & 3) * 2 + 1) ^ (c & 7)) << 4), v_by);
+          }
+        }
 #pragma unroll
         for (int i = 0; i < kGroup; ++i) {
           const int b = first + i;  // (past the item's last block: rows that nothing uses)
@@ -1062,11 +1153,12 @@ __device__ void widen_role(const ChunkParams& p, const Ctx<true>& x, int tpt) {
           const uint4 vr =
               *reinterpret_cast<const uint4*>(raw + i * kFp8HeadBlockBytes + kFp8VOff + c * 16);
           const float* fs = reinterpret_cast<const float*>(raw + i * kFp8HeadBlockBytes + kFp8KScaleOff);
-          const __half2 top = __float2half2_rn(fs[tok]);
-          const uint2 sc = make_uint2(as_u32(top), as_u32(__float2half2_rn(fs[tok] - __low2float(top))));
+          const float ks = fs[tok] * ku.up;
+          const __half2 top = __float2half2_rn(ks);
+          const uint2 sc = make_uint2(as_u32(top), as_u32(__float2half2_rn(ks - __low2float(top))));
           const float4* fv = reinterpret_cast<const float4*>(raw + i * kFp8HeadBlockBytes + kFp8VScaleOff);
           const float4 f0 = fv[0], f1 = fv[1], f2 = fv[2], f3 = fv[3];
-          auto pair = [](float x, float y) { return pack_f16(x * kV8Up, y * kV8Up); };
+          auto pair = [&](float x, float y) { return pack_f16(x * vu.up, y * vu.up); };
           const uint4 sl = make_uint4(pair(f0.x, f0.y), pair(f0.z, f0.w), pair(f1.x, f1.y), pair(f1.z, f1.w));
           const uint4 sh = make_uint4(pair(f2.x, f2.y), pair(f2.z, f2.w), pair(f3.x, f3.y), pair(f3.z, f3.w));
           uint4 lo, hi;
@@ -1106,6 +1198,7 @@ __device__ void widen_role(const ChunkParams& p, const Ctx<true>& x, int tpt) {
           *at = w;
         }
       }
+      if (c == 0) *x.unit(key) = make_float2(ku.value(), vu.value());
       fence_async_smem();
       __syncwarp();
       if (lane == 0) {

@@ -8,7 +8,8 @@ same module-level names (the reference's benchmark monkey-patches `_admit`,
     blocks up front (chat.py:117-125) and is rejected if that can never fit
     (chat.py:214-229);
   * idle chats are evicted least-recently-used first under `_cache_lock`
-    until the new message fits, else it is deferred (chat.py:128-146);
+    until the new message fits (its blocks, and a table row of the device
+    tables), else it is deferred (chat.py:128-146);
   * at most one prefill per worker tick (chat.py:232-254), then one batched
     decode step for every active job with a single device sync for sampling
     (chat.py:257-308, :103-107);
@@ -222,32 +223,37 @@ def _evict(chat):
 def _share_history(chat):
     """A forked chat's sequence, before its first message is admitted: the
     resident history of the chat it came from.  Left to the prefill if that
-    chat was evicted, or its ids changed."""
-    parent, chat.parent = chat.parent, None
-    cache = _kv()
-    with _cache_lock:
-        if chat.seq is not None or parent.seq is None:
+    chat was evicted, or its ids changed; to a later call while no table row
+    is free.  Called under _cache_lock."""
+    cache, parent = _kv(), chat.parent
+    if chat.seq is None and parent.seq is not None:
+        if cache.free_row_count() == 0:
             return
         n = min(len(chat.ids), cache.length(parent.seq))
         if cache.free_block_count() == 0:
             n -= n % cache.block_size  # no block for a copy: whole blocks only
-        if n == 0 or parent.ids[:n] != chat.ids[:n]:
-            return
-        chat.seq = cache.fork(parent.seq, n)
-        _resident.append(chat)
+        if n and parent.ids[:n] == chat.ids[:n]:
+            chat.seq = cache.fork(parent.seq, n)
+            _resident.append(chat)
+    chat.parent = None
 
 
 def _make_room(job):
-    if job.chat.parent is not None:
-        _share_history(job.chat)
-    busy = {j.chat for j in active} | {j.chat for j, _ in _mixed} | {job.chat}
+    """Evict idle chats until the job's blocks, and a table row if it has no
+    sequence, are free; False if that takes more than the idle ones."""
+    chat, cache = job.chat, _kv()
+    busy = {j.chat for j in active} | {j.chat for j, _ in _mixed} | {chat}
     with _cache_lock:
-        while _blocks_needed(job) > _kv().free_block_count():
+        while True:
+            if chat.parent is not None:
+                _share_history(chat)
+            if (_blocks_needed(job) <= cache.free_block_count()
+                    and (chat.seq is not None or cache.free_row_count())):
+                return True
             idle = [c for c in _resident if c not in busy]
             if not idle:
                 return False
             _evict(idle[0])
-    return True
 
 
 def _touch(chat):

@@ -152,6 +152,10 @@ class BlockTables:
     def free_block_count(self):
         return len(self._free_blocks)
 
+    def free_row_count(self):
+        """Sequences that can still be started (table rows not in use)."""
+        return len(self._free_rows)
+
     def blocks_needed(self, seq, total_len):
         """Extra blocks `seq` (None for a brand-new sequence) needs to hold total_len tokens."""
         held = len(self._block_tables[seq]) if seq is not None else 0

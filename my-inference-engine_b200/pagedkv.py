@@ -557,6 +557,13 @@ def _check_tables(tables: torch.Tensor, device: torch.device) -> None:
                          f"{tuple(tables.shape)} on {tables.device}")
     if tables.shape[1] > 1 and tables.stride(1) != 1:
         raise ValueError("table rows must be contiguous")
+    if tables.shape[0] > 1 and tables.stride(0) < tables.shape[1]:
+        raise ValueError("table rows overlap")
+
+
+def _pitch(tables: torch.Tensor) -> int:
+    """Row pitch of checked tables (a single row may have any stride)."""
+    return tables.stride(0) if tables.shape[0] > 1 else tables.shape[1]
 
 
 def _chunk_args(q, tables, rows, q_starts, kv_lens, max_kv_len, out, err):
@@ -620,7 +627,7 @@ def paged_chunk(q: torch.Tensor, k_plane: torch.Tensor, v_plane: torch.Tensor,
         ws, ws_bytes, keep = _chunk_workspace(dev.index, B, N, Hq, num_kv_heads, max_kv_len, dev)
         st = lib().pkv_paged_chunk(
             q.data_ptr(), q.stride(0), q.stride(1), k_plane.data_ptr(), v_plane.data_ptr(),
-            k_plane.shape[0], tables.data_ptr(), tables.stride(0), _ptr(rows), q_starts.data_ptr(),
+            k_plane.shape[0], tables.data_ptr(), _pitch(tables), _ptr(rows), q_starts.data_ptr(),
             kv_lens.data_ptr(), max_kv_len, B, N, Hq, num_kv_heads, HEAD_DIM, bool(causal), sm_scale,
             out.data_ptr(), out.stride(0), out.stride(1), ws, ws_bytes, _ptr(err),
             _stream_of(dev.index))
@@ -645,7 +652,7 @@ def paged_chunk_fp8(q: torch.Tensor, pool8: torch.Tensor, tables: torch.Tensor,
         ws, ws_bytes, keep = _chunk_workspace(dev.index, B, N, Hq, Hkv, max_kv_len, dev)
         st = lib().pkv_paged_chunk_fp8(
             q.data_ptr(), q.stride(0), q.stride(1), pool8.data_ptr(), pool8.shape[0],
-            tables.data_ptr(), tables.stride(0), _ptr(rows), q_starts.data_ptr(), kv_lens.data_ptr(),
+            tables.data_ptr(), _pitch(tables), _ptr(rows), q_starts.data_ptr(), kv_lens.data_ptr(),
             max_kv_len, B, N, Hq, Hkv, HEAD_DIM, bool(causal), sm_scale, out.data_ptr(),
             out.stride(0), out.stride(1), ws, ws_bytes, _ptr(err), _stream_of(dev.index))
     if st:
@@ -695,7 +702,7 @@ def move_blocks(pool: torch.Tensor, src: torch.Tensor, dst: torch.Tensor, tables
     _check_tables(tables, pool.device)
     with _OnDevice(pool.device.index):
         st = lib().pkv_move_blocks(_ptr(pool), planes, plane, block, blocks, _ptr(src), _ptr(dst), n,
-                                   _ptr(tables), tables.shape[0], tables.shape[1], tables.stride(0),
+                                   _ptr(tables), tables.shape[0], tables.shape[1], _pitch(tables),
                                    _ptr(err), _stream_of(pool.device.index))
     if st:
         _check(st, "pkv_move_blocks")

@@ -531,6 +531,8 @@ class KVCache(BlockTables):
         (reference kv_cache.py:108-115).  k, v: [B, NUM_KV_HEADS, T, HEAD_DIM];
         slot_mapping is the PagedStep from prepare().  FP8 mode quantises them."""
         step = slot_mapping
+        if k.numel() == 0:  # a packed step of idle rows
+            return
         if self.fp8:
             pagedkv.append_rope_fp8(None, k, v, None, None, None, self.pool8[layer_idx],
                                     self.block_tables, step.rows, step.starts, self.err_flag,

@@ -20,7 +20,7 @@ def _one_row(cuda, fmt):
 @FMT
 def test_one_row_as_a_turned_column(cuda, fmt):
     c = _one_row(cuda, fmt)
-    c["tables"] = c["tables"].T.contiguous().T
+    c["tables"] = c["tables"][0][:, None].T
     assert c["tables"].shape[0] == 1 and c["tables"].stride(0) == 1
     (check8 if fmt == "fp8" else check)(c)
 

@@ -63,7 +63,7 @@ class PagedStep:
 
     @property
     def batch(self) -> int:
-        return len(self.starts_host)
+        return self.rows.shape[0]
 
 
 @dataclass

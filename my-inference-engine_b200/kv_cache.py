@@ -411,7 +411,7 @@ class _PinnedUpload:
         out = self.buf[:n].to(device, non_blocking=True)
         if self.done is None:
             self.done = torch.cuda.Event()
-        self.done.record()
+        self.done.record(torch.cuda.current_stream(out.device))  # the copy's, whichever device is current
         return out
 
 

@@ -988,7 +988,6 @@ size_t pkv_chunk_workspace_size(int32_t batch, int32_t num_tokens, int32_t num_q
   return pkv::chunk_workspace_bytes(batch, num_tokens, num_q_heads, num_kv_heads, max_kv_len);
 }
 
-// What both pool formats check of a packed-chunk call; fills `a` but its pool.
 // The checks and the launch that both pools share.  k_pool, v_pool: the bf16
 // planes, whose tensor maps are made once every argument has passed (nullptr
 // for the FP8 pool, which is read by pointer).

@@ -45,7 +45,9 @@
 // needs no scale of its own; as columns of S the scales cost every softmax
 // thread 96 loads a tile).  f16's range is
 // used up to 2^(8 + 7): base = maximum - 7, so a term keeps 11 bits down to
-// 2^-21 of the largest and is off by at most 2^-32 of it below.
+// 2^-21 of the largest and is off by at most 2^-32 of it below.  (Both operands
+// of a product have one type: with bf16 values a probability is off by up to
+// 2^-8 of itself, as in the other bf16 kernels; in f16 by up to 2^-11.)
 #include <float.h>
 #include <limits.h>
 #include <math.h>
@@ -1540,7 +1542,7 @@ struct ChunkPlan {
 // of up to 60 rows on 3k caches: 30 us, with the short kernel beside it 47 us);
 // and all sequences of a call of at most kSmallRows rows, which is one launch.
 constexpr int kSmallRows = 128;
-constexpr int kShortCtas = 148 * 2;  // CTAs the short kernel is split into, if long enough
+constexpr int kShortCtas = 148 * 2;  // CTAs that long enough caches are split into: two per SM of a B200
 constexpr int kShortMinBlocks = 8;       // per partition: two per warp
 // chunk_kernel: one CTA per SM, fewer where the launch's sizes cannot give
 // each kMinStep.

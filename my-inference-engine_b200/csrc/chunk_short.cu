@@ -19,12 +19,16 @@
 //                                             ldmatrix.trans
 // FP8: fragments are e4m3 pairs widened to f16 in registers (exact), q / 16 as
 // f16, the key's scale applied to its scores and the value's to its
-// probabilities after the row's sum, relative to the largest scale so far (a
-// warp's `cap`): the product then is a f16 of up to 2^15 and is off by at most
-// 2^-32 of the largest term when it falls below f16's normal range, so that
-// thousands of small terms of a long cache keep their weight.  The warps join in shared memory, then
-// the partitions.  Every row's partitions follow from its own length, so a
-// captured call replays for other lengths.
+// probabilities after the row's sum, relative to 4 times the largest scale that
+// the warp has met (its `cap`): the product is a f16 of up to 2^15, off by at
+// most 2^-11 of itself, or 2^-30 of the row's largest probability times the
+// largest value where it falls below f16's normal range, so that thousands of
+// small terms of a long cache keep their weight.  (Values that a row does not
+// see, or that have no weight, raise the cap too.)  bf16: probabilities are
+// rounded to bf16, by at most 2^-8 of themselves, since both operands of a
+// product have the pool's type.
+// The warps join in shared memory, then the partitions.  Every row's partitions
+// follow from its own length, so a captured call replays for other lengths.
 //
 // mma.sync runs at about a tenth of the tensor cores' rate: 32 rows of bf16
 // are bound by it (64 sequences of up to 5 tokens at 6 heads, 347 MB: 83 us
@@ -467,7 +471,10 @@ __device__ __forceinline__ void short_part(const ShortParams& p, const CUtensorM
   }
   if (it.nparts == 1) return;
   // ---- join the partitions, in key order; each CTA of the cluster finishes
-  // every nparts-th row (CTAs past the last partition have left)
+  // every nparts-th row.  CTAs past the last partition have left, or, beside
+  // chunk.cu's kernel, wait for its end: a unit with fewer partitions than the
+  // cluster is then joined behind it (the barrier asks for every thread that
+  // has not left; that kernel waits for nothing here).
   cluster_sync();
   for (int n = it.part + it.nparts * warp; n < rows; n += it.nparts * kWarps) {
     float M = -INFINITY;

@@ -238,47 +238,62 @@ def _share_history(chat):
     chat.parent = None
 
 
-def _make_room(job):
+def _room(job):
     """Evict idle chats until the job's blocks, and a table row if it has no
-    sequence, are free; False if that takes more than the idle ones."""
+    sequence, are free; False if that takes more than the idle ones.  Called
+    under _cache_lock."""
     chat, cache = job.chat, _kv()
     busy = {j.chat for j in active} | {j.chat for j, _ in _mixed} | {chat}
+    while True:
+        if chat.parent is not None:
+            _share_history(chat)
+        if (_blocks_needed(job) <= cache.free_block_count()
+                and (chat.seq is not None or cache.free_row_count())):
+            return True
+        idle = [c for c in _resident if c not in busy]
+        if not idle:
+            return False
+        _evict(idle[0])
+
+
+def _make_room(job):
     with _cache_lock:
-        while True:
-            if chat.parent is not None:
-                _share_history(chat)
-            if (_blocks_needed(job) <= cache.free_block_count()
-                    and (chat.seq is not None or cache.free_row_count())):
-                return True
-            idle = [c for c in _resident if c not in busy]
-            if not idle:
-                return False
-            _evict(idle[0])
+        return _room(job)
+
+
+def _most_recent(chat):
+    if chat in _resident:
+        _resident.remove(chat)
+    _resident.append(chat)
 
 
 def _touch(chat):
     with _cache_lock:
-        if chat in _resident:
-            _resident.remove(chat)
-        _resident.append(chat)
+        _most_recent(chat)
 
 
 def _admit(job):
     """Prefill one job (chat.py:157-185)."""
     chat, model, text = job.chat, job.model, job.text
     cache = _kv()
-    reserve_len = _reserve_len(job)
-    with _cache_lock:  # Chat.fork must not see a message half taken over
+    # In one piece: Chat.fork must not see a message half taken over, and a
+    # Chat.release since _make_room may have given back fewer blocks than the
+    # message now needs (those that another chat shares stay in use).
+    with _cache_lock:
+        if not _room(job):
+            _deferred.append(job)
+            return
+        reserve_len = _reserve_len(job)
         chat.pending.remove(text)
         chat.messages.append(("user", text))
         chat.ids.extend(job.new_ids)
         chat.listeners = [job.out_queue]
         chat.in_progress = ""
-    if chat.seq is None:
-        chat.seq = cache.alloc()
-    prefill_ids = chat.ids[cache.length(chat.seq):]
-    cache.ensure_capacity(chat.seq, reserve_len)
-    _touch(chat)
+        if chat.seq is None:
+            chat.seq = cache.alloc()
+        prefill_ids = chat.ids[cache.length(chat.seq):]
+        cache.ensure_capacity(chat.seq, reserve_len)
+        _most_recent(chat)
     if (MIXED_PREFILL_MIN_TOKENS is not None and active and not _mixed
             and len(prefill_ids) >= MIXED_PREFILL_MIN_TOKENS and hasattr(model, "forward_mixed")):
         _mixed.append((job, prefill_ids))  # runs inside this tick's decode step

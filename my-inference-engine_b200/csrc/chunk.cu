@@ -1539,7 +1539,7 @@ struct ChunkPlan {
 // chunk_kernel as much for few rows as for many (96 sequences of 24 rows on 6k
 // caches: 91 us here, 127 us there), unless the call's sequences have more on
 // average, so that it runs anyway and takes the others along (24 sequences
-// of up to 60 rows on 3k caches: 30 us, with the short kernel beside it 47 us);
+// of up to 60 rows on 3k caches: 32 us, with the short kernel beside it 47 us);
 // and all sequences of a call of at most kSmallRows rows, which is one launch.
 constexpr int kSmallRows = 128;
 constexpr int kShortCtas = 148 * 2;  // CTAs that long enough caches are split into: two per SM of a B200

@@ -87,7 +87,7 @@ def test_ordinary_values(cuda, new, causal):
 
 
 @NEW
-@pytest.mark.parametrize("size", [2.0 ** -20, 3e3, 3e5, 1e20])
+@pytest.mark.parametrize("size", [2.0 ** -20, 3e3, 3e5, 1e20, 1e34])
 def test_values_of_any_size(cuda, new, size):
     def edit(kk, vv):
         vv *= size
